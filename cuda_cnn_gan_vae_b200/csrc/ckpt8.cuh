@@ -1,0 +1,51 @@
+// The 8-bit form of an activation tensor as device functions: a row is cut into blocks of 32 values, a block has one exponent
+// byte b and a signed byte q per value, and q stands for q/64 * 2^(b-127).
+//
+// The step 2^(b-133) is a power of two, so x / step is exact in fp32 and the code is the correctly rounded quotient: no
+// division, and the same codes from any correct implementation.  A value has 8 significant bits, so it is exact in bf16 (and
+// tf32): a tensor-core product over a checkpoint needs no separate scale.  A block of 32 keeps the shared exponent close to
+// the values it serves; the exponents cost one byte in 33.
+#pragma once
+#include <cuda_runtime.h>
+#include <cstdint>
+
+namespace b200 {
+
+constexpr int kCkptBlock = 32;
+__host__ __device__ inline size_t ckpt8_blocks(size_t n) { return (n + kCkptBlock - 1) / kCkptBlock; }
+
+// top: the largest magnitude of the block as the bits of a non-negative float (any NaN compares above infinity)
+__device__ __forceinline__ uint32_t ckpt8_exponent(uint32_t top)
+{
+    if (top >= 0x7f800000u) return 255u;                     // the block reads as NaN
+    const uint32_t e = top >> 23;
+    // magnitudes from 127.5 steps on would round to 128: the next exponent (the largest finite one saturates at 127 instead)
+    const uint32_t up = ((top & 0x7fffffu) >= 0x7f0000u && e >= 1u && e < 254u) ? 1u : 0u;
+    return max(e, 1u) + up;                                  // subnormals share the exponent of the smallest normal numbers
+}
+
+// 2^(133-b) as a product of two factors, each a normal number for every b
+struct CkptScale { float first, second; };
+__device__ __forceinline__ CkptScale ckpt8_scale(uint32_t b)
+{
+    const uint32_t m = max(b, 6u);
+    CkptScale s;
+    s.first = __uint_as_float((260u - m) << 23);             // 2^(133-m), m = 6 .. 255
+    s.second = __uint_as_float((127u + m - b) << 23);        // 2^(m-b)
+    return s;
+}
+
+__device__ __forceinline__ int ckpt8_code(float x, CkptScale s, uint32_t b, bool keep_sign)
+{
+    if (b == 255u) return 0;
+    int q = __float2int_rn(x * s.first * s.second);
+    q = max(-127, min(127, q));
+    if (keep_sign && q == 0 && x < 0.f) q = -1;
+    return q;
+}
+
+// b = 255: 0 * infinity = NaN
+__device__ __forceinline__ float ckpt8_unit(uint32_t b) { return __uint_as_float(b << 23); }
+__device__ __forceinline__ float ckpt8_value(int q, float unit) { return ((float)q * 0.015625f) * unit; }
+
+}  // namespace b200

@@ -68,6 +68,94 @@ def geom(in_z, in_y, in_x, kernel_amount, kernel_x, kernel_y, stride_x, stride_y
     return ConvGeom(in_z, in_y, in_x, kernel_amount, kernel_y, kernel_x, stride_y, stride_x, padding_y, padding_x, out_y, out_x)
 
 
+# ---- layer normalisation and 8-bit checkpoints: activations in fp32, bf16 or fp16, as matrices of rows --------------------------
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _rows(x, name="tensor"):
+    """(type code, rows, values in a row, pitch) of an activation tensor: its first dimension is the rows, the others (dense)
+    are a row.  A 2-D tensor may have any pitch between its rows."""
+    if not (isinstance(x, torch.Tensor) and x.is_cuda and x.dtype in _TYPES and x.dim() >= 1):
+        raise B200Error(2, f"{name} must be an fp32, bf16 or fp16 CUDA tensor")
+    if x.device.index != torch.cuda.current_device():
+        raise B200Error(2, f"{name} is on {x.device}, the current device is cuda:{torch.cuda.current_device()}")
+    rows = x.shape[0]
+    if x.dim() == 2 and x.shape[1]:
+        n, pitch = x.shape[1], x.stride(0)
+        if (x.stride(1) == 1 or n == 1) and (pitch >= n or rows <= 1):
+            return _TYPES[x.dtype], rows, n, max(pitch, n)
+    if not x.is_contiguous():
+        raise B200Error(2, f"{name} must be contiguous, or a matrix of contiguous rows")
+    n = x[0].numel() if rows else int(torch.Size(x.shape[1:]).numel())
+    return _TYPES[x.dtype], rows, n, n
+
+
+def _param(x, n, name):
+    """A contiguous fp32 tensor of n elements on the current device."""
+    _t(x, name)
+    if x.numel() != n:
+        raise B200Error(1, f"{name} must have {n} elements")
+    if x.device.index != torch.cuda.current_device():
+        raise B200Error(2, f"{name} is on {x.device}, the current device is cuda:{torch.cuda.current_device()}")
+    return x
+
+
+def _like(x, name, want, other):
+    """_rows(x), which must have the type, rows and row length of `other`."""
+    got = _rows(x, name)
+    if got[0] != want[0]:
+        raise B200Error(2, f"{name} must have the type of {other}")
+    if got[1:3] != want[1:3]:
+        raise B200Error(1, f"{name} must have the size of {other}")
+    return got
+
+
+class Checkpoint8:
+    """An activation tensor kept in 8 bits a value (see b200_ckpt8_store in include/b200conv.h for the format): `rows` rows of
+    `n` values, 33 bytes for 32 of them.  codes is an int8 tensor [rows, 32 * blocks], exponents a uint8 tensor [rows, blocks],
+    blocks = ceil(n / 32); both belong to the caller."""
+    __slots__ = ("codes", "exponents", "rows", "n")
+
+    def __init__(self, codes, exponents, n):
+        blocks = (n + 31) // 32
+        if not (codes.is_cuda and exponents.is_cuda and codes.dtype == torch.int8 and exponents.dtype == torch.uint8 and
+                codes.is_contiguous() and exponents.is_contiguous()):
+            raise B200Error(2, "codes and exponents must be contiguous int8 and uint8 CUDA tensors")
+        if codes.device != exponents.device or codes.device.index != torch.cuda.current_device():
+            raise B200Error(2, "codes and exponents must be on the current device")
+        if n < 1 or codes.dim() != 2 or exponents.dim() != 2 or codes.shape[1] != 32 * blocks or exponents.shape[1] != blocks or \
+                codes.shape[0] != exponents.shape[0]:
+            raise B200Error(1, "codes must be [rows, 32 * blocks] and exponents [rows, blocks], blocks = ceil(n / 32)")
+        self.codes, self.exponents, self.rows, self.n = codes, exponents, codes.shape[0], n
+
+    @classmethod
+    def empty(cls, rows, n, device="cuda"):
+        blocks = (n + 31) // 32
+        return cls(torch.empty(rows, 32 * blocks, dtype=torch.int8, device=device),
+                   torch.empty(rows, blocks, dtype=torch.uint8, device=device), n)
+
+    def _match(self, x, name):
+        got = _rows(x, name)
+        if got[1] != self.rows or got[2] != self.n:
+            raise B200Error(1, f"{name} must have {self.rows} rows of {self.n} values")
+        return got
+
+    def store(self, x, keep_sign=False):
+        """Keeps x.  keep_sign: a negative value never becomes 0 (the derivative of ReLU and LeakyReLU is then exact)."""
+        kind, rows, n, pitch = self._match(x, "x")
+        _check(load().b200_ckpt8_store(self.codes.data_ptr(), self.exponents.data_ptr(), x.data_ptr(), kind, rows, n, pitch,
+                                       int(keep_sign), _stream()))
+        return self
+
+    def load(self, output):
+        """The kept values into `output` (fp32, bf16 or fp16), which is returned."""
+        kind, rows, n, pitch = self._match(output, "output")
+        _check(load().b200_ckpt8_load(output.data_ptr(), self.codes.data_ptr(), self.exponents.data_ptr(), kind, rows, n, pitch,
+                                      _stream()))
+        return output
+
+
 class CTensorConv:
     """cuda/ctensorconv.cu.h:63-66."""
 
@@ -382,6 +470,13 @@ class CTensorApplyFunc:
 
     @staticmethod
     def Backward(output, z, error, func, leaky_slope=0.1):
+        """output = f'(z) * error.  z may be a Checkpoint8 (of the function's input); output and error then may be fp32, bf16 or fp16."""
+        if isinstance(z, Checkpoint8):
+            kind, rows, n, pitch = z._match(output, "output")
+            e = _like(error, "error", (kind, rows, n), "output")
+            _check(load().b200_ckpt8_activation_backward(output.data_ptr(), z.codes.data_ptr(), z.exponents.data_ptr(), error.data_ptr(),
+                                                         kind, rows, n, pitch, e[3], ACT[func], leaky_slope, _stream()))
+            return
         _t(output), _t(z), _t(error)
         _check(load().b200_activation_backward(_ptr(output), _ptr(z), _ptr(error), z.numel(), ACT[func], leaky_slope, _stream()))
 
@@ -411,6 +506,80 @@ def bn_backward(dy, xhat, ivar, gamma, dgamma, dbeta, create_delta_weight=True):
     _check(load().b200_bn_backward(_ptr(dx), _ptr(dgamma), _ptr(dbeta), _ptr(dy), _ptr(xhat), _ptr(ivar), _ptr(gamma),
                                    dy.shape[0], dy[0].numel(), int(create_delta_weight), _stream()))
     return dx
+
+
+def _workspace(size, given, name):
+    """The caller's workspace tensor, or a fresh one from torch's allocator (which orders its reuse by stream and keeps the
+    workspaces of captured graphs apart)."""
+    if given is None:
+        return torch.empty(max(size, 16), dtype=torch.uint8, device="cuda"), max(size, 16)
+    if not (isinstance(given, torch.Tensor) and given.is_cuda and given.is_contiguous() and given.device.index == torch.cuda.current_device()):
+        raise B200Error(2, f"{name}: the workspace must be a contiguous tensor on the current device")
+    return given, given.numel() * given.element_size()
+
+
+def ln_forward(x, gamma, beta, eps=1e-6, y=None, mean=None, rstd=None, checkpoint=None):
+    """Layer normalisation of every row of x (its first dimension is the rows, the others are normalised together) in fp32,
+    bf16 or fp16 with fp32 parameters.  checkpoint: a Checkpoint8 that receives the normalised values for ln_backward.
+    Returns dict(y, mean, rstd)."""
+    kind, rows, n, pitch = _rows(x, "x")
+    _param(gamma, n, "gamma"), _param(beta, n, "beta")
+    if y is None:
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    mean = torch.empty(rows, device=x.device) if mean is None else _param(mean, rows, "mean")
+    rstd = torch.empty(rows, device=x.device) if rstd is None else _param(rstd, rows, "rstd")
+    y_pitch = _like(y, "y", (kind, rows, n), "x")[3]
+    codes = exponents = None
+    if checkpoint is not None:
+        if checkpoint.rows != rows or checkpoint.n != n:
+            raise B200Error(1, f"the checkpoint must have {rows} rows of {n} values")
+        codes, exponents = checkpoint.codes.data_ptr(), checkpoint.exponents.data_ptr()
+    _check(load().b200_ln_forward(y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), codes, exponents, x.data_ptr(), gamma.data_ptr(),
+                                  beta.data_ptr(), kind, rows, n, pitch, y_pitch, eps, _stream()))
+    return dict(y=y, mean=mean, rstd=rstd)
+
+
+def ln_backward(dy, x, mean, rstd, gamma, dgamma, dbeta, create_delta_weight=True, accumulate=True, dx=None, workspace=None):
+    """Backward pass of ln_forward; returns dx.  x: the input of the forward pass, or the Checkpoint8 it filled (mean is then
+    not read and may be None).  dgamma, dbeta (fp32, n elements) are added to, or written with accumulate=False."""
+    kind, rows, n, dy_pitch = _rows(dy, "dy")
+    _param(gamma, n, "gamma"), _param(rstd, rows, "rstd")
+    if dx is None:
+        dx = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device)
+    dx_pitch = _like(dx, "dx", (kind, rows, n), "dy")[3]
+    codes = exponents = x_ptr = mean_ptr = None
+    x_pitch = n
+    if isinstance(x, Checkpoint8):
+        if x.rows != rows or x.n != n:
+            raise B200Error(1, f"the checkpoint must have {rows} rows of {n} values")
+        codes, exponents = x.codes.data_ptr(), x.exponents.data_ptr()
+    else:
+        x_pitch = _like(x, "x", (kind, rows, n), "dy")[3]
+        x_ptr, mean_ptr = x.data_ptr(), _param(mean, rows, "mean").data_ptr()
+    dg = db = ws = None
+    size = 0
+    if create_delta_weight:
+        dg, db = _param(dgamma, n, "dgamma").data_ptr(), _param(dbeta, n, "dbeta").data_ptr()
+        workspace, size = _workspace(load().b200_ln_backward_workspace(rows, n), workspace, "ln_backward")
+        ws = workspace.data_ptr()
+    _check(load().b200_ln_backward(dx.data_ptr(), dg, db, dy.data_ptr(), x_ptr, mean_ptr, rstd.data_ptr(), codes, exponents, gamma.data_ptr(),
+                                   kind, rows, n, dx_pitch, dy_pitch, x_pitch, int(create_delta_weight), int(accumulate), ws, size, _stream()))
+    return dx
+
+
+def checkpoint_wgrad(dweight, dbias, delta, checkpoint, accumulate=True, workspace=None):
+    """Gradients of a Linear layer whose input was kept in 8 bits: dweight [out x n] (+)= delta^T * values and, unless dbias is
+    None, dbias [out] (+)= sum of delta over the rows.  delta [rows x out] in fp32, bf16 or fp16; the gradients are fp32."""
+    kind, rows, out, pitch = _rows(delta, "delta")
+    if checkpoint.rows != rows:
+        raise B200Error(1, "delta and the checkpoint must have the same number of rows")
+    _param(dweight, out * checkpoint.n, "dweight")
+    if dbias is not None:
+        _param(dbias, out, "dbias")
+    workspace, size = _workspace(load().b200_ckpt8_wgrad_workspace(kind, rows, out, checkpoint.n), workspace, "checkpoint_wgrad")
+    _check(load().b200_ckpt8_wgrad(dweight.data_ptr(), dbias.data_ptr() if dbias is not None else None, int(accumulate), delta.data_ptr(),
+                                   checkpoint.codes.data_ptr(), checkpoint.exponents.data_ptr(), kind, rows, out, checkpoint.n, pitch,
+                                   workspace.data_ptr(), size, _stream()))
 
 
 def vae_forward(mu, logvar, eps, want_kl=True):

@@ -323,6 +323,56 @@ int b200_adam(float *weight, const float *dweight, float *m, float *v, size_t n,
  * replayed from a CUDA graph while the caller refreshes the two numbers before each replay.  No reference counterpart. */
 int b200_adam_prepared(float *weight, const float *dweight, float *m, float *v, size_t n, uint32_t batch_size, double speed,
                        double beta1, double beta2, double epsilon, const double *corrections, void *stream);
+/* ---- layer normalisation and 8-bit activation checkpoints ------------------------------------- */
+
+/* Element types of the entry points of this section.  Activations and errors may be fp32, bf16 or fp16 (all of one call in
+ * the same type); parameters, statistics and gradients of parameters are fp32, and so is all arithmetic in between. */
+enum { B200_F32 = 0, B200_BF16 = 1, B200_F16 = 2 };
+
+/* In this section a tensor is a matrix of `rows` rows of n values; row r starts at element r * pitch (pitch >= n; a dense
+ * tensor [W,Z,Y,X] taken per sample has rows = W, n = pitch = Z*Y*X).  1 <= n <= 2^31 - 64; rows may be 0 (nothing is read, and
+ * gradients that are not accumulated become zero).  Pointers are aligned to the element size, codes to 16 bytes.  Nothing here
+ * uses the library's scratch arena: a call that needs scratch takes it from the caller (16-byte aligned, at least as many bytes
+ * as its ..._workspace() says for the same sizes; the contents need not be kept between calls), so calls on several streams and
+ * captured graphs are independent as long as their workspaces are. */
+
+/* Layer normalisation of every row over its n values: y = gamma * xhat + beta, xhat = (x - mean) * rstd,
+ * rstd = 1 / sqrt(variance + eps), the variance being the row's own (divided by n).  mean and rstd [rows] may be NULL.  codes
+ * and exponents (both or neither): xhat is kept as an 8-bit checkpoint for b200_ln_backward.  y may be x. */
+int b200_ln_forward(void *y, float *mean, float *rstd, int8_t *codes, uint8_t *exponents, const void *x, const float *gamma,
+                    const float *beta, int type, int rows, size_t n, size_t x_pitch, size_t y_pitch, float eps, void *stream);
+/* Backward pass: with g = dy * gamma, dx = rstd * (g - mean(g) - xhat * mean(g * xhat)); create_delta_weight != 0 also forms
+ * dgamma (+)= sum over rows of dy * xhat and dbeta (+)= sum over rows of dy (accumulate != 0: added to what is there).  xhat
+ * comes from x with mean and rstd, or (x NULL) from the checkpoint; mean is then not read.  dx may be dy or x.  The workspace
+ * is used only with create_delta_weight. */
+size_t b200_ln_backward_workspace(int rows, size_t n);
+int b200_ln_backward(void *dx, float *dgamma, float *dbeta, const void *dy, const void *x, const float *mean, const float *rstd,
+                     const int8_t *codes, const uint8_t *exponents, const float *gamma, int type, int rows, size_t n,
+                     size_t dx_pitch, size_t dy_pitch, size_t x_pitch, int create_delta_weight, int accumulate, void *workspace,
+                     size_t workspace_bytes, void *stream);
+
+/* A tensor kept in 8 bits.  A row is cut into blocks of 32 values (the last one may be shorter); a block has one exponent byte b
+ * and a signed byte q per value, and q stands for q/64 * 2^(b-127).  codes: [rows][32 * blocks] bytes, exponents:
+ * [rows][blocks] bytes, blocks = ceil(n / 32): 33 bytes for 32 values.  b is the exponent field of the block's largest magnitude
+ * (at least 1), one more where that value would round to 128 (not past 254, where it saturates at 127); q is rounded to
+ * nearest, ties to even.  A value is off by at most half a step, 1/127 of the largest magnitude of its block (a whole step where
+ * it saturates).  A block that holds an infinity or a NaN reads as NaN.  keep_sign != 0: a negative value never gets q = 0
+ * but -1 (off by less than a step), so that the derivatives of ReLU and LeakyReLU at the kept values are those at the tensor's. */
+int b200_ckpt8_store(int8_t *codes, uint8_t *exponents, const void *x, int type, int rows, size_t n, size_t x_pitch, int keep_sign,
+                     void *stream);
+/* Reads the values back (exact in fp32 and bf16; in fp16 rounded once, beyond its range the largest finite number). */
+int b200_ckpt8_load(void *out, const int8_t *codes, const uint8_t *exponents, int type, int rows, size_t n, size_t out_pitch,
+                    void *stream);
+/* b200_activation_backward for a function layer whose input was kept in 8 bits: out = f'(value) * error.  out may be error. */
+int b200_ckpt8_activation_backward(void *out, const int8_t *codes, const uint8_t *exponents, const void *error, int type, int rows,
+                                   size_t n, size_t out_pitch, size_t error_pitch, int func, double leaky_slope, void *stream);
+/* Gradients of a Linear layer (netlayer/cnetlayerlinear.cu.h:415) whose input [rows][in] was kept in 8 bits:
+ * dweight[out][in] (+)= sum over rows of delta[row][out] * value[row][in], dbias[out] (+)= sum over rows of delta[row][out]
+ * (dbias may be NULL). */
+size_t b200_ckpt8_wgrad_workspace(int type, int rows, int out, size_t in);
+int b200_ckpt8_wgrad(float *dweight, float *dbias, int accumulate, const void *delta, const int8_t *codes, const uint8_t *exponents,
+                     int type, int rows, int out, size_t in, size_t delta_pitch, void *workspace, size_t workspace_bytes, void *stream);
+
 /* ---- helpers of the diffusion model and the drop-out layer ------------------------------------- */
 
 /* CTensorMath::SetTimeStep (cuda/ctensormath.cu.h:3029-3096; the forward pass of CNetLayerTimeEmbedding,

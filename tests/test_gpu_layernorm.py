@@ -1,0 +1,284 @@
+"""Layer normalisation on the GPU against the formulas in 64 bits."""
+import numpy as np
+import pytest
+import torch
+
+from tests import ckpt8_util as cu
+
+pytestmark = pytest.mark.gpu
+KINDS = ["float32", "bfloat16", "float16"]
+# rows x n: a single value, single rows, blocks that end early, odd lengths, the borders of the kernels' forms, long rows
+SIZES = [(1, 1), (5, 2), (3, 31), (4, 32), (7, 33), (1, 256), (129, 100), (37, 1021), (300, 1024), (20, 1025), (9, 4099), (33, 8192),
+         (5, 8200), (3, 16384), (4, 20001), (2, 65536), (3, 131072), (2, 300007)]
+
+
+@pytest.fixture(autouse=True)
+def ops():
+    from cuda_cnn_gan_vae_b200 import ops
+    return ops
+
+
+def make(rows, n, kind, seed=0, offset=0.5):
+    r = np.random.default_rng(seed + rows * 7919 + n)
+    t = getattr(torch, kind)
+    x = torch.from_numpy((r.normal(offset, 1.0, (rows, n)) * r.uniform(0.5, 2, (rows, 1))).astype(np.float32)).to(t).cuda()
+    dy = torch.from_numpy(r.normal(0, 1, (rows, n)).astype(np.float32)).to(t).cuda()
+    gamma = torch.from_numpy(r.normal(1, 0.3, n).astype(np.float32)).cuda()
+    beta = torch.from_numpy(r.normal(0, 0.3, n).astype(np.float32)).cuda()
+    return x, dy, gamma, beta
+
+
+def host(t):
+    return t.double().cpu().numpy()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows,n", SIZES)
+def test_forward(ops, rows, n, kind):
+    x, _, gamma, beta = make(rows, n, kind)
+    got = ops.ln_forward(x, gamma, beta, 1e-5)
+    ops.stream_status()
+    args = (host(x), host(gamma), host(beta), float(np.float32(1e-5)))
+    y, mu, r, _ = cu.ln_forward(*args)
+    ey, em, er, _ = cu.ln_forward_bounds(*args, kind)
+    cu.within(host(got["mean"]), mu, em, "mean")
+    cu.within(host(got["rstd"]), r, er, "rstd")
+    cu.within(host(got["y"]), y, ey, "y")
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows,n", SIZES)
+def test_forward_checkpoint(ops, rows, n, kind):
+    """The kept values are the normalised rows to half a step of their block; the outputs are those without a checkpoint."""
+    x, _, gamma, beta = make(rows, n, kind, 1)
+    plain = ops.ln_forward(x, gamma, beta, 1e-5)
+    c = ops.Checkpoint8.empty(rows, n)
+    got = ops.ln_forward(x, gamma, beta, 1e-5, checkpoint=c)
+    ops.stream_status()
+    assert all(torch.equal(got[k], plain[k]) for k in got)
+    args = (host(x), host(gamma), host(beta), float(np.float32(1e-5)))
+    xh = cu.ln_forward(*args)[3]
+    exh = cu.ln_forward_bounds(*args, kind)[3]
+    b = c.exponents.cpu().numpy()
+    step = np.repeat(np.ldexp(1.0, b.astype(np.int64) - 133), 32, axis=1)[:, :n]
+    cu.within(cu.decode(c.codes.cpu().numpy(), b, n), xh, 0.5 * step + exh, "kept")
+    # the exponent is that of the block's largest value (or a neighbour's where the largest value is at a border)
+    lo, hi = cu.encode(np.maximum(np.abs(xh) * (1 - 1e-3) - exh, 0))[1], cu.encode(np.abs(xh) * (1 + 1e-3) + exh)[1]
+    assert (np.minimum(lo, hi) <= b).all() and (b <= hi).all()
+    assert not c.codes.cpu().numpy().reshape(rows, -1)[:, n:].any()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("rows,n", SIZES)
+def test_backward(ops, rows, n, kind, accumulate):
+    x, dy, gamma, beta = make(rows, n, kind, 2)
+    mu = x.double().mean(1).float()
+    rstd = (1 / (x.double().var(1, correction=0) + 1e-5).sqrt()).float()
+    dgamma, dbeta = (torch.full((n,), 3.0, device="cuda") for _ in range(2))
+    dx = ops.ln_backward(dy, x, mu, rstd, gamma, dgamma, dbeta, accumulate=accumulate)
+    ops.stream_status()
+    xh = (host(x) - host(mu)[:, None]) * host(rstd)[:, None]
+    want = cu.ln_backward(host(dy), xh, host(rstd), host(gamma))
+    edx, edg, edb = cu.ln_backward_bounds(host(dy), xh, host(rstd), host(gamma), kind)
+    base = 3.0 if accumulate else 0.0
+    cu.within(host(dx), want[0], edx, "dx")
+    cu.within(host(dgamma), want[1] + base, edg + cu.U * np.abs(want[1] + base), "dgamma")
+    cu.within(host(dbeta), want[2] + base, edb + cu.U * np.abs(want[2] + base), "dbeta")
+    # without the parameters' gradients: the same dx, nothing else written
+    keep = dgamma.clone(), dbeta.clone()
+    again = ops.ln_backward(dy, x, mu, rstd, gamma, dgamma, dbeta, create_delta_weight=False)
+    assert torch.equal(again, dx) and torch.equal(dgamma, keep[0]) and torch.equal(dbeta, keep[1])
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows,n", SIZES)
+def test_backward_from_checkpoint(ops, rows, n, kind):
+    x, dy, gamma, beta = make(rows, n, kind, 3)
+    c = ops.Checkpoint8.empty(rows, n)
+    got = ops.ln_forward(x, gamma, beta, 1e-5, checkpoint=c)
+    dgamma, dbeta = (torch.zeros(n, device="cuda") for _ in range(2))
+    dx = ops.ln_backward(dy, c, None, got["rstd"], gamma, dgamma, dbeta)
+    ops.stream_status()
+    xh = cu.decode(c.codes.cpu().numpy(), c.exponents.cpu().numpy(), n)
+    want = cu.ln_backward(host(dy), xh, host(got["rstd"]), host(gamma))
+    edx, edg, edb = cu.ln_backward_bounds(host(dy), xh, host(got["rstd"]), host(gamma), kind)
+    cu.within(host(dx), want[0], edx, "dx")
+    cu.within(host(dgamma), want[1], edg + cu.U * np.abs(want[1]), "dgamma")
+    cu.within(host(dbeta), want[2], edb + cu.U * np.abs(want[2]), "dbeta")
+
+
+@pytest.mark.parametrize("n", [24, 1000, 8192, 40000])
+def test_pitched_rows_and_untouched_surroundings(ops, n):
+    """Rows inside wider matrices, starting at odd elements: nothing outside the rows is read into the result or written."""
+    rows = 6
+    for kind in KINDS:
+        t = getattr(torch, kind)
+        x, dy, gamma, beta = make(rows, n, kind, 4)
+        wide = [torch.full((rows, n + 7 + k), float("nan"), dtype=t, device="cuda") for k in range(4)]
+        vx, vdy, vy, vdx = (w[:, 3:3 + n] for w in wide)
+        vx.copy_(x), vdy.copy_(dy)
+        want = ops.ln_forward(x, gamma, beta, 1e-5)
+        got = ops.ln_forward(vx, gamma, beta, 1e-5, y=vy)
+        cu.within(host(got["y"]), host(want["y"]), cu.ln_forward_bounds(host(x), host(gamma), host(beta), 1e-5, kind)[0] * 2, "y")
+        dg, db, dg2, db2 = (torch.zeros(n, device="cuda") for _ in range(4))
+        ops.ln_backward(dy, x, want["mean"], want["rstd"], gamma, dg, db)
+        ops.ln_backward(vdy, vx, want["mean"], want["rstd"], gamma, dg2, db2, dx=vdx)
+        ops.stream_status()
+        xh = (host(x) - host(want["mean"])[:, None]) * host(want["rstd"])[:, None]
+        bounds = cu.ln_backward_bounds(host(dy), xh, host(want["rstd"]), host(gamma), kind)
+        cu.within(host(vdx), cu.ln_backward(host(dy), xh, host(want["rstd"]), host(gamma))[0], bounds[0], "dx")
+        cu.within(host(dg2), host(dg), 2 * bounds[1], "dgamma")
+        cu.within(host(db2), host(db), 2 * bounds[2], "dbeta")
+        for w in wide[2:]:
+            assert torch.isnan(w[:, :3]).all() and torch.isnan(w[:, 3 + n:]).all()
+
+
+@pytest.mark.parametrize("n", [100, 1024, 8192, 20000, 300000])
+def test_in_place(ops, n):
+    x, dy, gamma, beta = make(5, n, "float32", 5)
+    want = ops.ln_forward(x, gamma, beta, 1e-5)
+    dg, db, dg2, db2 = (torch.zeros(n, device="cuda") for _ in range(4))
+    dx = ops.ln_backward(dy, x, want["mean"], want["rstd"], gamma, dg, db)
+    for target in ("dy", "x"):
+        a, b = dy.clone(), x.clone()
+        dg2.zero_(), db2.zero_()
+        out = a if target == "dy" else b
+        ops.ln_backward(a, b, want["mean"], want["rstd"], gamma, dg2, db2, dx=out)
+        assert torch.equal(out, dx) and torch.equal(dg, dg2) and torch.equal(db, db2)
+    y = x.clone()
+    assert torch.equal(ops.ln_forward(y, gamma, beta, 1e-5, y=y)["y"], want["y"])
+    ops.stream_status()
+
+
+def test_constant_rows_infinities_and_nan(ops):
+    """A constant row has no deviation (y = beta); a row with an infinity or a NaN gives NaN, its neighbours are untouched."""
+    for n in (40, 1000, 9000):
+        x, dy, gamma, beta = make(6, n, "float32", 6)
+        x[1] = 4.0
+        x[3, n // 2] = float("inf")
+        x[4, n - 1] = float("nan")
+        c = ops.Checkpoint8.empty(6, n)
+        got = ops.ln_forward(x, gamma, beta, 1e-5, checkpoint=c)
+        ops.stream_status()
+        assert torch.equal(got["y"][1], beta)
+        assert torch.isnan(got["y"][3]).all() and torch.isnan(got["y"][4]).all()
+        for k in (0, 2, 5):
+            alone = ops.ln_forward(x[k:k + 1], gamma, beta, 1e-5)
+            assert torch.equal(alone["y"][0], got["y"][k])
+        kept = c.load(torch.empty(6, n, device="cuda"))
+        assert torch.isnan(kept[3]).all() and torch.isnan(kept[4]).all() and (kept[1] == 0).all()
+        assert torch.isfinite(kept[[0, 2, 5]]).all()
+
+
+def test_large_mean(ops):
+    """The variance comes from deviations about the mean: a mean of 1000 deviations costs no more than its own rounding."""
+    x, _, gamma, beta = make(8, 5000, "float32", 7, offset=0.0)
+    x += 1000.0
+    args = (host(x), host(gamma), host(beta), 1e-5)
+    got = ops.ln_forward(x, gamma, beta, 1e-5)
+    cu.within(host(got["y"]), cu.ln_forward(*args)[0], cu.ln_forward_bounds(*args, "float32")[0], "y")
+    cu.within(host(got["rstd"]), cu.ln_forward(*args)[2], cu.ln_forward_bounds(*args, "float32")[2], "rstd")
+
+
+@pytest.mark.parametrize("n", [48, 3000])
+def test_gradient_against_differences(ops, n):
+    """Directional derivative of sum(w * y) by central differences of the 64-bit forward formula."""
+    rows, h = 4, 1e-4
+    x, w, gamma, beta = make(rows, n, "float32", 8)
+    got = ops.ln_forward(x, gamma, beta, 1e-5)
+    dg, db = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+    dx = ops.ln_backward(w, x, got["mean"], got["rstd"], gamma, dg, db)
+    r = np.random.default_rng(3)
+    f = lambda X, G, B: float((cu.ln_forward(X, G, B, 1e-5)[0] * host(w)).sum())  # noqa: E731
+    X, G, B = host(x), host(gamma), host(beta)
+    for grad, move in ((host(dx), 0), (host(dg), 1), (host(db), 2)):
+        d = r.normal(0, 1, grad.shape)
+        args = [[X, G, B], [X, G, B]]
+        args[0][move] = args[0][move] + h * d
+        args[1][move] = args[1][move] - h * d
+        want = (f(*args[0]) - f(*args[1])) / (2 * h)
+        # the differences are off by h^2/6 times a third derivative (of order |w||d|^3 r^3 per value: below 1e-6 of the sum
+        # of magnitudes), the gradient by rounding (about (n/32 + 20) u of the same sum)
+        assert abs(want - (grad * d).sum()) <= (1e-6 + (n / 32 + 20) * cu.U) * 10 * np.abs(grad * d).sum() + 1e-6, move
+
+
+def test_runs_repeat_bit_for_bit(ops):
+    for rows, n in ((4000, 700), (50, 30000)):
+        x, dy, gamma, beta = make(rows, n, "bfloat16", 9)
+        got = ops.ln_forward(x, gamma, beta)
+        outs = []
+        for _ in range(3):
+            dg, db = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+            outs.append((ops.ln_backward(dy, x, got["mean"], got["rstd"], gamma, dg, db), dg, db))
+        for o in outs[1:]:
+            assert all(torch.equal(a, b) for a, b in zip(o, outs[0]))
+
+
+def test_no_rows(ops):
+    gamma = torch.ones(33, device="cuda")
+    empty = torch.empty(0, 33, device="cuda")
+    got = ops.ln_forward(empty, gamma, gamma)
+    assert got["y"].shape == (0, 33)
+    dg, db = torch.full((33,), 2.0, device="cuda"), torch.full((33,), 2.0, device="cuda")
+    ops.ln_backward(empty, empty, got["mean"], got["rstd"], gamma, dg, db)
+    assert (dg == 2).all() and (db == 2).all()
+    ops.ln_backward(empty, empty, got["mean"], got["rstd"], gamma, dg, db, accumulate=False)
+    ops.stream_status()
+    assert (dg == 0).all() and (db == 0).all()
+
+
+def test_captured_and_replayed_on_two_streams(ops):
+    """Two captured passes with workspaces of their own, replayed at the same time on two streams."""
+    graphs, results, wants = [], [], []
+    for k in range(2):
+        x, dy, gamma, beta = make(700, 900 + 64 * k, "float32", 10 + k)
+        n = x.shape[1]
+        dg, db = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+        mean, rstd, y, dx = torch.empty(700, device="cuda"), torch.empty(700, device="cuda"), torch.empty_like(x), torch.empty_like(x)
+
+        def step():
+            ops.ln_forward(x, gamma, beta, y=y, mean=mean, rstd=rstd)
+            ops.ln_backward(dy, x, mean, rstd, gamma, dg, db, accumulate=False, dx=dx)
+        step()
+        torch.cuda.synchronize()
+        wants.append([t.clone() for t in (y, dx, dg, db)])
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            step()
+        graphs.append(g)
+        results.append((y, dx, dg, db, x, dy, gamma, beta, mean, rstd))
+        for t in (y, dx, dg, db):
+            t.zero_()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(20):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for r, w in zip(results, wants):
+        assert all(torch.equal(a, b) for a, b in zip(r, w))
+
+
+def test_refusals(ops):
+    x, dy, gamma, beta = make(4, 64, "float32", 11)
+    B = ops.B200Error
+    for bad in (lambda: ops.ln_forward(x.double(), gamma, beta),
+                lambda: ops.ln_forward(x.cpu(), gamma, beta),
+                lambda: ops.ln_forward(x.t(), gamma, beta),
+                lambda: ops.ln_forward(x, gamma[:-1], beta),
+                lambda: ops.ln_forward(x, gamma.half(), beta),
+                lambda: ops.ln_forward(x, gamma, beta, eps=0.0),
+                lambda: ops.ln_forward(x, gamma, beta, eps=float("nan")),
+                lambda: ops.ln_forward(x, gamma, beta, y=torch.empty(4, 65, device="cuda")),
+                lambda: ops.ln_forward(x, gamma, beta, y=torch.empty(4, 64, device="cuda", dtype=torch.half)),
+                lambda: ops.ln_forward(x, gamma, beta, checkpoint=ops.Checkpoint8.empty(4, 63)),
+                lambda: ops.ln_forward(x.expand(4, 64)[:1].expand(4, 64), gamma, beta),
+                lambda: ops.ln_backward(dy, x, gamma[:3], gamma[:4], gamma, gamma.clone(), beta.clone()),
+                lambda: ops.ln_backward(dy, x, gamma[:4], gamma[:4], gamma, gamma.clone(), None),
+                lambda: ops.ln_backward(dy, x, gamma[:4], gamma[:4], gamma, gamma.clone(), beta.clone(), workspace=torch.empty(16, device="cuda")),
+                lambda: ops.ln_backward(dy, ops.Checkpoint8.empty(3, 64), None, gamma[:4], gamma, gamma.clone(), beta.clone())):
+        with pytest.raises(B):
+            bad()
+    ops.stream_status()
