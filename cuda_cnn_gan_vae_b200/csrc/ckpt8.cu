@@ -61,7 +61,7 @@ int check_ckpt8(const void *codes, const void *exponents)
 
 int check_rows(int rows, size_t n)
 {
-    if (rows < 0) return fail(B200_E_SHAPE, "negative number of rows");
+    if (rows < 0 || (size_t)rows > kMaxRow) return fail(B200_E_SHAPE, "the number of rows must be 0 to %zu", kMaxRow);
     if (n == 0 || n > kMaxRow) return fail(B200_E_SHAPE, "a row must have 1 to %zu values", kMaxRow);
     return B200_OK;
 }

@@ -4,6 +4,8 @@
 #include "types.cuh"
 #include "ckpt8.cuh"
 #include "norm.h"
+#include "kernels.h"
+#include "tc_ptx.cuh"
 
 namespace b200 {
 
@@ -59,6 +61,629 @@ __global__ void __launch_bounds__(256) ckpt8_wgrad_simt_kernel(float *dweight, f
     }
 }
 
+// ---- tensor-core form ---------------------------------------------------------------------------------------------------
+//
+// A CTA pair computes 256 x 256 outputs: 256 of delta's columns (128 per CTA) by 256 of the input's (128 decoded by each CTA and
+// read by both), one 256-row MMA per 16 rows of the batch, accumulated in tensor memory.  Both operands are MN-major, so a
+// row of delta or of the checkpoint becomes a row of the shared-memory tile as it lies in memory: no transposition anywhere.
+//   * The kept values have 8 significant bits and are exact in bf16 with their scale.  delta is cut into PARTS pieces of 8 bits (bf16 1,
+//     fp16 2, fp32 3, in either tensor-core mode), each exact, so every product is exact and the only
+//     roundings are those of the fp32 accumulator.  The tensor core truncates its sums, a bias that grows with their number:
+//     after kChunk stages the accumulator is added to the output (rounded to nearest) and starts again from zero.  8192 rows at
+//     a stretch were off by 2.5e-6 of the result, chunks of 2048 are by 4e-7.
+//   * One warp brings the codes and delta in by TMA (bf16 straight into the operand tile); sixteen warps decode and split from
+//     shared memory into a ring of operand stages (five instructions for two values, once per pair and tile).  A first form
+//     in which those warps loaded from global memory themselves, into registers three stages ahead, took 1030 us at
+//     8192 rows, 4096 x 4096: 340 instructions a warp and stage, half its time waiting for loads.
+//   * The grid is one pair per two SMs.  Whole tiles go round the pairs; what is left over (or everything, where there are
+//     fewer tiles than pairs) is split along the batch into units that write partial tiles, joined by a second
+//     kernel in the order of the units.  No atomics: the result does not depend on scheduling.
+constexpr int kPairTile = 256;                     // outputs of a pair in both directions
+constexpr int kEpilogueWarps = 4, kConverterWarps = 16;
+constexpr int kConverters = kConverterWarps * 32;
+constexpr int kTcThreads = (kEpilogueWarps + kConverterWarps + 2) * 32;
+constexpr int kPitch = 36;                         // floats in a row of the epilogue's transposition buffer
+constexpr size_t kUnitFloats = (size_t)kPairTile * kPairTile + kPairTile;      // a partial tile and its partial bias gradient
+
+struct WgradParams {
+    float *dweight, *dbias;
+    const uint8_t *exponents;
+    int rows, out, accumulate, vector_out;
+    size_t in, blocks;
+    int tiles_n, steps, chunk_steps, pairs, waves, first_tail, tail_units, splits;
+    float *partial;
+    unsigned *status;
+    uint32_t idesc;
+};
+
+// One chunk of a tile: `first` starts its output, later ones add to it; `last` ends it.
+struct WorkItem { int mt, nt, begin, steps, unit; bool first, last; };
+
+// The work items of a pair in order: the chunks of its whole tiles, then those of its tail unit.
+struct ItemCursor {
+    WorkItem w;
+    int turn, end;
+    __device__ __forceinline__ bool open(const WgradParams &p, int pair)
+    {
+        int tile;
+        w.begin = 0; end = p.steps; w.unit = -1;
+        if (turn < p.waves) {
+            tile = pair + turn * p.pairs;
+        } else {
+            if (turn > p.waves || pair >= p.tail_units) return false;
+            const int split = pair % p.splits;
+            tile = p.first_tail + pair / p.splits;
+            w.begin = (int)((long long)p.steps * split / p.splits);
+            end = (int)((long long)p.steps * (split + 1) / p.splits);
+            if (p.splits > 1) w.unit = pair;
+        }
+        w.mt = tile / p.tiles_n;
+        w.nt = tile - w.mt * p.tiles_n;
+        w.first = true;
+        return chunk(p);
+    }
+    __device__ __forceinline__ bool chunk(const WgradParams &p)
+    {
+        w.steps = min(p.chunk_steps, end - w.begin);
+        w.last = w.begin + w.steps == end;
+        return true;
+    }
+    __device__ __forceinline__ bool start(const WgradParams &p, int pair) { turn = 0; return open(p, pair); }
+    __device__ __forceinline__ bool next(const WgradParams &p, int pair)
+    {
+        if (w.last) { turn++; return open(p, pair); }
+        w.begin += w.steps;
+        w.first = false;
+        return chunk(p);
+    }
+};
+
+// Walks the stages of all work items of a pair in order.
+struct StageCursor {
+    ItemCursor i;
+    int step;
+    bool valid;
+    __device__ __forceinline__ void start(const WgradParams &p, int pair) { step = 0; valid = i.start(p, pair); }
+    __device__ __forceinline__ bool ends_tile() const { return i.w.last && step + 1 == i.w.steps; }
+    __device__ __forceinline__ void next(const WgradParams &p, int pair)
+    {
+        if (++step == i.w.steps) { step = 0; valid = i.next(p, pair); }
+    }
+};
+
+// Eight codes with the scale of their block -> eight bf16 values.  The bytes 0x43, u form the bf16 bits of 128 + (u & 127) and
+// of 128 + (u & 128); their difference is the signed code, exact, and so is its product with the power of two.
+__device__ __forceinline__ uint4 decode8(uint2 codes, uint32_t exponent)
+{
+    const uint32_t f = __float_as_uint(ckpt8_unit(exponent) * 0.015625f);      // 2^(b-133), exact in bf16
+    const uint32_t scale = __byte_perm(f, 0, 0x3232);
+    uint32_t v[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t t = __byte_perm(i < 2 ? codes.x : codes.y, 0x43434343u, i & 1 ? 0x4342 : 0x4140);
+        const uint32_t a = t & 0xff7fff7fu, b = t & 0xff80ff80u;
+        __nv_bfloat162 q = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&a), *reinterpret_cast<const __nv_bfloat162 *>(&b));
+        q = __hmul2(q, *reinterpret_cast<const __nv_bfloat162 *>(&scale));
+        v[i] = *reinterpret_cast<uint32_t *>(&q);
+    }
+    return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
+// x = piece 0 + piece 1 + ..., each the upper 16 bits of what is left: exact.  An infinity has no remainder; a NaN stays one in
+// the second piece.
+__device__ __forceinline__ float remainder_of(float x, float &upper)
+{
+    upper = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+    return fabsf(x) == INFINITY ? 0.f : x - upper;
+}
+__device__ __forceinline__ uint32_t upper_halves(float a, float b) { return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632); }
+
+// eight values of delta from two (fp32) or one 16-byte vector
+template <typename T> __device__ __forceinline__ void unpack8(uint4 lo, uint4 hi, float *f);
+template <> __device__ __forceinline__ void unpack8<float>(uint4 lo, uint4 hi, float *f)
+{
+    const uint32_t u[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+    for (int i = 0; i < 8; i++) f[i] = __uint_as_float(u[i]);
+}
+template <> __device__ __forceinline__ void unpack8<__nv_bfloat16>(uint4 lo, uint4, float *f)
+{
+    const uint32_t u[4] = {lo.x, lo.y, lo.z, lo.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) { f[2 * i] = __uint_as_float(u[i] << 16); f[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u); }
+}
+template <> __device__ __forceinline__ void unpack8<__half>(uint4 lo, uint4, float *f)
+{
+    const uint32_t u[4] = {lo.x, lo.y, lo.z, lo.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&u[i]));
+        f[2 * i] = h.x; f[2 * i + 1] = h.y;
+    }
+}
+
+// Rows of the batch in a stage, and the two rings: raw (codes as stored, and delta where it has to be split) and operands.
+template <typename T, int PARTS> struct TcShape {
+    static constexpr int kRows = PARTS == 1 ? 64 : 32;
+    static constexpr uint32_t kOperand = kRows * 256u;                        // bytes of a 128-wide bf16 tile
+    static constexpr uint32_t kStage = (PARTS + 1) * kOperand;
+    static constexpr int kStages = PARTS == 1 ? 5 : PARTS == 2 ? 4 : 3;
+    static constexpr uint32_t kCodes = kRows * 128u;
+    static constexpr uint32_t kRaw = kCodes + (PARTS == 1 ? 0u : kRows * 128u * (uint32_t)sizeof(T));
+    static constexpr int kRaws = PARTS == 1 ? 4 : PARTS == 2 ? 8 : 5;
+    static constexpr uint32_t kRing = kStages * kStage;                       // bytes before the raw ring
+    static constexpr int kCodesEach = kRows / 4;                              // codes per converter thread: 16 or 8
+    static constexpr int kChunk = (PARTS == 1 ? 2048 : 1024) / kRows;         // stages after which the accumulator is emptied
+};
+constexpr int kAhead = 4;                                                     // exponents are loaded this many stages ahead
+constexpr int kAccumulators = 2;                                              // the epilogue of an item overlaps the products of the next
+constexpr size_t kRingBytes = 200704;
+constexpr size_t kTcSmem = 1024 + kRingBytes + kEpilogueWarps * 32 * kPitch * 4 + kConverterWarps * 128 * 4 + 512;
+
+template <typename T, int PARTS>
+__global__ void __launch_bounds__(kTcThreads, 1)
+ckpt8_wgrad_tc_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_constant__ CUtensorMap delta_map, const __grid_constant__ WgradParams p)
+{
+    using S = TcShape<T, PARTS>;
+    static_assert(S::kRing + S::kRaws * S::kRaw <= kRingBytes, "rings");
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    float *turn = reinterpret_cast<float *>(smem + kRingBytes);               // epilogue: 32 x 32 per warp
+    float *bias_sums = turn + kEpilogueWarps * 32 * kPitch;                   // converters: [warp][128]
+    uint64_t *bars = reinterpret_cast<uint64_t *>(bias_sums + kConverterWarps * 128);
+    const uint32_t bar_base = ptx::smem_u32(bars);
+    auto full_bar = [&](int s) { return bar_base + 8u * s; };                 // operand stage: a CTA's own converters (and its delta tile)
+    auto empty_bar = [&](int s) { return bar_base + 8u * (S::kStages + s); };
+    auto peer_bar = [&](int s) { return bar_base + 8u * (2 * S::kStages + s); };       // in the leader: the peer's stage is full
+    auto raw_full_bar = [&](int s) { return bar_base + 8u * (3 * S::kStages + s); };
+    auto raw_empty_bar = [&](int s) { return bar_base + 8u * (3 * S::kStages + S::kRaws + s); };
+    auto tfull_bar = [&](int a) { return bar_base + 8u * (3 * S::kStages + 2 * S::kRaws + a); };
+    auto tempty_bar = [&](int a) { return bar_base + 8u * (3 * S::kStages + 2 * S::kRaws + 2 + a); };
+    constexpr int kBars = 3 * S::kStages + 2 * S::kRaws + 4;
+    static_assert(kBars * 8 + 8 <= 512, "barriers");
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + kBars);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)ptx::cluster_ctarank(), pair = (int)(blockIdx.x >> 1);
+    constexpr int kIssuer = kEpilogueWarps + kConverterWarps, kLoader = kIssuer + 1;
+    constexpr bool kDirect = PARTS == 1;                                      // delta goes straight into the operand stage
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S::kStages; s++) {
+            ptx::mbar_init(full_bar(s), kConverterWarps + (kDirect ? 1 : 0));
+            ptx::mbar_init(empty_bar(s), 1 + (kDirect ? kConverterWarps : 0));
+            ptx::mbar_init(peer_bar(s), 1);
+        }
+        for (int s = 0; s < S::kRaws; s++) { ptx::mbar_init(raw_full_bar(s), 1); ptx::mbar_init(raw_empty_bar(s), kConverterWarps); }
+        for (int a = 0; a < 2; a++) { ptx::mbar_init(tfull_bar(a), 1); ptx::mbar_init(tempty_bar(a), 2 * kEpilogueWarps); }
+        *abort_flag = 0;
+        ptx::fence_barrier_init();
+        ptx::prefetch_tensormap(&codes_map);
+        ptx::prefetch_tensormap(&delta_map);
+    }
+    if (warp == kIssuer) { ptx::tmem_alloc_pair(ptx::smem_u32(tmem_slot), 512u); ptx::tmem_relinquish_pair(); }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::cluster_sync();
+    ptx::tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    grid_dependency_wait();
+
+    if (warp == kLoader) {
+        // ------------------------------------------------------------------ TMA loads (one thread)
+        if (lane == 0) {
+            StageCursor at;
+            int stage = 0, rs = 0;
+            uint32_t phase = 0, rphase = 0;
+            const uint32_t ring = ptx::smem_u32(smem);
+            for (at.start(p, pair); at.valid; at.next(p, pair)) {
+                const WorkItem &w = at.i.w;
+                const int row = (w.begin + at.step) * S::kRows, o = w.mt * kPairTile + rank * 128, i = w.nt * kPairTile + rank * 128;
+                if (!wait_bar(raw_empty_bar(rs), rphase ^ 1u, abort_flag, p.status, 0x100u + B200_E_TIMEOUT)) break;
+                const uint32_t raw = ring + S::kRing + (uint32_t)rs * S::kRaw;
+                ptx::mbar_arrive_expect_tx(raw_full_bar(rs), S::kRaw);
+                ptx::tma_load_2d(raw, &codes_map, raw_full_bar(rs), i, row);
+                if (!kDirect) ptx::tma_load_2d(raw + S::kCodes, &delta_map, raw_full_bar(rs), o, row);
+                if (++rs == S::kRaws) { rs = 0; rphase ^= 1u; }
+                if (kDirect) {
+                    if (!wait_bar(empty_bar(stage), phase ^ 1u, abort_flag, p.status, 0x700u + B200_E_TIMEOUT)) break;
+                    const uint32_t dst = ring + (uint32_t)stage * S::kStage;
+                    ptx::mbar_arrive_expect_tx(full_bar(stage), S::kOperand);
+                    ptx::tma_load_2d(dst, &delta_map, full_bar(stage), o, row);
+                    ptx::tma_load_2d(dst + S::kOperand / 2, &delta_map, full_bar(stage), o + 64, row);
+                    if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
+                }
+            }
+        }
+    } else if (warp >= kEpilogueWarps && warp < kIssuer) {
+        // ------------------------------------------------------------------ converters
+        const int t = threadIdx.x - kEpilogueWarps * 32;
+        constexpr int kLanes = 128 / S::kCodesEach;                           // threads on a row of codes: 8 or 16
+        const int r = t / kLanes, c = t % kLanes;
+        const int r8 = t >> 4, c8 = t & 15;                                   // row (of 32) and group of eight columns of delta
+
+        // exponent of this thread's codes, kAhead stages before they are needed
+        StageCursor ahead;
+        const uint8_t *eptr = nullptr;
+        int erow = 0;
+        auto aim = [&]() {
+            const size_t i = (size_t)ahead.i.w.nt * kPairTile + rank * 128 + c * S::kCodesEach;
+            erow = (ahead.i.w.begin + ahead.step) * S::kRows + r;
+            eptr = i < p.blocks * kCkptBlock ? p.exponents + (size_t)erow * p.blocks + i / kCkptBlock : nullptr;
+        };
+        auto fetch = [&]() -> uint32_t {
+            uint32_t e = 0;
+            if (!ahead.valid) return e;
+            if (eptr) {
+                if (erow < p.rows) e = __ldg(eptr);
+                eptr += S::kRows * p.blocks;
+            }
+            erow += S::kRows;
+            ahead.next(p, pair);
+            if (ahead.step == 0 && ahead.valid) aim();
+            return e;
+        };
+        ahead.start(p, pair);
+        StageCursor at = ahead;
+        if (ahead.valid) aim();
+        uint32_t exps[kAhead];
+#pragma unroll
+        for (int d = 0; d < kAhead; d++) exps[d] = fetch();
+
+        int stage = 0, rs = 0;
+        uint32_t phase = 0, rphase = 0;
+        bool ok = true;
+        float sums[8] = {};
+        while (at.valid) {
+#pragma unroll
+            for (int d = 0; d < kAhead; d++) {
+                if (!at.valid) break;
+                const bool bias = p.dbias && at.i.w.nt == 0;
+                if (ok) ok = __all_sync(0xffffffffu, wait_bar(raw_full_bar(rs), rphase, abort_flag, p.status, 0x800u + B200_E_TIMEOUT));
+                if (ok) {
+                    const uint8_t *raw = smem + S::kRing + (uint32_t)rs * S::kRaw;
+                    uint4 q;
+                    if (S::kCodesEach == 16) {
+                        q = *reinterpret_cast<const uint4 *>(raw + t * 16);
+                    } else {
+                        const uint2 h = *reinterpret_cast<const uint2 *>(raw + t * 8);
+                        q = make_uint4(h.x, h.y, 0, 0);
+                    }
+                    uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+                    if (!kDirect) {
+                        const uint8_t *src = raw + S::kCodes + t * 8 * sizeof(T);
+                        if (sizeof(T) == 4) {
+                            // the upper four threads of eight take their halves in the other order: no two meet in a bank
+                            const int swap = (c8 >> 2) & 1;
+                            const uint4 x = *reinterpret_cast<const uint4 *>(src + swap * 16), y = *reinterpret_cast<const uint4 *>(src + 16 - swap * 16);
+                            lo = swap ? y : x;
+                            hi = swap ? x : y;
+                        } else {
+                            lo = *reinterpret_cast<const uint4 *>(src);
+                        }
+                    }
+                    __syncwarp();
+                    if (lane == 0) ptx::mbar_arrive(raw_empty_bar(rs));
+                    if (++rs == S::kRaws) { rs = 0; rphase ^= 1u; }
+                    uint4 v0 = decode8(make_uint2(q.x, q.y), exps[d]), v1 = v0;
+                    if (S::kCodesEach == 16) v1 = decode8(make_uint2(q.z, q.w), exps[d]);
+                    float f[8];
+                    if (!kDirect) {
+                        unpack8<T>(lo, hi, f);
+                        if (bias) {
+#pragma unroll
+                            for (int x = 0; x < 8; x++) sums[x] += f[x];
+                        }
+                    }
+                    ok = __all_sync(0xffffffffu, wait_bar(empty_bar(stage), phase ^ 1u, abort_flag, p.status, 0x900u + B200_E_TIMEOUT));
+                    if (ok) {
+                        uint8_t *tile = smem + (uint32_t)stage * S::kStage;
+                        uint8_t *b = tile + PARTS * S::kOperand + r * 128;
+                        if (S::kCodesEach == 16) {
+                            // chunks 2c and 2c + 1 of the row's sixteen; half the threads write theirs in the other order
+                            const int block = c >> 2, first = (2 * c) & 7, swap = block;
+                            b += block * (S::kRows * 128);
+                            *reinterpret_cast<uint4 *>(b + (((first + swap) ^ (r & 7)) << 4)) = swap ? v1 : v0;
+                            *reinterpret_cast<uint4 *>(b + (((first + 1 - swap) ^ (r & 7)) << 4)) = swap ? v0 : v1;
+                        } else {
+                            b += (c >> 3) * (S::kRows * 128);
+                            *reinterpret_cast<uint4 *>(b + (((c & 7) ^ (r & 7)) << 4)) = v0;
+                        }
+                        if (!kDirect) {
+                            uint8_t *a = tile + (c8 >> 3) * (S::kRows * 128) + r8 * 128 + (((c8 & 7) ^ (r8 & 7)) << 4);
+#pragma unroll
+                            for (int part = 0; part < PARTS; part++) {
+                                uint32_t h[4];
+#pragma unroll
+                                for (int x = 0; x < 4; x++) {
+                                    float u0, u1;
+                                    const float r0 = remainder_of(f[2 * x], u0), r1 = remainder_of(f[2 * x + 1], u1);
+                                    h[x] = upper_halves(u0, u1);
+                                    f[2 * x] = r0; f[2 * x + 1] = r1;
+                                }
+                                *reinterpret_cast<uint4 *>(a + part * S::kOperand) = make_uint4(h[0], h[1], h[2], h[3]);
+                            }
+                        }
+                        ptx::fence_proxy_async();
+                        __syncwarp();
+                        if (lane == 0) ptx::mbar_arrive(full_bar(stage));
+                        if (kDirect) {
+                            // the bias gradient sums delta from the operand tile, which stays until every warp has arrived here
+                            if (bias) {
+                                ok = __all_sync(0xffffffffu, wait_bar(full_bar(stage), phase, abort_flag, p.status, 0xa00u + B200_E_TIMEOUT));
+                                if (ok) {
+#pragma unroll
+                                    for (int g = 0; g < S::kRows / 32; g++) {
+                                        const int k = g * 32 + r8;
+                                        unpack8<T>(*reinterpret_cast<const uint4 *>(tile + (c8 >> 3) * (S::kRows * 128) + k * 128 + (((c8 & 7) ^ (k & 7)) << 4)), lo, f);
+#pragma unroll
+                                        for (int x = 0; x < 8; x++) sums[x] += f[x];
+                                    }
+                                }
+                                __syncwarp();
+                            }
+                            if (lane == 0) ptx::mbar_arrive(empty_bar(stage));
+                        }
+                        if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
+                    }
+                }
+                if (bias && at.ends_tile()) {
+                    // the thirty-two row slots (two a warp, joined by a shuffle), then one thread per column
+#pragma unroll
+                    for (int x = 0; x < 8; x++) sums[x] += __shfl_xor_sync(0xffffffffu, sums[x], 16);
+                    if (lane < 16) {
+#pragma unroll
+                        for (int x = 0; x < 8; x++) bias_sums[(t >> 5) * 128 + c8 * 8 + x] = sums[x];
+                    }
+                    asm volatile("bar.sync 1, %0;" ::"n"(kConverters) : "memory");
+                    if (t < 128) {
+                        float s = 0.f;
+#pragma unroll
+                        for (int k = 0; k < kConverterWarps; k++) s += bias_sums[k * 128 + t];
+                        const int o = at.i.w.mt * kPairTile + rank * 128 + t;
+                        if (at.i.w.unit >= 0) p.partial[(size_t)at.i.w.unit * kUnitFloats + kPairTile * kPairTile + rank * 128 + t] = s;
+                        else if (o < p.out) p.dbias[o] = p.accumulate ? p.dbias[o] + s : s;
+                    }
+                    asm volatile("bar.sync 1, %0;" ::"n"(kConverters) : "memory");
+#pragma unroll
+                    for (int x = 0; x < 8; x++) sums[x] = 0.f;
+                }
+                exps[d] = fetch();
+                at.next(p, pair);
+            }
+        }
+    } else if (warp == kIssuer) {
+        // ------------------------------------------------------------------ MMA issuer (one thread of the leader)
+        // The peer's thread passes its full stages on.  The producers do not arrive in the other CTA themselves: an arrival with
+        // cluster scope waits for everything its thread has under way, the loads of the stages ahead among them.
+        if (rank == 1 && lane == 0) {
+            StageCursor at;
+            int stage = 0;
+            uint32_t phase = 0;
+            for (at.start(p, pair); at.valid; at.next(p, pair)) {
+                if (!wait_bar(full_bar(stage), phase, abort_flag, p.status, 0x500u + B200_E_TIMEOUT)) break;
+                ptx::mbar_arrive_cluster(peer_bar(stage), 0);
+                if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
+            }
+        }
+        if (rank == 0 && lane == 0) {
+            const uint64_t desc = ptx::smem_desc(ptx::smem_u32(smem), S::kRows * 128u, 1024u, 2u);
+            int stage = 0, n = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            ItemCursor at;
+            for (bool more = at.start(p, pair); ok && more; more = at.next(p, pair), n++) {
+                const WorkItem w = at.w;
+                const int acc = n % kAccumulators;
+                if (!wait_bar<true>(tempty_bar(acc), ((uint32_t)(n / kAccumulators) & 1u) ^ 1u, abort_flag, p.status, 0x200u + B200_E_TIMEOUT)) break;
+                ptx::tc_fence_after();
+                const uint32_t d = tmem + (uint32_t)acc * 256u;
+                for (int step = 0; step < w.steps; step++) {
+                    ok = wait_bar(full_bar(stage), phase, abort_flag, p.status, 0x300u + B200_E_TIMEOUT) &&
+                         wait_bar<true>(peer_bar(stage), phase, abort_flag, p.status, 0x600u + B200_E_TIMEOUT);
+                    if (!ok) break;
+                    ptx::tc_fence_after();
+                    const uint64_t a = desc + (uint64_t)((uint32_t)stage * S::kStage >> 4), b = a + (PARTS * S::kOperand >> 4);
+#pragma unroll
+                    for (int k = 0; k < S::kRows / 16; k++) {
+#pragma unroll
+                        for (int part = PARTS - 1; part >= 0; part--)        // the small pieces first
+                            ptx::mma_bf16_pair(d, a + (part * S::kOperand >> 4) + k * 128, b + k * 128, p.idesc, step > 0 || k > 0 || part < PARTS - 1);
+                    }
+                    ptx::mma_commit_pair(empty_bar(stage));
+                    if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
+                }
+                if (ok) ptx::mma_commit_pair(tfull_bar(acc));
+            }
+        }
+    } else {
+        // ------------------------------------------------------------------ epilogue (warps 0 to 3, 32 rows each)
+        float *mine = turn + warp * 32 * kPitch;
+        const int sub = lane >> 3, quad = (lane & 7) * 4;
+        ItemCursor at;
+        int n = 0;
+        for (bool more = at.start(p, pair); more; more = at.next(p, pair), n++) {
+            const WorkItem w = at.w;
+            const bool add = !w.first || (w.unit < 0 && p.accumulate);
+            const int acc = n % kAccumulators;
+            bool ok = lane == 0 ? wait_bar(tfull_bar(acc), (uint32_t)(n / kAccumulators) & 1u, abort_flag, p.status, 0x400u + B200_E_TIMEOUT) : true;
+            ok = __shfl_sync(0xffffffffu, ok, 0);
+            if (!ok) break;
+            ptx::tc_fence_after();
+            const int row0 = rank * 128 + warp * 32, o0 = w.mt * kPairTile + row0;
+            const size_t i0 = (size_t)w.nt * kPairTile;
+            const uint32_t src = tmem + (uint32_t)acc * 256u + ((uint32_t)(warp * 32) << 16);
+            for (int col = 0; col < kPairTile; col += 32) {
+                uint32_t v[32];
+                ptx::tmem_ld16_issue(src + col, v);
+                ptx::tmem_ld16_issue(src + col + 16, v + 16);
+                ptx::tmem_ld_wait(v);
+                ptx::tmem_ld_wait(v + 16);
+                if (col + 32 == kPairTile) {             // the accumulator is read: the next tile may have it
+                    ptx::tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) ptx::mbar_arrive_cluster(tempty_bar(acc), 0);
+                }
+                // each thread holds 32 columns of a row; turned around, eight threads write 128 bytes of a row together
+#pragma unroll
+                for (int k = 0; k < 32; k += 4) *reinterpret_cast<uint4 *>(mine + lane * kPitch + k) = make_uint4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+                __syncwarp();
+                const size_t i = i0 + col + quad;
+#pragma unroll
+                for (int k = 0; k < 32; k += 4) {
+                    const int rr = k + sub;
+                    const float4 x = *reinterpret_cast<const float4 *>(mine + rr * kPitch + quad);
+                    float *dst;
+                    bool wide;
+                    if (w.unit >= 0) {
+                        dst = p.partial + (size_t)w.unit * kUnitFloats + (size_t)(row0 + rr) * kPairTile + col + quad;
+                        wide = true;
+                    } else {
+                        if (o0 + rr >= p.out) continue;
+                        dst = p.dweight + (size_t)(o0 + rr) * p.in + i;
+                        wide = p.vector_out && i + 4 <= p.in;
+                    }
+                    if (wide) {
+                        float4 y = x;
+                        if (add) {
+                            const float4 old = *reinterpret_cast<const float4 *>(dst);
+                            y.x += old.x; y.y += old.y; y.z += old.z; y.w += old.w;
+                        }
+                        *reinterpret_cast<float4 *>(dst) = y;
+                    } else {
+                        const float y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                        for (int m = 0; m < 4; m++)
+                            if (i + m < p.in) dst[m] = add ? dst[m] + y[m] : y[m];
+                    }
+                }
+                __syncwarp();
+            }
+        }
+    }
+
+    if (*abort_flag) {            // MMAs still in flight get time to end before the shared memory is released
+        const long long t0 = clock64();
+        while (clock64() - t0 < 200000) __nanosleep(200);
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::cluster_sync();          // neither CTA leaves while its partner may still arrive on its barriers or read its shared memory
+    if (warp == kIssuer) {
+        ptx::tc_fence_after();
+        ptx::tmem_dealloc_pair(tmem, 512u);
+    }
+}
+
+// Sum of the units of each split tile, in their order, and of their bias gradients.
+__global__ void __launch_bounds__(256) ckpt8_wgrad_join_kernel(const __grid_constant__ WgradParams p)
+{
+    grid_dependency_wait();
+    const int tile_index = blockIdx.y, tile = p.first_tail + tile_index;
+    const int mt = tile / p.tiles_n, nt = tile - mt * p.tiles_n;
+    const float *first = p.partial + (size_t)tile_index * p.splits * kUnitFloats;
+    const int at = (blockIdx.x * 256 + threadIdx.x) * 4;               // of the 256 x 256 outputs, then of the 256 sums
+    if (at >= (int)kUnitFloats) return;
+    float4 s = *reinterpret_cast<const float4 *>(first + at);
+    for (int k = 1; k < p.splits; k++) {
+        const float4 v = *reinterpret_cast<const float4 *>(first + (size_t)k * kUnitFloats + at);
+        s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+    }
+    const float v[4] = {s.x, s.y, s.z, s.w};
+    if (at >= kPairTile * kPairTile) {
+        if (!p.dbias || nt) return;
+#pragma unroll
+        for (int m = 0; m < 4; m++) {
+            const int o = mt * kPairTile + at - kPairTile * kPairTile + m;
+            if (o < p.out) p.dbias[o] = p.accumulate ? p.dbias[o] + v[m] : v[m];
+        }
+        return;
+    }
+    const int o = mt * kPairTile + at / kPairTile;
+    const size_t i = (size_t)nt * kPairTile + at % kPairTile;
+    if (o >= p.out) return;
+    float *dst = p.dweight + (size_t)o * p.in + i;
+#pragma unroll
+    for (int m = 0; m < 4; m++)
+        if (i + m < p.in) dst[m] = p.accumulate ? dst[m] + v[m] : v[m];
+}
+
+// Division of the work: `pairs` CTA pairs, `waves` whole tiles each, then the tail in `tail_units` units.
+struct WgradPlan { int tiles_m, tiles_n, steps, pairs, waves, first_tail, tail_units, splits, launch_pairs; };
+static WgradPlan wgrad_plan(int parts, int rows, int out, size_t in)
+{
+    WgradPlan w;
+    const int depth = parts == 1 ? 64 : 32;
+    w.tiles_m = ceil_div(out, kPairTile);
+    w.tiles_n = (int)((in + kPairTile - 1) / kPairTile);
+    w.steps = ceil_div(rows, depth);
+    w.pairs = sm_count() / 2;
+    const long long tiles = (long long)w.tiles_m * w.tiles_n;
+    w.waves = (int)(tiles / w.pairs);
+    w.first_tail = w.waves * w.pairs;
+    const int rest = (int)(tiles - w.first_tail);
+    // a unit has at least four stages: below that its partial tile costs more than the stages it saves
+    w.splits = rest ? max(1, min(w.pairs / rest, w.steps / 4)) : 1;
+    w.tail_units = rest * w.splits;
+    w.launch_pairs = w.waves ? w.pairs : w.tail_units;
+    return w;
+}
+static int wgrad_parts(int type) { return type == B200_BF16 ? 1 : type == B200_F16 ? 2 : 3; }
+
+// delta with rows at 16-byte boundaries, for the tensor map
+template <typename T>
+__global__ void __launch_bounds__(256) ckpt8_wgrad_align_kernel(T *__restrict__ dst, const T *__restrict__ src, int rows, int out, size_t src_pitch, size_t dst_pitch)
+{
+    grid_dependency_wait();
+    constexpr int kVector = 16 / sizeof(T);
+    const size_t vectors = dst_pitch / kVector, total = (size_t)rows * vectors;
+    for (size_t k = (size_t)blockIdx.x * 256 + threadIdx.x; k < total; k += (size_t)gridDim.x * 256) {
+        const size_t row = k / vectors, col = (k - row * vectors) * kVector;
+        T v[kVector];
+#pragma unroll
+        for (int x = 0; x < kVector; x++) v[x] = col + x < (size_t)out ? src[row * src_pitch + col + x] : from_float<T>(0.f);
+        *reinterpret_cast<uint4 *>(dst + row * dst_pitch + col) = *reinterpret_cast<const uint4 *>(v);
+    }
+}
+
+static bool delta_fits(const void *delta, int type, size_t pitch)
+{
+    return !(reinterpret_cast<uintptr_t>(delta) & 15) && !(pitch * type_size(type) & 15) && pitch * type_size(type) < ((size_t)1 << 40);
+}
+static size_t aligned_pitch(int type, int out) { return align_up((size_t)out, 16 / type_size(type)); }
+static size_t partial_bytes(const WgradPlan &w) { return w.splits > 1 ? sizeof(float) * kUnitFloats * (size_t)w.tail_units : 0; }
+
+template <typename T, int PARTS>
+static int wgrad_tc_launch(WgradParams p, const WgradPlan &w, const void *delta, size_t delta_pitch, const int8_t *codes, int type, bool fits, cudaStream_t s)
+{
+    using S = TcShape<T, PARTS>;
+    if (!fits) {
+        T *copy = reinterpret_cast<T *>(reinterpret_cast<char *>(p.partial) + partial_bytes(w));
+        const size_t pitch = aligned_pitch(type, p.out), vectors = (size_t)p.rows * pitch * sizeof(T) / 16;
+        const size_t most = (size_t)sm_count() * 16;
+        Launch((unsigned)min((vectors + 255) / 256, most), 256, 0, s)(ckpt8_wgrad_align_kernel<T>, copy, (const T *)delta, p.rows, p.out, delta_pitch, pitch);
+        B200_LAUNCH_CHECK();
+        delta = copy;
+        delta_pitch = pitch;
+    }
+    CUtensorMap codes_map, delta_map;
+    int r = tensor_map_2d(&codes_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, p.blocks * kCkptBlock, (size_t)p.rows, p.blocks * kCkptBlock, 128, S::kRows, false);
+    if (r) return r;
+    const CUtensorMapDataType kind = type == B200_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : type == B200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    r = tensor_map_2d(&delta_map, kind, delta, (size_t)p.out, (size_t)p.rows, delta_pitch * sizeof(T), PARTS == 1 ? 64 : 128, S::kRows, PARTS == 1);
+    if (r) return r;
+    p.chunk_steps = S::kChunk;
+    B200_CUDA(cudaFuncSetAttribute(ckpt8_wgrad_tc_kernel<T, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTcSmem));
+    Launch((unsigned)w.launch_pairs * 2, kTcThreads, kTcSmem, s).cluster(2)(ckpt8_wgrad_tc_kernel<T, PARTS>, codes_map, delta_map, p);
+    B200_LAUNCH_CHECK();
+    if (w.splits > 1) {
+        Launch(dim3((unsigned)((kUnitFloats / 4 + 255) / 256), (unsigned)(w.tail_units / w.splits)), 256, 0, s)(ckpt8_wgrad_join_kernel, p);
+        B200_LAUNCH_CHECK();
+    }
+    return B200_OK;
+}
+
 }  // namespace b200
 
 using namespace b200;
@@ -66,9 +691,11 @@ using namespace b200;
 
 extern "C" {
 
-size_t b200_ckpt8_wgrad_workspace(int type, int rows, int out, size_t in)
+size_t b200_ckpt8_wgrad_workspace(int type, int rows, int out, size_t in, const void *delta, size_t delta_pitch)
 {
-    return 0;
+    if (!known_type(type) || check_rows(rows, in) || rows == 0 || out <= 0 || precision() == B200_FP32) return 0;
+    const size_t copy = delta_fits(delta, type, delta_pitch) ? 0 : (size_t)rows * aligned_pitch(type, out) * type_size(type);
+    return partial_bytes(wgrad_plan(wgrad_parts(type), rows, out, in)) + copy;
 }
 
 int b200_ckpt8_wgrad(float *dweight, float *dbias, int accumulate, const void *delta, const int8_t *codes, const uint8_t *exponents, int type, int rows,
@@ -88,6 +715,28 @@ int b200_ckpt8_wgrad(float *dweight, float *dbias, int accumulate, const void *d
     }
     if ((r = check_ckpt8(codes, exponents)) || (r = check_matrix(delta, type, rows, (size_t)out, delta_pitch, "delta"))) return r;
     const size_t blocks = ckpt8_blocks(in);
+    if (precision() != B200_FP32) {
+        const WgradPlan w = wgrad_plan(wgrad_parts(type), rows, out, in);
+        const bool fits = delta_fits(delta, type, delta_pitch);
+        const size_t need = b200_ckpt8_wgrad_workspace(type, rows, out, in, delta, delta_pitch);
+        if (need && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15))) return fail(B200_E_ARG, "the workspace must be given, aligned to 16 bytes");
+        if (workspace_bytes < need) return fail(B200_E_NOMEM, "the workspace has %zu bytes, %zu are needed", workspace_bytes, need);
+        WgradParams p = {};
+        p.dweight = dweight; p.dbias = dbias; p.exponents = exponents;
+        p.rows = rows; p.out = out; p.accumulate = accumulate != 0;
+        p.vector_out = !(reinterpret_cast<uintptr_t>(dweight) & 15) && !(in & 3);
+        p.in = in; p.blocks = blocks;
+        p.tiles_n = w.tiles_n; p.steps = w.steps; p.pairs = w.pairs; p.waves = w.waves; p.first_tail = w.first_tail;
+        p.tail_units = w.tail_units; p.splits = w.splits;
+        p.partial = (float *)workspace;
+        p.idesc = make_idesc_bf16(kPairTile, 1, 1, kPairTile);
+        if ((r = status_word(&p.status))) return r;
+        set_path(B200_PATH_TCGEN05);
+        if (type == B200_BF16) return wgrad_tc_launch<__nv_bfloat16, 1>(p, w, delta, delta_pitch, codes, type, fits, ST(stream));
+        if (type == B200_F16) return wgrad_tc_launch<__half, 2>(p, w, delta, delta_pitch, codes, type, fits, ST(stream));
+        return wgrad_tc_launch<float, 3>(p, w, delta, delta_pitch, codes, type, fits, ST(stream));
+    }
+    // B200_FP32: fp32 products on the CUDA cores, summed row by row
     const Launch launch(dim3((unsigned)((in + kTile - 1) / kTile), (unsigned)ceil_div(out, kTile)), 256, 0, ST(stream));
     if (type == B200_F32) launch(ckpt8_wgrad_simt_kernel<float>, dweight, dbias, (const float *)delta, codes, exponents, rows, out, in, delta_pitch, blocks, accumulate);
     else if (type == B200_BF16) launch(ckpt8_wgrad_simt_kernel<__nv_bfloat16>, dweight, dbias, (const __nv_bfloat16 *)delta, codes, exponents, rows, out, in, delta_pitch, blocks, accumulate);

@@ -1,5 +1,6 @@
 // Internal launcher prototypes shared by the translation units of the library.
 #pragma once
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include "../../include/b200conv.h"
 
@@ -32,6 +33,10 @@ int tc_conv_wgrad_batch(const b200_conv_geom &g, float *dkernel, float *dbias, i
                         const float *delta, int batch, int precision, cudaStream_t s);
 int tc_gemm(float *out, const float *a, const float *b, int m, int n, int k, int a_mn_major, int b_mn_major,
             int precision, cudaStream_t s);
+
+// 2-D tensor map (tc_conv.cu), with the 128-byte swizzle or none
+int tensor_map_2d(CUtensorMap *m, CUtensorMapDataType type, const void *base, size_t cols, size_t rows, size_t pitch_bytes, int box_cols, int box_rows,
+                  bool swizzle);
 
 // Packed operands of the tensor-core kernels (tc_conv.cu): a phase-split NHWC copy of an activation
 // tensor, TF32-rounded high part `hi` and (3xTF32 only) remainder `lo`.  Buffers hold elems() floats

@@ -39,7 +39,6 @@ constexpr int kThreads = 224;            // warps: 0 and 6 TMA producers, 1 MMA 
 constexpr int kABytes = 128 * 128;        // 128 rows x 32 tf32
 constexpr int kMaxTaps = 64;
 constexpr int kMaxPhases = 16;
-constexpr long long kWaitCycles = 2000000000LL;
 
 struct TapEntry { int8_t dy, dx; uint8_t in_phase, wtap; };
 struct TapGroup { uint8_t count, tap[4], unused[3]; };      // WGRAD with packed taps: the taps (of one stride phase) of a work item
@@ -188,24 +187,6 @@ __device__ __forceinline__ TileCtx decode_tile(const TcParams &p, int tile, int 
         c.nsteps = total * (c.split + 1) / p.ksplit - c.step_begin;
     }
     return c;
-}
-
-__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile int *abort_flag, unsigned *status, unsigned code)
-{
-    if (ptx::mbar_try_wait(bar, parity)) return true;
-    const long long t0 = clock64();
-    while (true) {
-#pragma unroll 1
-        for (int i = 0; i < 128; i++)
-            if (ptx::mbar_try_wait(bar, parity)) return true;
-        if (*abort_flag) return false;
-        if (clock64() - t0 > kWaitCycles) {
-            *abort_flag = 1;
-            atomicExch(status, code);
-            __threadfence_system();
-            return false;
-        }
-    }
 }
 
 // ACT: the CONV epilogue also applies a neuron function and / or writes the value before it (instantiated separately so that
@@ -919,6 +900,21 @@ static int make_map(CUtensorMap *m, const float *base, const long long dims[5], 
     if (r != CUDA_SUCCESS)
         return fail(B200_E_CUDA, "cuTensorMapEncodeTiled failed (%d) dims %lld %lld %lld %lld %lld box %d %d %d %d %d", (int)r,
                     dims[0], dims[1], dims[2], dims[3], dims[4], box[0], box[1], box[2], box[3], box[4]);
+    return B200_OK;
+}
+
+// 2-D map of `rows` rows of `cols` elements, `pitch_bytes` apart (a multiple of 16, as is the base): boxes of box_cols x box_rows,
+// out-of-range elements read as zero.
+int tensor_map_2d(CUtensorMap *m, CUtensorMapDataType type, const void *base, size_t cols, size_t rows, size_t pitch_bytes, int box_cols, int box_rows,
+                  bool swizzle)
+{
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return fail(B200_E_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, pitch[1] = {(cuuint64_t)pitch_bytes};
+    const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows}, one[2] = {1, 1};
+    const CUresult r = fn(m, type, 2, const_cast<void *>(base), dims, pitch, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(B200_E_CUDA, "cuTensorMapEncodeTiled failed (%d): %zu x %zu, pitch %zu bytes", (int)r, rows, cols, pitch_bytes);
     return B200_OK;
 }
 

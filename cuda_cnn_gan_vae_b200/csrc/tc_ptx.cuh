@@ -51,6 +51,12 @@ __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap *map
         ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
         : "memory");
 }
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int c0, int c1)
+{
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1)
+                 : "memory");
+}
 __device__ __forceinline__ void prefetch_tensormap(const CUtensorMap *map)
 {
     asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
@@ -171,6 +177,38 @@ __device__ __forceinline__ void mma_tf32_pair(uint32_t d_tmem, uint64_t adesc, u
         ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
+// The same with bf16 operands (K = 16)
+__device__ __forceinline__ void mma_bf16_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// Arrival that publishes this CTA's shared-memory writes to the CTA of the pair that owns the barrier, and the wait for it
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar, uint32_t cta)
+{
+    asm volatile(
+        "{\n\t.reg .b32 ra;\n\t"
+        "mapa.shared::cluster.u32 ra, %0, %1;\n\t"
+        "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [ra];\n\t}"
+        ::"r"(bar), "r"(cta)
+        : "memory");
+}
+__device__ __forceinline__ uint32_t mbar_try_wait_cluster(uint32_t bar, uint32_t parity)
+{
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(kMbarSuspendNs)
+        : "memory");
+    return ok;
+}
 // arrive on the mbarrier at this offset in both CTAs of the pair once the issued MMAs have completed
 __device__ __forceinline__ void mma_commit_pair(uint32_t bar)
 {
@@ -202,6 +240,29 @@ __device__ __forceinline__ float to_tf32(float x)
 
 }  // namespace ptx
 
+// A bounded wait: after about a second of polling the kernel records `code` in the status word, raises its abort flag and
+// goes on without the data; every other wait of the block then gives up too.
+constexpr long long kWaitCycles = 2000000000LL;
+template <bool CLUSTER = false>
+__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile int *abort_flag, unsigned *status, unsigned code)
+{
+    auto poll = [&]() { return CLUSTER ? ptx::mbar_try_wait_cluster(bar, parity) : ptx::mbar_try_wait(bar, parity); };
+    if (poll()) return true;
+    const long long t0 = clock64();
+    while (true) {
+#pragma unroll 1
+        for (int i = 0; i < 128; i++)
+            if (poll()) return true;
+        if (*abort_flag) return false;
+        if (clock64() - t0 > kWaitCycles) {
+            *abort_flag = 1;
+            atomicExch(status, code);
+            __threadfence_system();
+            return false;
+        }
+    }
+}
+
 // Instruction descriptor of tcgen05.mma kind::tf32: fp32 accumulator, TF32 A and B, M = 128 (one CTA)
 // or 256 (CTA pair).
 inline uint32_t make_idesc_tf32(int n, int a_mn_major, int b_mn_major, int m = 128)
@@ -215,6 +276,12 @@ inline uint32_t make_idesc_tf32(int n, int a_mn_major, int b_mn_major, int m = 1
     d |= (uint32_t)(n >> 3) << 17;
     d |= (uint32_t)(m >> 4) << 24;
     return d;
+}
+
+// The same for kind::f16 with bf16 operands
+inline uint32_t make_idesc_bf16(int n, int a_mn_major, int b_mn_major, int m = 128)
+{
+    return (make_idesc_tf32(n, a_mn_major, b_mn_major, m) & ~((7u << 7) | (7u << 10))) | (1u << 7) | (1u << 10);
 }
 
 }  // namespace b200

@@ -81,7 +81,7 @@ SIGNATURES = {
     "b200_ckpt8_store": (_i, [_vp, _vp, _vp, _i, _i, _sz, _sz, _i, _vp]),
     "b200_ckpt8_load": (_i, [_vp, _vp, _vp, _i, _i, _sz, _sz, _vp]),
     "b200_ckpt8_activation_backward": (_i, [_vp] * 4 + [_i, _i, _sz, _sz, _sz, _i, _d, _vp]),
-    "b200_ckpt8_wgrad_workspace": (_sz, [_i, _i, _i, _sz]),
+    "b200_ckpt8_wgrad_workspace": (_sz, [_i, _i, _i, _sz, _vp, _sz]),
     "b200_ckpt8_wgrad": (_i, [_vp, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _sz, _sz, _vp, _sz, _vp]),
     "b200_vae_forward": (_i, [_fp, _fp, _fp, _fp, _i, _sz, C.POINTER(C.c_float), _vp]),
     "b200_vae_backward": (_i, [_fp] * 6 + [_sz, _f, _vp]),

@@ -576,7 +576,7 @@ def checkpoint_wgrad(dweight, dbias, delta, checkpoint, accumulate=True, workspa
     _param(dweight, out * checkpoint.n, "dweight")
     if dbias is not None:
         _param(dbias, out, "dbias")
-    workspace, size = _workspace(load().b200_ckpt8_wgrad_workspace(kind, rows, out, checkpoint.n), workspace, "checkpoint_wgrad")
+    workspace, size = _workspace(load().b200_ckpt8_wgrad_workspace(kind, rows, out, checkpoint.n, delta.data_ptr(), pitch), workspace, "checkpoint_wgrad")
     _check(load().b200_ckpt8_wgrad(dweight.data_ptr(), dbias.data_ptr() if dbias is not None else None, int(accumulate), delta.data_ptr(),
                                    checkpoint.codes.data_ptr(), checkpoint.exponents.data_ptr(), kind, rows, out, checkpoint.n, pitch,
                                    workspace.data_ptr(), size, _stream()))

@@ -330,7 +330,7 @@ int b200_adam_prepared(float *weight, const float *dweight, float *m, float *v, 
 enum { B200_F32 = 0, B200_BF16 = 1, B200_F16 = 2 };
 
 /* In this section a tensor is a matrix of `rows` rows of n values; row r starts at element r * pitch (pitch >= n; a dense
- * tensor [W,Z,Y,X] taken per sample has rows = W, n = pitch = Z*Y*X).  1 <= n <= 2^31 - 64; rows may be 0 (nothing is read, and
+ * tensor [W,Z,Y,X] taken per sample has rows = W, n = pitch = Z*Y*X).  1 <= n <= 2^31 - 64, as many rows at most; rows may be 0 (nothing is read, and
  * gradients that are not accumulated become zero).  Pointers are aligned to the element size, codes to 16 bytes.  Nothing here
  * uses the library's scratch arena: a call that needs scratch takes it from the caller (16-byte aligned, at least as many bytes
  * as its ..._workspace() says for the same sizes; the contents need not be kept between calls), so calls on several streams and
@@ -368,8 +368,9 @@ int b200_ckpt8_activation_backward(void *out, const int8_t *codes, const uint8_t
                                    size_t n, size_t out_pitch, size_t error_pitch, int func, double leaky_slope, void *stream);
 /* Gradients of a Linear layer (netlayer/cnetlayerlinear.cu.h:415) whose input [rows][in] was kept in 8 bits:
  * dweight[out][in] (+)= sum over rows of delta[row][out] * value[row][in], dbias[out] (+)= sum over rows of delta[row][out]
- * (dbias may be NULL). */
-size_t b200_ckpt8_wgrad_workspace(int type, int rows, int out, size_t in);
+ * (dbias may be NULL).  A delta whose rows do not all start at a 16-byte boundary is copied into the workspace first.  delta enters
+ * exactly in both tensor-core modes; B200_FP32 forms the products on the CUDA cores. */
+size_t b200_ckpt8_wgrad_workspace(int type, int rows, int out, size_t in, const void *delta, size_t delta_pitch);
 int b200_ckpt8_wgrad(float *dweight, float *dbias, int accumulate, const void *delta, const int8_t *codes, const uint8_t *exponents,
                      int type, int rows, int out, size_t in, size_t delta_pitch, void *workspace, size_t workspace_bytes, void *stream);
 
