@@ -71,15 +71,16 @@ __global__ void __launch_bounds__(256) ckpt8_wgrad_simt_kernel(float *dweight, f
 //     roundings are those of the fp32 accumulator.  The tensor core truncates its sums, a bias that grows with their number:
 //     after kChunk stages the accumulator is added to the output (rounded to nearest) and starts again from zero.  8192 rows at
 //     a stretch were off by 2.5e-6 of the result, chunks of 2048 are by 4e-7.
-//   * One warp brings the codes and delta in by TMA (bf16 straight into the operand tile); sixteen warps decode and split from
-//     shared memory into a ring of operand stages (five instructions for two values, once per pair and tile).  A first form
-//     in which those warps loaded from global memory themselves, into registers three stages ahead, took 1030 us at
-//     8192 rows, 4096 x 4096: 340 instructions a warp and stage, half its time waiting for loads.
+//   * One warp brings the codes and delta in by TMA (bf16 straight into the operand tile); four groups of four warps decode and
+//     split from shared memory into a ring of operand stages (five instructions for two values, once per pair and tile).  A
+//     group takes every fourth stage, so four stages are in work at a time: with all sixteen warps on each stage its chain of
+//     waits, loads and stores was in series with the next one's (514 us at 8192 rows, 4096 x 4096, bf16; and 1030 us where
+//     they loaded from global memory into registers three stages ahead).
 //   * The grid is one pair per two SMs.  Whole tiles go round the pairs; what is left over (or everything, where there are
 //     fewer tiles than pairs) is split along the batch into units that write partial tiles, joined by a second
 //     kernel in the order of the units.  No atomics: the result does not depend on scheduling.
 constexpr int kPairTile = 256;                     // outputs of a pair in both directions
-constexpr int kEpilogueWarps = 4, kConverterWarps = 16;
+constexpr int kEpilogueWarps = 4, kConverterWarps = 16, kGroupWarps = 4, kGroups = kConverterWarps / kGroupWarps;
 constexpr int kConverters = kConverterWarps * 32;
 constexpr int kTcThreads = (kEpilogueWarps + kConverterWarps + 2) * 32;
 constexpr int kPitch = 36;                         // floats in a row of the epilogue's transposition buffer
@@ -207,15 +208,14 @@ template <typename T, int PARTS> struct TcShape {
     static constexpr int kRows = PARTS == 1 ? 64 : 32;
     static constexpr uint32_t kOperand = kRows * 256u;                        // bytes of a 128-wide bf16 tile
     static constexpr uint32_t kStage = (PARTS + 1) * kOperand;
-    static constexpr int kStages = PARTS == 1 ? 5 : PARTS == 2 ? 4 : 3;
+    static constexpr int kStages = PARTS == 1 ? 5 : 4;
     static constexpr uint32_t kCodes = kRows * 128u;
     static constexpr uint32_t kRaw = kCodes + (PARTS == 1 ? 0u : kRows * 128u * (uint32_t)sizeof(T));
-    static constexpr int kRaws = PARTS == 1 ? 4 : PARTS == 2 ? 8 : 5;
+    static constexpr int kRaws = PARTS == 1 ? 4 : PARTS == 2 ? 8 : 3;
     static constexpr uint32_t kRing = kStages * kStage;                       // bytes before the raw ring
-    static constexpr int kCodesEach = kRows / 4;                              // codes per converter thread: 16 or 8
+    static constexpr int kCodePasses = kRows / 16, kDeltaPasses = kRows / 8;  // of a group's 128 threads over the stage
     static constexpr int kChunk = (PARTS == 1 ? 2048 : 1024) / kRows;         // stages after which the accumulator is emptied
 };
-constexpr int kAhead = 4;                                                     // exponents are loaded this many stages ahead
 constexpr int kAccumulators = 2;                                              // the epilogue of an item overlaps the products of the next
 constexpr size_t kRingBytes = 200704;
 constexpr size_t kTcSmem = 1024 + kRingBytes + kEpilogueWarps * 32 * kPitch * 4 + kConverterWarps * 128 * 4 + 512;
@@ -251,11 +251,11 @@ ckpt8_wgrad_tc_kernel(const __grid_constant__ CUtensorMap codes_map, const __gri
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::kStages; s++) {
-            ptx::mbar_init(full_bar(s), kConverterWarps + (kDirect ? 1 : 0));
-            ptx::mbar_init(empty_bar(s), 1 + (kDirect ? kConverterWarps : 0));
+            ptx::mbar_init(full_bar(s), kGroupWarps + (kDirect ? 1 : 0));
+            ptx::mbar_init(empty_bar(s), 1 + (kDirect ? kGroupWarps : 0));
             ptx::mbar_init(peer_bar(s), 1);
         }
-        for (int s = 0; s < S::kRaws; s++) { ptx::mbar_init(raw_full_bar(s), 1); ptx::mbar_init(raw_empty_bar(s), kConverterWarps); }
+        for (int s = 0; s < S::kRaws; s++) { ptx::mbar_init(raw_full_bar(s), 1); ptx::mbar_init(raw_empty_bar(s), kGroupWarps); }
         for (int a = 0; a < 2; a++) { ptx::mbar_init(tfull_bar(a), 1); ptx::mbar_init(tempty_bar(a), 2 * kEpilogueWarps); }
         *abort_flag = 0;
         ptx::fence_barrier_init();
@@ -298,100 +298,75 @@ ckpt8_wgrad_tc_kernel(const __grid_constant__ CUtensorMap codes_map, const __gri
         }
     } else if (warp >= kEpilogueWarps && warp < kIssuer) {
         // ------------------------------------------------------------------ converters
-        const int t = threadIdx.x - kEpilogueWarps * 32;
-        constexpr int kLanes = 128 / S::kCodesEach;                           // threads on a row of codes: 8 or 16
-        const int r = t / kLanes, c = t % kLanes;
-        const int r8 = t >> 4, c8 = t & 15;                                   // row (of 32) and group of eight columns of delta
+        const int group = (warp - kEpilogueWarps) / kGroupWarps, t = (threadIdx.x - kEpilogueWarps * 32) & 127;
+        const int r = t >> 3, c = t & 7;                                      // codes: row (of 16) and run of sixteen columns
+        const int r8 = t >> 4, c8 = t & 15;                                   // delta: row (of 8) and group of eight columns
 
-        // exponent of this thread's codes, kAhead stages before they are needed
+        // exponents of this thread's codes in the group's next stage, loaded while the current one is converted
         StageCursor ahead;
-        const uint8_t *eptr = nullptr;
-        int erow = 0;
-        auto aim = [&]() {
-            const size_t i = (size_t)ahead.i.w.nt * kPairTile + rank * 128 + c * S::kCodesEach;
-            erow = (ahead.i.w.begin + ahead.step) * S::kRows + r;
-            eptr = i < p.blocks * kCkptBlock ? p.exponents + (size_t)erow * p.blocks + i / kCkptBlock : nullptr;
-        };
-        auto fetch = [&]() -> uint32_t {
-            uint32_t e = 0;
-            if (!ahead.valid) return e;
-            if (eptr) {
-                if (erow < p.rows) e = __ldg(eptr);
-                eptr += S::kRows * p.blocks;
-            }
-            erow += S::kRows;
-            ahead.next(p, pair);
-            if (ahead.step == 0 && ahead.valid) aim();
-            return e;
-        };
         ahead.start(p, pair);
-        StageCursor at = ahead;
-        if (ahead.valid) aim();
-        uint32_t exps[kAhead];
+        for (int k = 0; k < group && ahead.valid; k++) ahead.next(p, pair);
+        uint32_t exps[S::kCodePasses];
+        auto fetch = [&]() {
+            const size_t i = (size_t)ahead.i.w.nt * kPairTile + rank * 128 + c * 16;
+            const int row = (ahead.i.w.begin + ahead.step) * S::kRows + r;
+            const bool in = ahead.valid && i < p.blocks * kCkptBlock;
+            const uint8_t *src = p.exponents + (size_t)row * p.blocks + i / kCkptBlock;
 #pragma unroll
-        for (int d = 0; d < kAhead; d++) exps[d] = fetch();
+            for (int k = 0; k < S::kCodePasses; k++) {
+                exps[k] = 0;
+                if (in && row + 16 * k < p.rows) exps[k] = __ldg(src + (size_t)(16 * k) * p.blocks);
+            }
+        };
+        fetch();
 
-        int stage = 0, rs = 0;
+        StageCursor at;
+        int turn_of = 0, stage = 0, rs = 0;
         uint32_t phase = 0, rphase = 0;
         bool ok = true;
         float sums[8] = {};
-        while (at.valid) {
-#pragma unroll
-            for (int d = 0; d < kAhead; d++) {
-                if (!at.valid) break;
-                const bool bias = p.dbias && at.i.w.nt == 0;
+        for (at.start(p, pair); at.valid;) {
+            const bool bias = p.dbias && at.i.w.nt == 0;
+            if (turn_of == group) {
                 if (ok) ok = __all_sync(0xffffffffu, wait_bar(raw_full_bar(rs), rphase, abort_flag, p.status, 0x800u + B200_E_TIMEOUT));
+                if (ok) ok = __all_sync(0xffffffffu, wait_bar(empty_bar(stage), phase ^ 1u, abort_flag, p.status, 0x900u + B200_E_TIMEOUT));
                 if (ok) {
                     const uint8_t *raw = smem + S::kRing + (uint32_t)rs * S::kRaw;
-                    uint4 q;
-                    if (S::kCodesEach == 16) {
-                        q = *reinterpret_cast<const uint4 *>(raw + t * 16);
-                    } else {
-                        const uint2 h = *reinterpret_cast<const uint2 *>(raw + t * 8);
-                        q = make_uint4(h.x, h.y, 0, 0);
-                    }
-                    uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-                    if (!kDirect) {
-                        const uint8_t *src = raw + S::kCodes + t * 8 * sizeof(T);
-                        if (sizeof(T) == 4) {
-                            // the upper four threads of eight take their halves in the other order: no two meet in a bank
-                            const int swap = (c8 >> 2) & 1;
-                            const uint4 x = *reinterpret_cast<const uint4 *>(src + swap * 16), y = *reinterpret_cast<const uint4 *>(src + 16 - swap * 16);
-                            lo = swap ? y : x;
-                            hi = swap ? x : y;
-                        } else {
-                            lo = *reinterpret_cast<const uint4 *>(src);
-                        }
-                    }
-                    __syncwarp();
-                    if (lane == 0) ptx::mbar_arrive(raw_empty_bar(rs));
-                    if (++rs == S::kRaws) { rs = 0; rphase ^= 1u; }
-                    uint4 v0 = decode8(make_uint2(q.x, q.y), exps[d]), v1 = v0;
-                    if (S::kCodesEach == 16) v1 = decode8(make_uint2(q.z, q.w), exps[d]);
-                    float f[8];
-                    if (!kDirect) {
-                        unpack8<T>(lo, hi, f);
-                        if (bias) {
+                    uint8_t *tile = smem + (uint32_t)stage * S::kStage;
+                    // chunks 2c and 2c + 1 of a row's sixteen; half the threads write theirs in the other order, so that no two meet
+                    // in a bank
+                    const int block = c >> 2, chunk = ((2 * c) & 7) + block;
+                    uint8_t *b = tile + PARTS * S::kOperand + block * (S::kRows * 128) + r * 128;
+                    const uint32_t first = (uint32_t)((chunk ^ (r & 7)) << 4), second = (uint32_t)(((chunk + 1 - 2 * block) ^ (r & 7)) << 4);
 #pragma unroll
-                            for (int x = 0; x < 8; x++) sums[x] += f[x];
-                        }
+                    for (int k = 0; k < S::kCodePasses; k++) {
+                        const uint4 q = *reinterpret_cast<const uint4 *>(raw + k * 2048 + t * 16);
+                        const uint4 v0 = decode8(make_uint2(q.x, q.y), exps[k]), v1 = decode8(make_uint2(q.z, q.w), exps[k]);
+                        *reinterpret_cast<uint4 *>(b + k * 2048 + first) = block ? v1 : v0;
+                        *reinterpret_cast<uint4 *>(b + k * 2048 + second) = block ? v0 : v1;
                     }
-                    ok = __all_sync(0xffffffffu, wait_bar(empty_bar(stage), phase ^ 1u, abort_flag, p.status, 0x900u + B200_E_TIMEOUT));
-                    if (ok) {
-                        uint8_t *tile = smem + (uint32_t)stage * S::kStage;
-                        uint8_t *b = tile + PARTS * S::kOperand + r * 128;
-                        if (S::kCodesEach == 16) {
-                            // chunks 2c and 2c + 1 of the row's sixteen; half the threads write theirs in the other order
-                            const int block = c >> 2, first = (2 * c) & 7, swap = block;
-                            b += block * (S::kRows * 128);
-                            *reinterpret_cast<uint4 *>(b + (((first + swap) ^ (r & 7)) << 4)) = swap ? v1 : v0;
-                            *reinterpret_cast<uint4 *>(b + (((first + 1 - swap) ^ (r & 7)) << 4)) = swap ? v0 : v1;
-                        } else {
-                            b += (c >> 3) * (S::kRows * 128);
-                            *reinterpret_cast<uint4 *>(b + (((c & 7) ^ (r & 7)) << 4)) = v0;
-                        }
-                        if (!kDirect) {
-                            uint8_t *a = tile + (c8 >> 3) * (S::kRows * 128) + r8 * 128 + (((c8 & 7) ^ (r8 & 7)) << 4);
+                    if (!kDirect) {
+                        uint8_t *a = tile + (c8 >> 3) * (S::kRows * 128) + r8 * 128 + (((c8 & 7) ^ (r8 & 7)) << 4);
+                        const uint8_t *src = raw + S::kCodes + t * 8 * sizeof(T);
+#pragma unroll
+                        for (int k = 0; k < S::kDeltaPasses; k++) {
+                            uint4 lo, hi = make_uint4(0, 0, 0, 0);
+                            if (sizeof(T) == 4) {
+                                // the upper four threads of eight take their halves in the other order
+                                const int swap = (c8 >> 2) & 1;
+                                const uint4 x = *reinterpret_cast<const uint4 *>(src + k * 1024 * sizeof(T) + swap * 16),
+                                            y = *reinterpret_cast<const uint4 *>(src + k * 1024 * sizeof(T) + 16 - swap * 16);
+                                lo = swap ? y : x;
+                                hi = swap ? x : y;
+                            } else {
+                                lo = *reinterpret_cast<const uint4 *>(src + k * 1024 * sizeof(T));
+                            }
+                            float f[8];
+                            unpack8<T>(lo, hi, f);
+                            if (bias) {
+#pragma unroll
+                                for (int x = 0; x < 8; x++) sums[x] += f[x];
+                            }
 #pragma unroll
                             for (int part = 0; part < PARTS; part++) {
                                 uint32_t h[4];
@@ -402,56 +377,61 @@ ckpt8_wgrad_tc_kernel(const __grid_constant__ CUtensorMap codes_map, const __gri
                                     h[x] = upper_halves(u0, u1);
                                     f[2 * x] = r0; f[2 * x + 1] = r1;
                                 }
-                                *reinterpret_cast<uint4 *>(a + part * S::kOperand) = make_uint4(h[0], h[1], h[2], h[3]);
+                                *reinterpret_cast<uint4 *>(a + part * S::kOperand + k * 1024) = make_uint4(h[0], h[1], h[2], h[3]);
                             }
                         }
-                        ptx::fence_proxy_async();
-                        __syncwarp();
-                        if (lane == 0) ptx::mbar_arrive(full_bar(stage));
-                        if (kDirect) {
-                            // the bias gradient sums delta from the operand tile, which stays until every warp has arrived here
-                            if (bias) {
-                                ok = __all_sync(0xffffffffu, wait_bar(full_bar(stage), phase, abort_flag, p.status, 0xa00u + B200_E_TIMEOUT));
-                                if (ok) {
+                    }
+                    ptx::fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) { ptx::mbar_arrive(full_bar(stage)); ptx::mbar_arrive(raw_empty_bar(rs)); }
+                    if (kDirect) {
+                        // the bias gradient sums delta from the operand tile, which stays until every warp of the group has arrived here
+                        if (bias) {
+                            ok = __all_sync(0xffffffffu, wait_bar(full_bar(stage), phase, abort_flag, p.status, 0xa00u + B200_E_TIMEOUT));
+                            if (ok) {
 #pragma unroll
-                                    for (int g = 0; g < S::kRows / 32; g++) {
-                                        const int k = g * 32 + r8;
-                                        unpack8<T>(*reinterpret_cast<const uint4 *>(tile + (c8 >> 3) * (S::kRows * 128) + k * 128 + (((c8 & 7) ^ (k & 7)) << 4)), lo, f);
+                                for (int k = 0; k < S::kDeltaPasses; k++) {
+                                    const uint4 lo = *reinterpret_cast<const uint4 *>(tile + (c8 >> 3) * (S::kRows * 128) + (k * 8 + r8) * 128 + (((c8 & 7) ^ r8) << 4));
+                                    float f[8];
+                                    unpack8<T>(lo, lo, f);
 #pragma unroll
-                                        for (int x = 0; x < 8; x++) sums[x] += f[x];
-                                    }
+                                    for (int x = 0; x < 8; x++) sums[x] += f[x];
                                 }
-                                __syncwarp();
                             }
-                            if (lane == 0) ptx::mbar_arrive(empty_bar(stage));
+                            __syncwarp();
                         }
-                        if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
+                        if (lane == 0) ptx::mbar_arrive(empty_bar(stage));
                     }
                 }
-                if (bias && at.ends_tile()) {
-                    // the thirty-two row slots (two a warp, joined by a shuffle), then one thread per column
-#pragma unroll
-                    for (int x = 0; x < 8; x++) sums[x] += __shfl_xor_sync(0xffffffffu, sums[x], 16);
-                    if (lane < 16) {
-#pragma unroll
-                        for (int x = 0; x < 8; x++) bias_sums[(t >> 5) * 128 + c8 * 8 + x] = sums[x];
-                    }
-                    asm volatile("bar.sync 1, %0;" ::"n"(kConverters) : "memory");
-                    if (t < 128) {
-                        float s = 0.f;
-#pragma unroll
-                        for (int k = 0; k < kConverterWarps; k++) s += bias_sums[k * 128 + t];
-                        const int o = at.i.w.mt * kPairTile + rank * 128 + t;
-                        if (at.i.w.unit >= 0) p.partial[(size_t)at.i.w.unit * kUnitFloats + kPairTile * kPairTile + rank * 128 + t] = s;
-                        else if (o < p.out) p.dbias[o] = p.accumulate ? p.dbias[o] + s : s;
-                    }
-                    asm volatile("bar.sync 1, %0;" ::"n"(kConverters) : "memory");
-#pragma unroll
-                    for (int x = 0; x < 8; x++) sums[x] = 0.f;
-                }
-                exps[d] = fetch();
-                at.next(p, pair);
+#pragma unroll 1
+                for (int k = 0; k < kGroups && ahead.valid; k++) ahead.next(p, pair);
+                fetch();
             }
+            if (++turn_of == kGroups) turn_of = 0;
+            if (++rs == S::kRaws) { rs = 0; rphase ^= 1u; }
+            if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
+            if (bias && at.ends_tile()) {
+                // the thirty-two row slots (two a warp, joined by a shuffle), then one thread per column
+#pragma unroll
+                for (int x = 0; x < 8; x++) sums[x] += __shfl_xor_sync(0xffffffffu, sums[x], 16);
+                if (lane < 16) {
+#pragma unroll
+                    for (int x = 0; x < 8; x++) bias_sums[(warp - kEpilogueWarps) * 128 + c8 * 8 + x] = sums[x];
+                }
+                asm volatile("bar.sync 1, %0;" ::"n"(kConverters) : "memory");
+                if (group == 0) {
+                    float s = 0.f;
+#pragma unroll
+                    for (int k = 0; k < kConverterWarps; k++) s += bias_sums[k * 128 + t];
+                    const int o = at.i.w.mt * kPairTile + rank * 128 + t;
+                    if (at.i.w.unit >= 0) p.partial[(size_t)at.i.w.unit * kUnitFloats + kPairTile * kPairTile + rank * 128 + t] = s;
+                    else if (o < p.out) p.dbias[o] = p.accumulate ? p.dbias[o] + s : s;
+                }
+                asm volatile("bar.sync 1, %0;" ::"n"(kConverters) : "memory");
+#pragma unroll
+                for (int x = 0; x < 8; x++) sums[x] = 0.f;
+            }
+            at.next(p, pair);
         }
     } else if (warp == kIssuer) {
         // ------------------------------------------------------------------ MMA issuer (one thread of the leader)
