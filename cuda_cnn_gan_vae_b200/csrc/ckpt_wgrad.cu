@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(256) ckpt8_wgrad_simt_kernel(float *dweight, f
 constexpr int kPairTile = 256;                     // outputs of a pair in both directions
 constexpr int kEpilogueWarps = 4, kConverterWarps = 16, kGroupWarps = 4, kGroups = kConverterWarps / kGroupWarps;
 constexpr int kConverters = kConverterWarps * 32;
-constexpr int kTcThreads = (kEpilogueWarps + kConverterWarps + 2) * 32;
+constexpr int kTcThreads = (kEpilogueWarps + kConverterWarps + 3) * 32;
 constexpr int kPitch = 36;                         // floats in a row of the epilogue's transposition buffer
 constexpr size_t kUnitFloats = (size_t)kPairTile * kPairTile + kPairTile;      // a partial tile and its partial bias gradient
 
@@ -139,19 +139,6 @@ struct ItemCursor {
     }
 };
 
-// Walks the stages of all work items of a pair in order.
-struct StageCursor {
-    ItemCursor i;
-    int step;
-    bool valid;
-    __device__ __forceinline__ void start(const WgradParams &p, int pair) { step = 0; valid = i.start(p, pair); }
-    __device__ __forceinline__ bool ends_tile() const { return i.w.last && step + 1 == i.w.steps; }
-    __device__ __forceinline__ void next(const WgradParams &p, int pair)
-    {
-        if (++step == i.w.steps) { step = 0; valid = i.next(p, pair); }
-    }
-};
-
 // Eight codes with the scale of their block -> eight bf16 values.  The bytes 0x43, u form the bf16 bits of 128 + (u & 127) and
 // of 128 + (u & 128); their difference is the signed code, exact, and so is its product with the power of two.
 __device__ __forceinline__ uint4 decode8(uint2 codes, uint32_t exponent)
@@ -203,15 +190,17 @@ template <> __device__ __forceinline__ void unpack8<__half>(uint4 lo, uint4, flo
     }
 }
 
-// Rows of the batch in a stage, and the two rings: raw (codes as stored, and delta where it has to be split) and operands.
+// Rows of the batch in a stage, and the two rings: raw (codes as stored, and delta where it has to be split) and operands.  Both
+// have a multiple of kGroups slots, so a slot always belongs to the same group: a group that waits for a phase has itself seen the
+// one before, which the parity of a barrier cannot tell from it.
 template <typename T, int PARTS> struct TcShape {
-    static constexpr int kRows = PARTS == 1 ? 64 : 32;
+    static constexpr int kRows = PARTS == 1 ? 64 : PARTS == 2 ? 32 : 16;
     static constexpr uint32_t kOperand = kRows * 256u;                        // bytes of a 128-wide bf16 tile
     static constexpr uint32_t kStage = (PARTS + 1) * kOperand;
-    static constexpr int kStages = PARTS == 1 ? 5 : 4;
+    static constexpr int kStages = PARTS == 3 ? 8 : 4;
     static constexpr uint32_t kCodes = kRows * 128u;
     static constexpr uint32_t kRaw = kCodes + (PARTS == 1 ? 0u : kRows * 128u * (uint32_t)sizeof(T));
-    static constexpr int kRaws = PARTS == 1 ? 4 : PARTS == 2 ? 8 : 3;
+    static constexpr int kRaws = PARTS == 3 ? 4 : 8;
     static constexpr uint32_t kRing = kStages * kStage;                       // bytes before the raw ring
     static constexpr int kCodePasses = kRows / 16, kDeltaPasses = kRows / 8;  // of a group's 128 threads over the stage
     static constexpr int kChunk = (PARTS == 1 ? 2048 : 1024) / kRows;         // stages after which the accumulator is emptied
@@ -226,6 +215,7 @@ ckpt8_wgrad_tc_kernel(const __grid_constant__ CUtensorMap codes_map, const __gri
 {
     using S = TcShape<T, PARTS>;
     static_assert(S::kRing + S::kRaws * S::kRaw <= kRingBytes, "rings");
+    static_assert(S::kStages % kGroups == 0 && S::kRaws % kGroups == 0, "a slot belongs to one group");
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     float *turn = reinterpret_cast<float *>(smem + kRingBytes);               // epilogue: 32 x 32 per warp
@@ -239,23 +229,25 @@ ckpt8_wgrad_tc_kernel(const __grid_constant__ CUtensorMap codes_map, const __gri
     auto raw_empty_bar = [&](int s) { return bar_base + 8u * (3 * S::kStages + S::kRaws + s); };
     auto tfull_bar = [&](int a) { return bar_base + 8u * (3 * S::kStages + 2 * S::kRaws + a); };
     auto tempty_bar = [&](int a) { return bar_base + 8u * (3 * S::kStages + 2 * S::kRaws + 2 + a); };
-    constexpr int kBars = 3 * S::kStages + 2 * S::kRaws + 4;
+    auto read_bar = [&](int s) { return bar_base + 8u * (3 * S::kStages + 2 * S::kRaws + 4 + s); };      // direct delta: its tile has been summed
+    constexpr int kBars = 4 * S::kStages + 2 * S::kRaws + 4;
     static_assert(kBars * 8 + 8 <= 512, "barriers");
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + kBars);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)ptx::cluster_ctarank(), pair = (int)(blockIdx.x >> 1);
-    constexpr int kIssuer = kEpilogueWarps + kConverterWarps, kLoader = kIssuer + 1;
+    constexpr int kIssuer = kEpilogueWarps + kConverterWarps, kCodesLoader = kIssuer + 1, kDeltaLoader = kIssuer + 2;
     constexpr bool kDirect = PARTS == 1;                                      // delta goes straight into the operand stage
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::kStages; s++) {
             ptx::mbar_init(full_bar(s), kGroupWarps + (kDirect ? 1 : 0));
-            ptx::mbar_init(empty_bar(s), 1 + (kDirect ? kGroupWarps : 0));
+            ptx::mbar_init(empty_bar(s), 1);
+            ptx::mbar_init(read_bar(s), kGroupWarps);
             ptx::mbar_init(peer_bar(s), 1);
         }
-        for (int s = 0; s < S::kRaws; s++) { ptx::mbar_init(raw_full_bar(s), 1); ptx::mbar_init(raw_empty_bar(s), kGroupWarps); }
+        for (int s = 0; s < S::kRaws; s++) { ptx::mbar_init(raw_full_bar(s), kDirect ? 1 : 2); ptx::mbar_init(raw_empty_bar(s), kGroupWarps); }
         for (int a = 0; a < 2; a++) { ptx::mbar_init(tfull_bar(a), 1); ptx::mbar_init(tempty_bar(a), 2 * kEpilogueWarps); }
         *abort_flag = 0;
         ptx::fence_barrier_init();
@@ -270,29 +262,30 @@ ckpt8_wgrad_tc_kernel(const __grid_constant__ CUtensorMap codes_map, const __gri
     const uint32_t tmem = *tmem_slot;
     grid_dependency_wait();
 
-    if (warp == kLoader) {
-        // ------------------------------------------------------------------ TMA loads (one thread)
+    if (warp == kCodesLoader || warp == kDeltaLoader) {
+        // ------------------------------------------------------------------ TMA loads (one thread each for the codes and for delta)
         if (lane == 0) {
-            StageCursor at;
-            int stage = 0, rs = 0;
-            uint32_t phase = 0, rphase = 0;
-            const uint32_t ring = ptx::smem_u32(smem);
-            for (at.start(p, pair); at.valid; at.next(p, pair)) {
-                const WorkItem &w = at.i.w;
-                const int row = (w.begin + at.step) * S::kRows, o = w.mt * kPairTile + rank * 128, i = w.nt * kPairTile + rank * 128;
-                if (!wait_bar(raw_empty_bar(rs), rphase ^ 1u, abort_flag, p.status, 0x100u + B200_E_TIMEOUT)) break;
-                const uint32_t raw = ring + S::kRing + (uint32_t)rs * S::kRaw;
-                ptx::mbar_arrive_expect_tx(raw_full_bar(rs), S::kRaw);
-                ptx::tma_load_2d(raw, &codes_map, raw_full_bar(rs), i, row);
-                if (!kDirect) ptx::tma_load_2d(raw + S::kCodes, &delta_map, raw_full_bar(rs), o, row);
-                if (++rs == S::kRaws) { rs = 0; rphase ^= 1u; }
-                if (kDirect) {
-                    if (!wait_bar(empty_bar(stage), phase ^ 1u, abort_flag, p.status, 0x700u + B200_E_TIMEOUT)) break;
-                    const uint32_t dst = ring + (uint32_t)stage * S::kStage;
-                    ptx::mbar_arrive_expect_tx(full_bar(stage), S::kOperand);
-                    ptx::tma_load_2d(dst, &delta_map, full_bar(stage), o, row);
-                    ptx::tma_load_2d(dst + S::kOperand / 2, &delta_map, full_bar(stage), o + 64, row);
-                    if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
+            const bool codes = warp == kCodesLoader, direct = kDirect && !codes;
+            const int slots = direct ? S::kStages : S::kRaws;
+            const uint32_t base = ptx::smem_u32(smem) + (direct ? 0u : S::kRing + (codes ? 0u : S::kCodes)), pitch = direct ? S::kStage : S::kRaw;
+            const uint32_t full = direct ? full_bar(0) : raw_full_bar(0), empty = direct ? empty_bar(0) : raw_empty_bar(0);
+            const uint32_t bytes = codes ? S::kCodes : direct ? S::kOperand : S::kRaw - S::kCodes;
+            const CUtensorMap *map = codes ? &codes_map : &delta_map;
+            int slot = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            ItemCursor at;
+            for (bool more = at.start(p, pair); more && ok; more = at.next(p, pair)) {
+                const int col = (codes ? at.w.nt : at.w.mt) * kPairTile + rank * 128, end = (at.w.begin + at.w.steps) * S::kRows;
+                for (int row = at.w.begin * S::kRows; row < end; row += S::kRows) {
+                    ok = wait_bar(empty + 8u * slot, phase ^ 1u, abort_flag, p.status, 0x100u + B200_E_TIMEOUT) &&
+                         (!direct || wait_bar(read_bar(slot), phase ^ 1u, abort_flag, p.status, 0x700u + B200_E_TIMEOUT));
+                    if (!ok) break;
+                    const uint32_t dst = base + (uint32_t)slot * pitch, bar = full + 8u * slot;
+                    ptx::mbar_arrive_expect_tx(bar, bytes);
+                    ptx::tma_load_2d(dst, map, bar, col, row);
+                    if (direct) ptx::tma_load_2d(dst + S::kOperand / 2, map, bar, col + 64, row);
+                    if (++slot == slots) { slot = 0; phase ^= 1u; }
                 }
             }
         }
@@ -303,47 +296,106 @@ ckpt8_wgrad_tc_kernel(const __grid_constant__ CUtensorMap codes_map, const __gri
         const int r8 = t >> 4, c8 = t & 15;                                   // delta: row (of 8) and group of eight columns
 
         // exponents of this thread's codes in the group's next stage, loaded while the current one is converted
-        StageCursor ahead;
-        ahead.start(p, pair);
-        for (int k = 0; k < group && ahead.valid; k++) ahead.next(p, pair);
+        ItemCursor ahead;
+        bool more_ahead = ahead.start(p, pair);
+        int step_ahead = group, row_ahead = 0;
+        const uint8_t *src_ahead = nullptr;
         uint32_t exps[S::kCodePasses];
-        auto fetch = [&]() {
-            const size_t i = (size_t)ahead.i.w.nt * kPairTile + rank * 128 + c * 16;
-            const int row = (ahead.i.w.begin + ahead.step) * S::kRows + r;
-            const bool in = ahead.valid && i < p.blocks * kCkptBlock;
-            const uint8_t *src = p.exponents + (size_t)row * p.blocks + i / kCkptBlock;
+        const size_t stride = (size_t)kGroups * S::kRows * p.blocks;
+        auto fetch = [&](bool fresh) {
+            while (more_ahead && step_ahead >= ahead.w.steps) {
+                step_ahead -= ahead.w.steps;
+                more_ahead = ahead.next(p, pair);
+                fresh = true;
+            }
+            if (fresh) {
+                const size_t i = (size_t)ahead.w.nt * kPairTile + rank * 128 + c * 16;
+                row_ahead = (ahead.w.begin + step_ahead) * S::kRows + r;
+                src_ahead = p.exponents + (size_t)row_ahead * p.blocks + i / kCkptBlock;
+                if (!more_ahead || i >= p.blocks * kCkptBlock) row_ahead = p.rows;       // nothing to load
+            }
 #pragma unroll
             for (int k = 0; k < S::kCodePasses; k++) {
                 exps[k] = 0;
-                if (in && row + 16 * k < p.rows) exps[k] = __ldg(src + (size_t)(16 * k) * p.blocks);
+                if (row_ahead + 16 * k < p.rows) exps[k] = __ldg(src_ahead + (size_t)(16 * k) * p.blocks);
             }
+            if (row_ahead < p.rows) row_ahead += kGroups * S::kRows;
+            src_ahead += stride;
+            step_ahead += kGroups;
         };
-        fetch();
+        fetch(true);
 
-        StageCursor at;
-        int turn_of = 0, stage = 0, rs = 0;
-        uint32_t phase = 0, rphase = 0;
-        bool ok = true;
         float sums[8] = {};
-        for (at.start(p, pair); at.valid;) {
-            const bool bias = p.dbias && at.i.w.nt == 0;
-            if (turn_of == group) {
-                if (ok) ok = __all_sync(0xffffffffu, wait_bar(raw_full_bar(rs), rphase, abort_flag, p.status, 0x800u + B200_E_TIMEOUT));
-                if (ok) ok = __all_sync(0xffffffffu, wait_bar(empty_bar(stage), phase ^ 1u, abort_flag, p.status, 0x900u + B200_E_TIMEOUT));
+        // the end of a tile: its bias gradient
+        auto finish = [&](const WorkItem &w) {
+            // the thirty-two row slots (two a warp, joined by a shuffle), then one thread per column
+#pragma unroll
+            for (int x = 0; x < 8; x++) sums[x] += __shfl_xor_sync(0xffffffffu, sums[x], 16);
+            if (lane < 16) {
+#pragma unroll
+                for (int x = 0; x < 8; x++) bias_sums[(warp - kEpilogueWarps) * 128 + c8 * 8 + x] = sums[x];
+            }
+            asm volatile("bar.sync 1, %0;" ::"n"(kConverters) : "memory");
+            if (group == 0) {
+                float s = 0.f;
+#pragma unroll
+                for (int k = 0; k < kConverterWarps; k++) s += bias_sums[k * 128 + t];
+                const int o = w.mt * kPairTile + rank * 128 + t;
+                if (w.unit >= 0) p.partial[(size_t)w.unit * kUnitFloats + kPairTile * kPairTile + rank * 128 + t] = s;
+                else if (o < p.out) p.dbias[o] = p.accumulate ? p.dbias[o] + s : s;
+            }
+            asm volatile("bar.sync 1, %0;" ::"n"(kConverters) : "memory");
+#pragma unroll
+            for (int x = 0; x < 8; x++) sums[x] = 0.f;
+        };
+
+        ItemCursor at;
+        bool more = at.start(p, pair), ok = true;
+        int step = group, stage = group, rs = group;
+        uint32_t phase = 0, rphase = 0;
+        auto wrap = [&]() {
+            if (rs >= S::kRaws) { rs -= S::kRaws; rphase ^= 1u; }
+            if (stage >= S::kStages) { stage -= S::kStages; phase ^= 1u; }
+        };
+        while (true) {
+            bool bias = p.dbias && at.w.nt == 0;
+            while (more && step >= at.w.steps) {         // every group passes the end of every item, in the same order
+                step -= at.w.steps;
+                if (bias && at.w.last) finish(at.w);
+                more = at.next(p, pair);
+                bias = p.dbias && at.w.nt == 0;
+            }
+            if (!more) break;
+            if (ok) {
+                if (lane == 0) ok = wait_bar(raw_full_bar(rs), rphase, abort_flag, p.status, 0x800u + B200_E_TIMEOUT);
+                ok = __shfl_sync(0xffffffffu, ok, 0);
+                const uint8_t *raw = smem + S::kRing + (uint32_t)rs * S::kRaw;
+                // Chunks 2c and 2c + 1 of a row's sixteen.  The threads of the row's second half take theirs in the other order, so that
+                // no two of a store meet in a bank.
+                const int block = c >> 2, chunk = ((2 * c) & 7) + block;
+                uint2 q[S::kCodePasses][2];
                 if (ok) {
-                    const uint8_t *raw = smem + S::kRing + (uint32_t)rs * S::kRaw;
+#pragma unroll
+                    for (int k = 0; k < S::kCodePasses; k++) {
+                        const uint4 v = *reinterpret_cast<const uint4 *>(raw + k * 2048 + t * 16);
+                        q[k][0] = block ? make_uint2(v.z, v.w) : make_uint2(v.x, v.y);
+                        q[k][1] = block ? make_uint2(v.x, v.y) : make_uint2(v.z, v.w);
+                    }
+                    if (kDirect) {
+                        __syncwarp();
+                        if (lane == 0) ptx::mbar_arrive(raw_empty_bar(rs));
+                    }
+                    if (lane == 0) ok = wait_bar(empty_bar(stage), phase ^ 1u, abort_flag, p.status, 0x900u + B200_E_TIMEOUT);
+                    ok = __shfl_sync(0xffffffffu, ok, 0);
+                }
+                if (ok) {
                     uint8_t *tile = smem + (uint32_t)stage * S::kStage;
-                    // chunks 2c and 2c + 1 of a row's sixteen; half the threads write theirs in the other order, so that no two meet
-                    // in a bank
-                    const int block = c >> 2, chunk = ((2 * c) & 7) + block;
                     uint8_t *b = tile + PARTS * S::kOperand + block * (S::kRows * 128) + r * 128;
                     const uint32_t first = (uint32_t)((chunk ^ (r & 7)) << 4), second = (uint32_t)(((chunk + 1 - 2 * block) ^ (r & 7)) << 4);
 #pragma unroll
                     for (int k = 0; k < S::kCodePasses; k++) {
-                        const uint4 q = *reinterpret_cast<const uint4 *>(raw + k * 2048 + t * 16);
-                        const uint4 v0 = decode8(make_uint2(q.x, q.y), exps[k]), v1 = decode8(make_uint2(q.z, q.w), exps[k]);
-                        *reinterpret_cast<uint4 *>(b + k * 2048 + first) = block ? v1 : v0;
-                        *reinterpret_cast<uint4 *>(b + k * 2048 + second) = block ? v0 : v1;
+                        *reinterpret_cast<uint4 *>(b + k * 2048 + first) = decode8(q[k][0], exps[k]);
+                        *reinterpret_cast<uint4 *>(b + k * 2048 + second) = decode8(q[k][1], exps[k]);
                     }
                     if (!kDirect) {
                         uint8_t *a = tile + (c8 >> 3) * (S::kRows * 128) + r8 * 128 + (((c8 & 7) ^ (r8 & 7)) << 4);
@@ -383,11 +435,16 @@ ckpt8_wgrad_tc_kernel(const __grid_constant__ CUtensorMap codes_map, const __gri
                     }
                     ptx::fence_proxy_async();
                     __syncwarp();
-                    if (lane == 0) { ptx::mbar_arrive(full_bar(stage)); ptx::mbar_arrive(raw_empty_bar(rs)); }
+                    if (lane == 0) {
+                        if (!kDirect) ptx::mbar_arrive(raw_empty_bar(rs));
+                        ptx::mbar_arrive(full_bar(stage));
+                    }
                     if (kDirect) {
-                        // the bias gradient sums delta from the operand tile, which stays until every warp of the group has arrived here
+                        // the bias gradient sums delta from the operand tile, which is not loaded again until every warp of the group has
+                        // arrived here
                         if (bias) {
-                            ok = __all_sync(0xffffffffu, wait_bar(full_bar(stage), phase, abort_flag, p.status, 0xa00u + B200_E_TIMEOUT));
+                            if (lane == 0) ok = wait_bar(full_bar(stage), phase, abort_flag, p.status, 0xa00u + B200_E_TIMEOUT);
+                            ok = __shfl_sync(0xffffffffu, ok, 0);
                             if (ok) {
 #pragma unroll
                                 for (int k = 0; k < S::kDeltaPasses; k++) {
@@ -400,51 +457,32 @@ ckpt8_wgrad_tc_kernel(const __grid_constant__ CUtensorMap codes_map, const __gri
                             }
                             __syncwarp();
                         }
-                        if (lane == 0) ptx::mbar_arrive(empty_bar(stage));
+                        if (lane == 0) ptx::mbar_arrive(read_bar(stage));
                     }
                 }
-#pragma unroll 1
-                for (int k = 0; k < kGroups && ahead.valid; k++) ahead.next(p, pair);
-                fetch();
             }
-            if (++turn_of == kGroups) turn_of = 0;
-            if (++rs == S::kRaws) { rs = 0; rphase ^= 1u; }
-            if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
-            if (bias && at.ends_tile()) {
-                // the thirty-two row slots (two a warp, joined by a shuffle), then one thread per column
-#pragma unroll
-                for (int x = 0; x < 8; x++) sums[x] += __shfl_xor_sync(0xffffffffu, sums[x], 16);
-                if (lane < 16) {
-#pragma unroll
-                    for (int x = 0; x < 8; x++) bias_sums[(warp - kEpilogueWarps) * 128 + c8 * 8 + x] = sums[x];
-                }
-                asm volatile("bar.sync 1, %0;" ::"n"(kConverters) : "memory");
-                if (group == 0) {
-                    float s = 0.f;
-#pragma unroll
-                    for (int k = 0; k < kConverterWarps; k++) s += bias_sums[k * 128 + t];
-                    const int o = at.i.w.mt * kPairTile + rank * 128 + t;
-                    if (at.i.w.unit >= 0) p.partial[(size_t)at.i.w.unit * kUnitFloats + kPairTile * kPairTile + rank * 128 + t] = s;
-                    else if (o < p.out) p.dbias[o] = p.accumulate ? p.dbias[o] + s : s;
-                }
-                asm volatile("bar.sync 1, %0;" ::"n"(kConverters) : "memory");
-#pragma unroll
-                for (int x = 0; x < 8; x++) sums[x] = 0.f;
-            }
-            at.next(p, pair);
+            fetch(false);
+            step += kGroups;
+            rs += kGroups;
+            stage += kGroups;
+            wrap();
         }
     } else if (warp == kIssuer) {
         // ------------------------------------------------------------------ MMA issuer (one thread of the leader)
-        // The peer's thread passes its full stages on.  The producers do not arrive in the other CTA themselves: an arrival with
-        // cluster scope waits for everything its thread has under way, the loads of the stages ahead among them.
+        // The peer's thread passes its full stages on.  (An arrival with .release.cluster here took some 1500 cycles, more than all
+        // the work on a stage, 900 us in place of MEASURE at 8192 rows, 4096 x 4096.  The tile itself stays in the peer's shared
+        // memory, where its writers have made it visible to the tensor core before they arrived.)
         if (rank == 1 && lane == 0) {
-            StageCursor at;
+            ItemCursor at;
             int stage = 0;
             uint32_t phase = 0;
-            for (at.start(p, pair); at.valid; at.next(p, pair)) {
-                if (!wait_bar(full_bar(stage), phase, abort_flag, p.status, 0x500u + B200_E_TIMEOUT)) break;
-                ptx::mbar_arrive_cluster(peer_bar(stage), 0);
-                if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
+            bool ok = true;
+            for (bool more = at.start(p, pair); more && ok; more = at.next(p, pair)) {
+                for (int step = 0; step < at.w.steps; step++) {
+                    if (!(ok = wait_bar(full_bar(stage), phase, abort_flag, p.status, 0x500u + B200_E_TIMEOUT))) break;
+                    ptx::mbar_arrive_remote(peer_bar(stage), 0);
+                    if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
+                }
             }
         }
         if (rank == 0 && lane == 0) {
@@ -456,12 +494,12 @@ ckpt8_wgrad_tc_kernel(const __grid_constant__ CUtensorMap codes_map, const __gri
             for (bool more = at.start(p, pair); ok && more; more = at.next(p, pair), n++) {
                 const WorkItem w = at.w;
                 const int acc = n % kAccumulators;
-                if (!wait_bar<true>(tempty_bar(acc), ((uint32_t)(n / kAccumulators) & 1u) ^ 1u, abort_flag, p.status, 0x200u + B200_E_TIMEOUT)) break;
+                if (!wait_bar(tempty_bar(acc), ((uint32_t)(n / kAccumulators) & 1u) ^ 1u, abort_flag, p.status, 0x200u + B200_E_TIMEOUT)) break;
                 ptx::tc_fence_after();
                 const uint32_t d = tmem + (uint32_t)acc * 256u;
                 for (int step = 0; step < w.steps; step++) {
                     ok = wait_bar(full_bar(stage), phase, abort_flag, p.status, 0x300u + B200_E_TIMEOUT) &&
-                         wait_bar<true>(peer_bar(stage), phase, abort_flag, p.status, 0x600u + B200_E_TIMEOUT);
+                         wait_bar(peer_bar(stage), phase, abort_flag, p.status, 0x600u + B200_E_TIMEOUT);
                     if (!ok) break;
                     ptx::tc_fence_after();
                     const uint64_t a = desc + (uint64_t)((uint32_t)stage * S::kStage >> 4), b = a + (PARTS * S::kOperand >> 4);
@@ -503,7 +541,7 @@ ckpt8_wgrad_tc_kernel(const __grid_constant__ CUtensorMap codes_map, const __gri
                 if (col + 32 == kPairTile) {             // the accumulator is read: the next tile may have it
                     ptx::tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) ptx::mbar_arrive_cluster(tempty_bar(acc), 0);
+                    if (lane == 0) ptx::mbar_arrive_remote(tempty_bar(acc), 0);
                 }
                 // each thread holds 32 columns of a row; turned around, eight threads write 128 bytes of a row together
 #pragma unroll
@@ -594,7 +632,7 @@ struct WgradPlan { int tiles_m, tiles_n, steps, pairs, waves, first_tail, tail_u
 static WgradPlan wgrad_plan(int parts, int rows, int out, size_t in)
 {
     WgradPlan w;
-    const int depth = parts == 1 ? 64 : 32;
+    const int depth = parts == 3 ? TcShape<float, 3>::kRows : parts == 2 ? TcShape<__half, 2>::kRows : TcShape<__nv_bfloat16, 1>::kRows;
     w.tiles_m = ceil_div(out, kPairTile);
     w.tiles_n = (int)((in + kPairTile - 1) / kPairTile);
     w.steps = ceil_div(rows, depth);
@@ -603,8 +641,8 @@ static WgradPlan wgrad_plan(int parts, int rows, int out, size_t in)
     w.waves = (int)(tiles / w.pairs);
     w.first_tail = w.waves * w.pairs;
     const int rest = (int)(tiles - w.first_tail);
-    // a unit has at least four stages: below that its partial tile costs more than the stages it saves
-    w.splits = rest ? max(1, min(w.pairs / rest, w.steps / 4)) : 1;
+    // a unit has at least 128 rows: below that its partial tile costs more than the rows it saves
+    w.splits = rest ? max(1, min(w.pairs / rest, rows / 128)) : 1;
     w.tail_units = rest * w.splits;
     w.launch_pairs = w.waves ? w.pairs : w.tail_units;
     return w;

@@ -187,28 +187,6 @@ __device__ __forceinline__ void mma_bf16_pair(uint32_t d_tmem, uint64_t adesc, u
         ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-// Arrival that publishes this CTA's shared-memory writes to the CTA of the pair that owns the barrier, and the wait for it
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar, uint32_t cta)
-{
-    asm volatile(
-        "{\n\t.reg .b32 ra;\n\t"
-        "mapa.shared::cluster.u32 ra, %0, %1;\n\t"
-        "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [ra];\n\t}"
-        ::"r"(bar), "r"(cta)
-        : "memory");
-}
-__device__ __forceinline__ uint32_t mbar_try_wait_cluster(uint32_t bar, uint32_t parity)
-{
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity), "r"(kMbarSuspendNs)
-        : "memory");
-    return ok;
-}
 // arrive on the mbarrier at this offset in both CTAs of the pair once the issued MMAs have completed
 __device__ __forceinline__ void mma_commit_pair(uint32_t bar)
 {
@@ -243,16 +221,14 @@ __device__ __forceinline__ float to_tf32(float x)
 // A bounded wait: after about a second of polling the kernel records `code` in the status word, raises its abort flag and
 // goes on without the data; every other wait of the block then gives up too.
 constexpr long long kWaitCycles = 2000000000LL;
-template <bool CLUSTER = false>
 __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile int *abort_flag, unsigned *status, unsigned code)
 {
-    auto poll = [&]() { return CLUSTER ? ptx::mbar_try_wait_cluster(bar, parity) : ptx::mbar_try_wait(bar, parity); };
-    if (poll()) return true;
+    if (ptx::mbar_try_wait(bar, parity)) return true;
     const long long t0 = clock64();
     while (true) {
 #pragma unroll 1
         for (int i = 0; i < 128; i++)
-            if (poll()) return true;
+            if (ptx::mbar_try_wait(bar, parity)) return true;
         if (*abort_flag) return false;
         if (clock64() - t0 > kWaitCycles) {
             *abort_flag = 1;
