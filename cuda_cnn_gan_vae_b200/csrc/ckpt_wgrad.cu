@@ -229,8 +229,7 @@ ckpt8_wgrad_tc_kernel(const __grid_constant__ CUtensorMap codes_map, const __gri
     auto raw_empty_bar = [&](int s) { return bar_base + 8u * (3 * S::kStages + S::kRaws + s); };
     auto tfull_bar = [&](int a) { return bar_base + 8u * (3 * S::kStages + 2 * S::kRaws + a); };
     auto tempty_bar = [&](int a) { return bar_base + 8u * (3 * S::kStages + 2 * S::kRaws + 2 + a); };
-    auto read_bar = [&](int s) { return bar_base + 8u * (3 * S::kStages + 2 * S::kRaws + 4 + s); };      // direct delta: its tile has been summed
-    constexpr int kBars = 4 * S::kStages + 2 * S::kRaws + 4;
+    constexpr int kBars = 3 * S::kStages + 2 * S::kRaws + 4;
     static_assert(kBars * 8 + 8 <= 512, "barriers");
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + kBars);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
@@ -243,8 +242,7 @@ ckpt8_wgrad_tc_kernel(const __grid_constant__ CUtensorMap codes_map, const __gri
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::kStages; s++) {
             ptx::mbar_init(full_bar(s), kGroupWarps + (kDirect ? 1 : 0));
-            ptx::mbar_init(empty_bar(s), 1);
-            ptx::mbar_init(read_bar(s), kGroupWarps);
+            ptx::mbar_init(empty_bar(s), 1 + (kDirect ? kGroupWarps : 0));
             ptx::mbar_init(peer_bar(s), 1);
         }
         for (int s = 0; s < S::kRaws; s++) { ptx::mbar_init(raw_full_bar(s), kDirect ? 1 : 2); ptx::mbar_init(raw_empty_bar(s), kGroupWarps); }
@@ -278,9 +276,7 @@ ckpt8_wgrad_tc_kernel(const __grid_constant__ CUtensorMap codes_map, const __gri
             for (bool more = at.start(p, pair); more && ok; more = at.next(p, pair)) {
                 const int col = (codes ? at.w.nt : at.w.mt) * kPairTile + rank * 128, end = (at.w.begin + at.w.steps) * S::kRows;
                 for (int row = at.w.begin * S::kRows; row < end; row += S::kRows) {
-                    ok = wait_bar(empty + 8u * slot, phase ^ 1u, abort_flag, p.status, 0x100u + B200_E_TIMEOUT) &&
-                         (!direct || wait_bar(read_bar(slot), phase ^ 1u, abort_flag, p.status, 0x700u + B200_E_TIMEOUT));
-                    if (!ok) break;
+                    if (!(ok = wait_bar(empty + 8u * slot, phase ^ 1u, abort_flag, p.status, 0x100u + B200_E_TIMEOUT))) break;
                     const uint32_t dst = base + (uint32_t)slot * pitch, bar = full + 8u * slot;
                     ptx::mbar_arrive_expect_tx(bar, bytes);
                     ptx::tma_load_2d(dst, map, bar, col, row);
@@ -457,7 +453,7 @@ ckpt8_wgrad_tc_kernel(const __grid_constant__ CUtensorMap codes_map, const __gri
                             }
                             __syncwarp();
                         }
-                        if (lane == 0) ptx::mbar_arrive(read_bar(stage));
+                        if (lane == 0) ptx::mbar_arrive(empty_bar(stage));
                     }
                 }
             }

@@ -273,3 +273,17 @@ def test_refusals(ops):
         with pytest.raises(B):
             bad()
     ops.stream_status()
+
+
+@pytest.mark.parametrize("kind,rows,n,out", [("bfloat16", 8192, 2048, 1024), ("float32", 2000, 1500, 700), ("float16", 1000, 513, 300)])
+def test_wgrad_repeats_bit_for_bit(ops, kind, rows, n, out):
+    """Many launches in a row: no wait of the kernel gives up, and the result is the same every time."""
+    c = ops.Checkpoint8.empty(rows, n).store(torch.randn(rows, n, device="cuda"))
+    delta = torch.randn(rows, out, device="cuda").to(getattr(torch, kind))
+    first = None
+    for i in range(60):
+        dw, db = torch.empty(out, n, device="cuda"), torch.empty(out, device="cuda")
+        ops.checkpoint_wgrad(dw, db, delta, c, accumulate=False)
+        first = first or (dw, db)
+        assert i % 20 or (torch.equal(dw, first[0]) and torch.equal(db, first[1]))
+    ops.stream_status()
