@@ -8,47 +8,103 @@
 
 namespace b200 {
 
-// One warp per block of 32 values, one value per lane.
-template <typename T>
+// Store and load are bound by memory.  A warp takes kSpans spans at a time, a span being V neighbouring values per lane (16
+// bytes, or one value where the rows cannot be read in 16-byte pieces); a block's lanes find its largest magnitude by shuffles.  All
+// loads of the kSpans spans are under way before the first is used.  A dense tensor whose rows are whole blocks is one long
+// row, so the division that finds a span's row is left to ragged ones.
+constexpr int kSpans = 4;
+
+struct CkptShape {
+    size_t total, spans, n, blocks, pitch;      // spans in all and per row
+    int one_row;
+};
+__device__ __forceinline__ void span_at(const CkptShape &g, size_t i, size_t &row, size_t &span)
+{
+    if (g.one_row) { row = 0; span = i; }
+    else if (g.total <= 0xffffffffu) { row = (uint32_t)i / (uint32_t)g.spans; span = i - row * g.spans; }
+    else { row = i / g.spans; span = i - row * g.spans; }
+}
+
+template <typename T, int V>
 __global__ void __launch_bounds__(256) ckpt8_store_kernel(int8_t *__restrict__ codes, uint8_t *__restrict__ exponents, const T *__restrict__ x,
-                                                          size_t total, size_t blocks, size_t n, size_t pitch, int keep_sign)
+                                                          const __grid_constant__ CkptShape g, int keep_sign)
 {
     grid_dependency_wait();
     const int lane = threadIdx.x & 31;
-    const size_t step = (size_t)gridDim.x * (blockDim.x >> 5);
-    for (size_t i = (size_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); i < total; i += step) {
-        const size_t row = i / blocks, col = (i - row * blocks) * kCkptBlock + lane;
-        const float v = col < n ? to_float(x[row * pitch + col]) : 0.f;
-        const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(v) & 0x7fffffffu);
-        const uint32_t b = ckpt8_exponent(top);
-        codes[i * kCkptBlock + lane] = (int8_t)ckpt8_code(v, ckpt8_scale(b), b, keep_sign != 0);
-        if (lane == 0) exponents[i] = (uint8_t)b;
+    const size_t warps = (size_t)gridDim.x * 8;
+    for (size_t first = (size_t)blockIdx.x * 8 + (threadIdx.x >> 5); first * kSpans < g.total; first += warps) {
+        Pack<T, V> in[kSpans];
+        size_t row[kSpans], col[kSpans];
+#pragma unroll
+        for (int k = 0; k < kSpans; k++) {
+            size_t span;
+            const size_t i = first * kSpans + k;
+            span_at(g, i < g.total ? i : g.total - 1, row[k], span);
+            col[k] = (span * 32 + lane) * V;
+            if (i < g.total && col[k] < g.n) {
+                in[k] = load_pack<T, V>(x + row[k] * g.pitch + col[k]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; j++) in[k].v[j] = from_float<T>(0.f);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kSpans; k++) {
+            if (first * kSpans + k >= g.total) break;
+            float f[V];
+#pragma unroll
+            for (int j = 0; j < V; j++) f[j] = to_float(in[k].v[j]);
+            const uint32_t b = ckpt8_exponent(ckpt8_top<V>(f));
+            const size_t block = col[k] / kCkptBlock;
+            if (block < g.blocks) {
+                ckpt8_put<V>(codes + row[k] * g.blocks * kCkptBlock + col[k], f, b, keep_sign != 0);
+                if (col[k] % kCkptBlock == 0) exponents[row[k] * g.blocks + block] = (uint8_t)b;
+            }
+        }
     }
 }
 
 // A value beyond the range of fp16 reads as the largest finite number (only the rounding of the code can bring it there).
-template <typename T> __device__ __forceinline__ T ckpt8_out(float v) { return from_float<T>(v); }
-template <> __device__ __forceinline__ __half ckpt8_out<__half>(float v)
-{
-    if (fabsf(v) > 65504.f && !isinf(v)) v = copysignf(65504.f, v);
-    return __float2half_rn(v);
-}
+template <typename T> __device__ __forceinline__ float ckpt8_clip(float v) { return v; }
+template <> __device__ __forceinline__ float ckpt8_clip<__half>(float v) { return fabsf(v) > 65504.f && !isinf(v) ? copysignf(65504.f, v) : v; }
 
 // FUNC < 0 reads the values back; otherwise out = f'(value) * error
-template <typename T>
+template <typename T, int V, int FUNC>
 __global__ void __launch_bounds__(256) ckpt8_load_kernel(T *out, const int8_t *__restrict__ codes, const uint8_t *__restrict__ exponents,
-                                                         const T *error, size_t total, size_t blocks, size_t n, size_t pitch,
-                                                         size_t error_pitch, int func, double slope)
+                                                         const T *error, const __grid_constant__ CkptShape g, size_t error_pitch, double slope)
 {
     grid_dependency_wait();
     const int lane = threadIdx.x & 31;
-    const size_t step = (size_t)gridDim.x * (blockDim.x >> 5);
-    for (size_t i = (size_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); i < total; i += step) {
-        const size_t row = i / blocks, col = (i - row * blocks) * kCkptBlock + lane;
-        if (col >= n) continue;
-        const float v = ckpt8_value(codes[i * kCkptBlock + lane], ckpt8_unit(exponents[i]));
-        if (func < 0) out[row * pitch + col] = ckpt8_out<T>(v);
-        else out[row * pitch + col] = from_float<T>(act_derivative(v, func, slope) * to_float(error[row * error_pitch + col]));
+    const size_t warps = (size_t)gridDim.x * 8;
+    for (size_t first = (size_t)blockIdx.x * 8 + (threadIdx.x >> 5); first * kSpans < g.total; first += warps) {
+        CkptCodes<V> c[kSpans];
+        uint32_t b[kSpans];
+        Pack<T, V> e[kSpans];
+        size_t row[kSpans], col[kSpans];
+#pragma unroll
+        for (int k = 0; k < kSpans; k++) {
+            size_t span;
+            const size_t i = first * kSpans + k;
+            span_at(g, i < g.total ? i : g.total - 1, row[k], span);
+            col[k] = i < g.total ? (span * 32 + lane) * V : g.n;
+            if (col[k] < g.n) {
+                c[k] = ckpt8_get<V>(codes + row[k] * g.blocks * kCkptBlock + col[k]);
+                b[k] = exponents[row[k] * g.blocks + col[k] / kCkptBlock];
+                if (FUNC >= 0) e[k] = load_pack<T, V>(error + row[k] * error_pitch + col[k]);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kSpans; k++) {
+            if (col[k] >= g.n) continue;
+            float f[V];
+            ckpt8_values<V>(f, c[k], b[k]);
+#pragma unroll
+            for (int j = 0; j < V; j++) {
+                if (FUNC < 0) f[j] = ckpt8_clip<T>(f[j]);
+                else f[j] = act_derivative(f[j], FUNC, slope) * to_float(e[k].v[j]);
+            }
+            store_pack<T, V>(out + row[k] * g.pitch + col[k], f);
+        }
     }
 }
 
@@ -74,18 +130,63 @@ int check_matrix(const void *p, int type, int rows, size_t n, size_t pitch, cons
     return B200_OK;
 }
 
-static unsigned ckpt8_grid(size_t total)
+static CkptShape ckpt8_shape(int rows, size_t n, size_t pitch, int v, bool same_pitch)
 {
-    const size_t want = (total + 7) / 8, most = (size_t)sm_count() * 8;
+    CkptShape g;
+    g.one_row = rows == 1 || (pitch == n && same_pitch && n % kCkptBlock == 0);
+    g.n = g.one_row ? n * (size_t)rows : n;
+    g.blocks = ckpt8_blocks(g.n);
+    g.pitch = pitch;
+    g.spans = (g.blocks * kCkptBlock + 32 * v - 1) / (32 * v);      // whole blocks: the last one is filled up with zeros
+    g.total = g.one_row ? g.spans : g.spans * (size_t)rows;
+    return g;
+}
+static unsigned ckpt8_grid(const CkptShape &g)
+{
+    const size_t want = (g.total + 8 * kSpans - 1) / (8 * kSpans), most = (size_t)sm_count() * 8;
     return (unsigned)(want < most ? want : most);
 }
 
-template <typename T>
-static void launch_load(T *out, const int8_t *codes, const uint8_t *exponents, const T *error, int rows, size_t n, size_t pitch, size_t error_pitch,
-                        int func, double slope, cudaStream_t s)
+template <typename T, int V>
+static void launch_load(const Launch &launch, T *out, const int8_t *codes, const uint8_t *exponents, const T *error, const CkptShape &g, size_t error_pitch,
+                        int func, double slope)
 {
-    const size_t blocks = ckpt8_blocks(n), total = (size_t)rows * blocks;
-    Launch(ckpt8_grid(total), 256, 0, s)(ckpt8_load_kernel<T>, out, codes, exponents, error, total, blocks, n, pitch, error_pitch, func, slope);
+#define B200_CKPT8_LOAD(F) launch(ckpt8_load_kernel<T, V, F>, out, codes, exponents, error, g, error_pitch, slope)
+    switch (func) {
+    case B200_ACT_SIGMOID: B200_CKPT8_LOAD(B200_ACT_SIGMOID); break;
+    case B200_ACT_RELU: B200_CKPT8_LOAD(B200_ACT_RELU); break;
+    case B200_ACT_LEAKY_RELU: B200_CKPT8_LOAD(B200_ACT_LEAKY_RELU); break;
+    case B200_ACT_LINEAR: B200_CKPT8_LOAD(B200_ACT_LINEAR); break;
+    case B200_ACT_TANH: B200_CKPT8_LOAD(B200_ACT_TANH); break;
+    case B200_ACT_GELU: B200_CKPT8_LOAD(B200_ACT_GELU); break;
+    default: B200_CKPT8_LOAD(-1); break;
+    }
+#undef B200_CKPT8_LOAD
+}
+
+template <typename T>
+static int load_typed(T *out, const int8_t *codes, const uint8_t *exponents, const T *error, int type, int rows, size_t n, size_t pitch, size_t error_pitch,
+                      int func, double slope, cudaStream_t s)
+{
+    const bool wide = wide_rows(out, type, n, pitch) && (!error || wide_rows(error, type, n, error_pitch));
+    const CkptShape g = ckpt8_shape(rows, n, pitch, wide ? kWide<T> : 1, !error || error_pitch == pitch);
+    const Launch launch(ckpt8_grid(g), 256, 0, s);
+    if (wide) launch_load<T, kWide<T>>(launch, out, codes, exponents, error, g, error_pitch, func, slope);
+    else launch_load<T, 1>(launch, out, codes, exponents, error, g, error_pitch, func, slope);
+    B200_LAUNCH_CHECK();
+    return B200_OK;
+}
+
+template <typename T>
+static int store_typed(int8_t *codes, uint8_t *exponents, const T *x, int type, int rows, size_t n, size_t pitch, int keep_sign, cudaStream_t s)
+{
+    const bool wide = wide_rows(x, type, n, pitch);
+    const CkptShape g = ckpt8_shape(rows, n, pitch, wide ? kWide<T> : 1, true);
+    const Launch launch(ckpt8_grid(g), 256, 0, s);
+    if (wide) launch(ckpt8_store_kernel<T, kWide<T>>, codes, exponents, x, g, keep_sign);
+    else launch(ckpt8_store_kernel<T, 1>, codes, exponents, x, g, keep_sign);
+    B200_LAUNCH_CHECK();
+    return B200_OK;
 }
 
 }  // namespace b200
@@ -101,24 +202,18 @@ int b200_ckpt8_store(int8_t *codes, uint8_t *exponents, const void *x, int type,
     int r = check_rows(rows, n);
     if (r || rows == 0) return r;
     if ((r = check_ckpt8(codes, exponents)) || (r = check_matrix(x, type, rows, n, x_pitch, "x"))) return r;
-    const size_t blocks = ckpt8_blocks(n), total = (size_t)rows * blocks;
-    const Launch launch(ckpt8_grid(total), 256, 0, ST(stream));
-    if (type == B200_F32) launch(ckpt8_store_kernel<float>, codes, exponents, (const float *)x, total, blocks, n, x_pitch, keep_sign);
-    else if (type == B200_BF16) launch(ckpt8_store_kernel<__nv_bfloat16>, codes, exponents, (const __nv_bfloat16 *)x, total, blocks, n, x_pitch, keep_sign);
-    else launch(ckpt8_store_kernel<__half>, codes, exponents, (const __half *)x, total, blocks, n, x_pitch, keep_sign);
-    B200_LAUNCH_CHECK();
-    return B200_OK;
+    if (type == B200_F32) return store_typed(codes, exponents, (const float *)x, type, rows, n, x_pitch, keep_sign, ST(stream));
+    if (type == B200_BF16) return store_typed(codes, exponents, (const __nv_bfloat16 *)x, type, rows, n, x_pitch, keep_sign, ST(stream));
+    return store_typed(codes, exponents, (const __half *)x, type, rows, n, x_pitch, keep_sign, ST(stream));
 }
 
 static int load_impl(void *out, const int8_t *codes, const uint8_t *exponents, const void *error, int type, int rows, size_t n, size_t out_pitch,
                      size_t error_pitch, int func, double slope, void *stream)
 {
     cudaStream_t s = ST(stream);
-    if (type == B200_F32) launch_load((float *)out, codes, exponents, (const float *)error, rows, n, out_pitch, error_pitch, func, slope, s);
-    else if (type == B200_BF16) launch_load((__nv_bfloat16 *)out, codes, exponents, (const __nv_bfloat16 *)error, rows, n, out_pitch, error_pitch, func, slope, s);
-    else launch_load((__half *)out, codes, exponents, (const __half *)error, rows, n, out_pitch, error_pitch, func, slope, s);
-    B200_LAUNCH_CHECK();
-    return B200_OK;
+    if (type == B200_F32) return load_typed((float *)out, codes, exponents, (const float *)error, type, rows, n, out_pitch, error_pitch, func, slope, s);
+    if (type == B200_BF16) return load_typed((__nv_bfloat16 *)out, codes, exponents, (const __nv_bfloat16 *)error, type, rows, n, out_pitch, error_pitch, func, slope, s);
+    return load_typed((__half *)out, codes, exponents, (const __half *)error, type, rows, n, out_pitch, error_pitch, func, slope, s);
 }
 
 int b200_ckpt8_load(void *out, const int8_t *codes, const uint8_t *exponents, int type, int rows, size_t n, size_t out_pitch, void *stream)

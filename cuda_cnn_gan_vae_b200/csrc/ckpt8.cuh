@@ -48,4 +48,51 @@ __device__ __forceinline__ int ckpt8_code(float x, CkptScale s, uint32_t b, bool
 __device__ __forceinline__ float ckpt8_unit(uint32_t b) { return __uint_as_float(b << 23); }
 __device__ __forceinline__ float ckpt8_value(int q, float unit) { return ((float)q * 0.015625f) * unit; }
 
+// A group of lanes that hold V neighbouring values each shares a block: its largest magnitude.
+template <int V> __device__ __forceinline__ uint32_t ckpt8_top(const float *f)
+{
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < V; i++) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
+    if constexpr (V == 1) return __reduce_max_sync(0xffffffffu, top);
+#pragma unroll
+    for (int o = 1; o < kCkptBlock / V; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    return top;
+}
+
+// codes of V values at dst (a multiple of V bytes), and the values of V codes
+template <int V> __device__ __forceinline__ void ckpt8_put(int8_t *dst, const float *f, uint32_t b, bool keep_sign)
+{
+    const CkptScale s = ckpt8_scale(b);
+    if constexpr (V == 1) {
+        *dst = (int8_t)ckpt8_code(f[0], s, b, keep_sign);
+    } else {
+        uint32_t w[V / 4];
+#pragma unroll
+        for (int i = 0; i < V / 4; i++) {
+            uint32_t q[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) q[k] = (uint32_t)ckpt8_code(f[4 * i + k], s, b, keep_sign);
+            w[i] = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+        }
+        if constexpr (V == 4) *reinterpret_cast<uint32_t *>(dst) = w[0];
+        else *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0], w[1]);
+    }
+}
+template <int V> struct CkptCodes { uint32_t w[V <= 4 ? 1 : V / 4]; };
+template <int V> __device__ __forceinline__ CkptCodes<V> ckpt8_get(const int8_t *src)
+{
+    CkptCodes<V> c;
+    if constexpr (V == 1) c.w[0] = (uint32_t)(int)*src;
+    else if constexpr (V == 4) c.w[0] = *reinterpret_cast<const uint32_t *>(src);
+    else { const uint2 u = *reinterpret_cast<const uint2 *>(src); c.w[0] = u.x; c.w[1] = u.y; }
+    return c;
+}
+template <int V> __device__ __forceinline__ void ckpt8_values(float *f, CkptCodes<V> c, uint32_t b)
+{
+    const float unit = ckpt8_unit(b);
+#pragma unroll
+    for (int i = 0; i < V; i++) f[i] = ckpt8_value(V == 1 ? (int)c.w[0] : (int)(int8_t)(c.w[i / 4] >> (8 * (i & 3))), unit);
+}
+
 }  // namespace b200

@@ -556,14 +556,13 @@ def ln_backward(dy, x, mean, rstd, gamma, dgamma, dbeta, create_delta_weight=Tru
     else:
         x_pitch = _like(x, "x", (kind, rows, n), "dy")[3]
         x_ptr, mean_ptr = x.data_ptr(), _param(mean, rows, "mean").data_ptr()
-    dg = db = ws = None
-    size = 0
+    dg = db = None
     if create_delta_weight:
         dg, db = _param(dgamma, n, "dgamma").data_ptr(), _param(dbeta, n, "dbeta").data_ptr()
-        workspace, size = _workspace(load().b200_ln_backward_workspace(rows, n), workspace, "ln_backward")
-        ws = workspace.data_ptr()
+    workspace, size = _workspace(load().b200_ln_backward_workspace(rows, n), workspace, "ln_backward")
     _check(load().b200_ln_backward(dx.data_ptr(), dg, db, dy.data_ptr(), x_ptr, mean_ptr, rstd.data_ptr(), codes, exponents, gamma.data_ptr(),
-                                   kind, rows, n, dx_pitch, dy_pitch, x_pitch, int(create_delta_weight), int(accumulate), ws, size, _stream()))
+                                   kind, rows, n, dx_pitch, dy_pitch, x_pitch, int(create_delta_weight), int(accumulate),
+                                   workspace.data_ptr(), size, _stream()))
     return dx
 
 

@@ -343,8 +343,7 @@ int b200_ln_forward(void *y, float *mean, float *rstd, int8_t *codes, uint8_t *e
                     const float *beta, int type, int rows, size_t n, size_t x_pitch, size_t y_pitch, float eps, void *stream);
 /* Backward pass: with g = dy * gamma, dx = rstd * (g - mean(g) - xhat * mean(g * xhat)); create_delta_weight != 0 also forms
  * dgamma (+)= sum over rows of dy * xhat and dbeta (+)= sum over rows of dy (accumulate != 0: added to what is there).  xhat
- * comes from x with mean and rstd, or (x NULL) from the checkpoint; mean is then not read.  dx may be dy or x.  The workspace
- * is used only with create_delta_weight. */
+ * comes from x with mean and rstd, or (x NULL) from the checkpoint; mean is then not read.  dx may be dy or x. */
 size_t b200_ln_backward_workspace(int rows, size_t n);
 int b200_ln_backward(void *dx, float *dgamma, float *dbeta, const void *dy, const void *x, const float *mean, const float *rstd,
                      const int8_t *codes, const uint8_t *exponents, const float *gamma, int type, int rows, size_t n,
