@@ -24,24 +24,25 @@ __device__ __forceinline__ uint32_t ckpt8_exponent(uint32_t top)
     return max(e, 1u) + up;                                  // subnormals share the exponent of the smallest normal numbers
 }
 
-// 2^(133-b) as a product of two factors, each a normal number for every b
-struct CkptScale { float first, second; };
-__device__ __forceinline__ CkptScale ckpt8_scale(uint32_t b)
+// Codes of V values.  x * 2^(133-b) + 1.5 * 2^23 in one fused step rounds the quotient to nearest, ties to even, and leaves it in the
+// low byte of the sum.  Three kinds of blocks need more, and are rare enough for a branch: b < 6, where the factor is not a
+// finite number; b = 254, where a code may have to be held at 127; and b = 255, all of whose codes are 0.
+template <int V> __device__ __forceinline__ void ckpt8_codes(uint32_t *q, const float *x, uint32_t b, bool keep_sign)
 {
-    const uint32_t m = max(b, 6u);
-    CkptScale s;
-    s.first = __uint_as_float((260u - m) << 23);             // 2^(133-m), m = 6 .. 255
-    s.second = __uint_as_float((127u + m - b) << 23);        // 2^(m-b)
-    return s;
-}
-
-__device__ __forceinline__ int ckpt8_code(float x, CkptScale s, uint32_t b, bool keep_sign)
-{
-    if (b == 255u) return 0;
-    int q = __float2int_rn(x * s.first * s.second);
-    q = max(-127, min(127, q));
-    if (keep_sign && q == 0 && x < 0.f) q = -1;
-    return q;
+    const float scale = __uint_as_float((260u - max(b, 6u)) << 23);            // 2^(133-b) for b = 6 .. 255
+    if (b >= 6u && b < 254u) {
+#pragma unroll
+        for (int i = 0; i < V; i++) q[i] = __float_as_uint(fmaf(x[i], scale, 12582912.f));
+    } else {
+        const float more = __uint_as_float((127u + max(b, 6u) - b) << 23);     // 2^(6-b) below 6, else 1
+#pragma unroll
+        for (int i = 0; i < V; i++) q[i] = b == 255u ? 0u : (uint32_t)max(-127, min(127, __float2int_rn(x[i] * more * scale)));
+    }
+    if (keep_sign) {
+#pragma unroll
+        for (int i = 0; i < V; i++)
+            if ((q[i] & 0xffu) == 0u && x[i] < 0.f && b != 255u) q[i] = 0xffu;
+    }
 }
 
 // b = 255: 0 * infinity = NaN
@@ -63,18 +64,15 @@ template <int V> __device__ __forceinline__ uint32_t ckpt8_top(const float *f)
 // codes of V values at dst (a multiple of V bytes), and the values of V codes
 template <int V> __device__ __forceinline__ void ckpt8_put(int8_t *dst, const float *f, uint32_t b, bool keep_sign)
 {
-    const CkptScale s = ckpt8_scale(b);
+    uint32_t q[V];
+    ckpt8_codes<V>(q, f, b, keep_sign);
     if constexpr (V == 1) {
-        *dst = (int8_t)ckpt8_code(f[0], s, b, keep_sign);
+        *dst = (int8_t)q[0];
     } else {
         uint32_t w[V / 4];
 #pragma unroll
-        for (int i = 0; i < V / 4; i++) {
-            uint32_t q[4];
-#pragma unroll
-            for (int k = 0; k < 4; k++) q[k] = (uint32_t)ckpt8_code(f[4 * i + k], s, b, keep_sign);
-            w[i] = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
-        }
+        for (int i = 0; i < V / 4; i++)
+            w[i] = __byte_perm(__byte_perm(q[4 * i], q[4 * i + 1], 0x0040), __byte_perm(q[4 * i + 2], q[4 * i + 3], 0x0040), 0x5410);
         if constexpr (V == 4) *reinterpret_cast<uint32_t *>(dst) = w[0];
         else *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0], w[1]);
     }

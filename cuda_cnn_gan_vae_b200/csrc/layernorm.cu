@@ -11,6 +11,8 @@
 #include "types.cuh"
 #include "ckpt8.cuh"
 #include "norm.h"
+#include "kernels.h"
+#include "tc_ptx.cuh"
 #include <cooperative_groups.h>
 
 namespace cg = cooperative_groups;
@@ -280,6 +282,12 @@ struct LnBackward {
     int groups;
     float2 *row_part;            // long rows: [rows][pieces] partial sums of g and g xh
     int pieces;
+    // one-pass form: shared memory of a team's slot for a row of dy, a row of x or codes, and its number of slots
+    uint32_t dy_bytes, x_bytes;
+    int depth;
+    unsigned *status;
+    float *dgamma, *dbeta;       // written directly where there is one group
+    int accumulate;
 };
 
 // V values of dy and of what xh comes from, as loaded
@@ -309,41 +317,162 @@ __device__ __forceinline__ void ln_values(const LnBackward<T> &p, const LnRaw<T,
     for (int j = 0; j < V; j++) dy[j] = to_float(in.dy.v[j]);
 }
 
-constexpr int kLnBack = 8;          // columns of a thread in the one-pass form
+// Rows of up to 8192 values in one pass: a team holds a row, a thread the same eight columns of every row, so gamma stays in
+// registers and dgamma, dbeta are summed there; the teams of a block join theirs in shared memory, the blocks (one per SM) in a
+// second kernel.  Rows come into a ring of slots in shared memory by bulk copies, several rows ahead: with loads into
+// registers, two blocks an SM, 16384 x 2048 bf16 took 91 us.  A bulk copy moves whole 16-byte pieces; the values before the first and
+// after the last of a row that starts anywhere (at most seven each) are loaded by their threads a row ahead.
+constexpr int kLnBack = 8;
+constexpr int kLnBlock = 1024;
+constexpr uint32_t kLnRing = 198656;
+constexpr int kLnMostDepth = 8;
 
-// Rows of up to 8192 values in one pass: a team holds a row, a thread the same columns of every row, so gamma stays in
-// registers and dgamma, dbeta are summed there; the teams of a block join theirs in shared memory, the blocks in a second
-// kernel.
-template <typename T, int V, int TEAM, int BLOCK>
-__global__ void __launch_bounds__(BLOCK, 1024 / BLOCK) ln_backward_rows_kernel(const __grid_constant__ LnBackward<T> p)
+// the whole 16-byte pieces of a row of n values: values [first, last)
+template <typename T>
+__device__ __forceinline__ void whole_pieces(const T *row, int n, int &first, int &last)
 {
-    constexpr int K = kLnBack / V, kTeams = BLOCK / TEAM, kColumns = TEAM * kLnBack;
+    const uintptr_t s = reinterpret_cast<uintptr_t>(row), e = s + (size_t)n * sizeof(T);
+    const uintptr_t lo = (s + 15) & ~(uintptr_t)15, hi = e & ~(uintptr_t)15;
+    if (hi > lo) { first = (int)((lo - s) / sizeof(T)); last = (int)((hi - s) / sizeof(T)); }
+    else { first = n; last = n; }
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+template <int THREADS>
+__device__ __forceinline__ void team_sync(int id)
+{
+    if constexpr (THREADS == 32) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(THREADS) : "memory");
+}
+
+template <typename T, int V, int TEAM>
+__global__ void __launch_bounds__(kLnBlock, 1) ln_backward_rows_kernel(const __grid_constant__ LnBackward<T> p)
+{
+    constexpr int K = kLnBack / V, kTeams = kLnBlock / TEAM, kColumns = TEAM * kLnBack;
+    extern __shared__ __align__(128) uint8_t ring[];
     __shared__ float scratch[kTeams][2 * TEAM / 32];
-    __shared__ float joined[kTeams > 1 ? 2 * kColumns : 1];
+    __shared__ uint8_t exps[kTeams][2][kColumns / kCkptBlock];
+    __shared__ __align__(8) uint64_t bars[kTeams][kLnMostDepth];
+    const int t = threadIdx.x % TEAM, team = threadIdx.x / TEAM, n = (int)p.n, depth = p.depth;
+    const uint32_t slot_bytes = p.dy_bytes + p.x_bytes;
+    uint8_t *mine = ring + (size_t)team * depth * slot_bytes;
+    const uint32_t bar0 = ptx::smem_u32(bars[team]);
+    if (t == 0) {
+        for (int d = 0; d < depth; d++) ptx::mbar_init(bar0 + 8u * d, 1);
+        ptx::fence_barrier_init();
+    }
+    __syncthreads();
     grid_dependency_wait();
-    const int t = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
+
+    const int step = (int)gridDim.x * kTeams;
+    int row = (int)blockIdx.x * kTeams + team;
+    // one thread of the team: the whole pieces of a row into slot d
+    auto issue = [&](int at, int d) {
+        const uint32_t bar = bar0 + 8u * d, dst = ptx::smem_u32(mine + (size_t)d * slot_bytes);
+        const T *dy = p.dy + (size_t)at * p.dy_pitch;
+        int f0, l0, f1 = 0, l1 = 0;
+        whole_pieces(dy, n, f0, l0);
+        const T *x = p.x + (size_t)at * p.x_pitch;
+        const uint32_t dy_size = (uint32_t)(l0 - f0) * (uint32_t)sizeof(T);
+        uint32_t x_size;
+        if (p.codes) {
+            x_size = (uint32_t)(p.blocks * kCkptBlock);
+        } else {
+            whole_pieces(x, n, f1, l1);
+            x_size = (uint32_t)(l1 - f1) * (uint32_t)sizeof(T);
+        }
+        ptx::mbar_arrive_expect_tx(bar, dy_size + x_size);
+        // a value lies in its slot at the row's own offset from a 16-byte boundary
+        if (dy_size) bulk_load(dst + (uint32_t)(reinterpret_cast<uintptr_t>(dy) & 15) + (uint32_t)f0 * (uint32_t)sizeof(T), dy + f0, dy_size, bar);
+        if (p.codes) bulk_load(dst + p.dy_bytes, p.codes + (size_t)at * p.blocks * kCkptBlock, x_size, bar);
+        else if (x_size) bulk_load(dst + p.dy_bytes + (uint32_t)(reinterpret_cast<uintptr_t>(x) & 15) + (uint32_t)f1 * (uint32_t)sizeof(T), x + f1, x_size, bar);
+    };
+    if (t == 0) {
+        for (int d = 0, at = row; d < depth && at < p.rows; d++, at += step) issue(at, d);
+    }
+    // what does not come by bulk copies, a row ahead: statistics, exponents, the ends of unaligned rows (this thread's column
+    // among the first seven, and the one among the last)
+    float next_mu = 0.f, next_r = 0.f, head_dy = 0.f, head_x = 0.f, tail_dy = 0.f, tail_x = 0.f;
+    const int tail_column = V == 1 ? ((n - 1 - t) / TEAM) * TEAM + t : 0;
+    const bool has_head = V == 1 && t < 7 && t < n, has_tail = V == 1 && t < n && tail_column >= n - 7;
+    auto ahead = [&](int at) {
+        next_r = p.rstd[at];
+        next_mu = p.mean ? p.mean[at] : 0.f;
+        if (has_head) {
+            head_dy = to_float(p.dy[(size_t)at * p.dy_pitch + t]);
+            if (!p.codes) head_x = to_float(p.x[(size_t)at * p.x_pitch + t]);
+        }
+        if (has_tail) {
+            tail_dy = to_float(p.dy[(size_t)at * p.dy_pitch + tail_column]);
+            if (!p.codes) tail_x = to_float(p.x[(size_t)at * p.x_pitch + tail_column]);
+        }
+    };
+    // exponents: into a register two rows ahead, into shared memory one row ahead
+    const bool has_exp = p.codes && t < (int)p.blocks;
+    uint8_t next_exp = 0;
+    int turn = 0, limit = 1000000;
+    if (row < p.rows) {
+        ahead(row);
+        if (has_exp) {
+            exps[team][0][t] = p.exponents[(size_t)row * p.blocks + t];
+            if (row + step < p.rows) next_exp = p.exponents[(size_t)(row + step) * p.blocks + t];
+        }
+    }
+    team_sync<TEAM>(1 + team);
+
     float gamma[K][V], dgamma[K][V], dbeta[K][V];
     bool in[K];
 #pragma unroll
     for (int k = 0; k < K; k++) {
-        const size_t col = (size_t)(k * TEAM + t) * V;
-        in[k] = col < p.n;
+        const int col = (k * TEAM + t) * V;
+        in[k] = col < n;
 #pragma unroll
         for (int j = 0; j < V; j++) { gamma[k][j] = in[k] ? __ldg(p.gamma + col + j) : 0.f; dgamma[k][j] = dbeta[k][j] = 0.f; }
     }
-    const int step = (int)gridDim.x * kTeams;
-    int row = (int)blockIdx.x * kTeams + team;
-    for (; row < p.rows; row += step) {
-        LnRaw<T, V> raw[K];
-#pragma unroll
-        for (int k = 0; k < K; k++)
-            if (in[k]) ln_load<T, V>(p, row, (size_t)(k * TEAM + t) * V, raw[k]);
-        const float r = p.rstd[row], mu = p.mean ? p.mean[row] : 0.f;
+    int slot = 0;
+    uint32_t phase = 0;
+    for (; row < p.rows; row += step, turn ^= 1) {
+        for (int polls = 0; !ptx::mbar_try_wait(bar0 + 8u * slot, phase); polls++) {
+            if (polls >= limit) {                           // a second or so: the results are reported invalid, no later wait takes long
+                atomicExch(p.status, 0xb00u + B200_E_TIMEOUT);
+                __threadfence_system();
+                limit = 0;
+                break;
+            }
+        }
+        const uint8_t *src = mine + (size_t)slot * slot_bytes;
+        const T *dy_row = p.dy + (size_t)row * p.dy_pitch, *x_row = p.x + (size_t)row * p.x_pitch;
+        const T *dy_in = reinterpret_cast<const T *>(src + (reinterpret_cast<uintptr_t>(dy_row) & 15));
+        const T *x_in = reinterpret_cast<const T *>(src + p.dy_bytes + (p.codes ? 0 : (reinterpret_cast<uintptr_t>(x_row) & 15)));
+        const int8_t *code_in = reinterpret_cast<const int8_t *>(src + p.dy_bytes);
+        int dy_first = 0, dy_last = n, x_first = 0, x_last = n;
+        if (V == 1) {
+            whole_pieces(dy_row, n, dy_first, dy_last);
+            if (!p.codes) whole_pieces(x_row, n, x_first, x_last);
+        }
+        const float r = next_r, mu = next_mu;
         float dy[K][V], xh[K][V], s[2] = {0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < K; k++) {
+            const int col = (k * TEAM + t) * V;
             if (in[k]) {
-                ln_values<T, V>(p, raw[k], mu, r, dy[k], xh[k]);
+                const Pack<T, V> a = load_pack<T, V>(dy_in + col);
+#pragma unroll
+                for (int j = 0; j < V; j++) dy[k][j] = to_float(a.v[j]);
+                if (V == 1) dy[k][0] = col < dy_first && col < 7 ? head_dy : col >= dy_last ? tail_dy : dy[k][0];
+                if (p.codes) {
+                    ckpt8_values<V>(xh[k], ckpt8_get<V>(code_in + col), exps[team][turn][col / kCkptBlock]);
+                } else {
+                    const Pack<T, V> b = load_pack<T, V>(x_in + col);
+#pragma unroll
+                    for (int j = 0; j < V; j++) xh[k][j] = to_float(b.v[j]);
+                    if (V == 1) xh[k][0] = col < x_first && col < 7 ? head_x : col >= x_last ? tail_x : xh[k][0];
+#pragma unroll
+                    for (int j = 0; j < V; j++) xh[k][j] = (xh[k][j] - mu) * r;
+                }
             } else {
 #pragma unroll
                 for (int j = 0; j < V; j++) dy[k][j] = xh[k][j] = 0.f;
@@ -357,45 +486,71 @@ __global__ void __launch_bounds__(BLOCK, 1024 / BLOCK) ln_backward_rows_kernel(c
                 s[1] = fmaf(dy[k][j], xh[k][j], s[1]);
             }
         }
-        team_total<TEAM, 2>(s, scratch[team], 1 + team);
-        const float c1 = s[0] / (float)p.n, c2 = s[1] / (float)p.n;
+        if (has_exp) {
+            exps[team][turn ^ 1][t] = next_exp;
+            if (row + 2ll * step < p.rows) next_exp = p.exponents[(size_t)(row + 2 * step) * p.blocks + t];
+        }
+        if (row + step < p.rows) ahead(row + step);
+        team_total<TEAM, 2>(s, scratch[team], 1 + team);    // and with it: every thread has read the slot, and wrote its exponents
+        if (TEAM == 32) __syncwarp();
+        if (t == 0 && row + (long long)depth * step < p.rows) issue(row + depth * step, slot);
+        if (++slot == depth) { slot = 0; phase ^= 1u; }
+        const float c1 = s[0] / (float)n, c2 = s[1] / (float)n;
+        T *dx_row = p.dx + (size_t)row * p.dx_pitch;
 #pragma unroll
         for (int k = 0; k < K; k++) {
             if (!in[k]) continue;
             float dx[V];
 #pragma unroll
             for (int j = 0; j < V; j++) dx[j] = r * (dy[k][j] - c1 - xh[k][j] * c2);
-            store_pack<T, V>(p.dx + (size_t)row * p.dx_pitch + (size_t)(k * TEAM + t) * V, dx);
+            store_pack<T, V>(dx_row + (k * TEAM + t) * V, dx);
         }
     }
+    if (limit == 0) {                                       // copies still under way get time to land before the block ends
+        for (int k = 0; k < 1000; k++) __nanosleep(200);
+    }
     if (!p.weights) return;
-    if constexpr (kTeams > 1) {
-        for (int w = 0; w < kTeams; w++) {                  // in the order of the teams
-            if (team == w) {
+    // the teams' sums, pair by pair (the ring is free: every copy has been waited for)
+    __syncthreads();
+    float *tree = reinterpret_cast<float *>(ring);
 #pragma unroll
-                for (int k = 0; k < K; k++) {
+    for (int half = kTeams / 2; half > 0; half /= 2) {
+        if (team >= half && team < 2 * half) {
+            float *a = tree + (size_t)(team - half) * 2 * kColumns;
 #pragma unroll
-                    for (int j = 0; j < V; j++) {
-                        float *a = joined + (k * TEAM + t) * V + j;
-                        a[0] = w ? a[0] + dgamma[k][j] : dgamma[k][j];
-                        a[kColumns] = w ? a[kColumns] + dbeta[k][j] : dbeta[k][j];
-                    }
+            for (int k = 0; k < K; k++) {
+#pragma unroll
+                for (int j = 0; j < V; j++) {
+                    a[(k * TEAM + t) * V + j] = dgamma[k][j];
+                    a[kColumns + (k * TEAM + t) * V + j] = dbeta[k][j];
                 }
             }
-            __syncthreads();
         }
-        float *out = p.part + (size_t)blockIdx.x * 2 * p.n;
-        for (int c = threadIdx.x; c < (int)p.n; c += BLOCK) { out[c] = joined[c]; out[p.n + c] = joined[kColumns + c]; }
-    } else {
-        float *out = p.part + (size_t)blockIdx.x * 2 * p.n;
+        __syncthreads();
+        if (team < half) {
+            const float *a = tree + (size_t)team * 2 * kColumns;
 #pragma unroll
-        for (int k = 0; k < K; k++) {
-            if (!in[k]) continue;
+            for (int k = 0; k < K; k++) {
 #pragma unroll
-            for (int j = 0; j < V; j++) {
-                out[(size_t)(k * TEAM + t) * V + j] = dgamma[k][j];
-                out[p.n + (size_t)(k * TEAM + t) * V + j] = dbeta[k][j];
+                for (int j = 0; j < V; j++) {
+                    dgamma[k][j] += a[(k * TEAM + t) * V + j];
+                    dbeta[k][j] += a[kColumns + (k * TEAM + t) * V + j];
+                }
             }
+        }
+        __syncthreads();
+    }
+    if (team) return;
+    float *out_g = p.groups == 1 ? p.dgamma : p.part + (size_t)blockIdx.x * 2 * n, *out_b = p.groups == 1 ? p.dbeta : out_g + n;
+    const bool add = p.groups == 1 && p.accumulate;
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+        if (!in[k]) continue;
+        const int col = (k * TEAM + t) * V;
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            out_g[col + j] = add ? out_g[col + j] + dgamma[k][j] : dgamma[k][j];
+            out_b[col + j] = add ? out_b[col + j] + dbeta[k][j] : dbeta[k][j];
         }
     }
 }
@@ -481,38 +636,45 @@ __global__ void __launch_bounds__(256) ln_backward_apply_kernel(const __grid_con
     }
 }
 
-// Sum of the groups' partial rows, in an order that does not depend on how they were scheduled: eight threads take every eighth group.
-__global__ void __launch_bounds__(256) ln_backward_join_kernel(float *dgamma, float *dbeta, const float *__restrict__ part, int groups, size_t n, int accumulate)
+// Sum of the groups' partial rows, in an order that does not depend on how they were scheduled: SPLIT threads take every SPLIT-th
+// group of a column.
+template <int SPLIT>
+__global__ void __launch_bounds__(1024) ln_backward_join_kernel(float *dgamma, float *dbeta, const float *__restrict__ part, int groups, size_t n, int accumulate)
 {
-    __shared__ float sums[8][33];
+    constexpr int kWide = 1024 / SPLIT;
+    __shared__ float sums[SPLIT][kWide + 1];
     grid_dependency_wait();
-    const int c = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const size_t i = (size_t)blockIdx.x * 32 + c;
+    const int c = threadIdx.x % kWide, w = threadIdx.x / kWide;
+    const size_t i = (size_t)blockIdx.x * kWide + c;
     float s = 0.f;
     if (i < 2 * n) {
-#pragma unroll 4
-        for (int g = w; g < groups; g += 8) s += part[(size_t)g * 2 * n + i];
+#pragma unroll 8
+        for (int g = w; g < groups; g += SPLIT) s += part[(size_t)g * 2 * n + i];
     }
-    sums[w][c] = s;
-    __syncthreads();
-    if (w || i >= 2 * n) return;
+    if constexpr (SPLIT > 1) {
+        sums[w][c] = s;
+        __syncthreads();
+        if (w == 0) {
 #pragma unroll
-    for (int k = 1; k < 8; k++) s += sums[k][c];
+            for (int k = 1; k < SPLIT; k++) s += sums[k][c];
+        }
+    }
+    if (w || i >= 2 * n) return;
     float *out = i < n ? dgamma + i : dbeta + (i - n);
     *out = accumulate ? *out + s : s;
 }
 
 constexpr size_t kLnOnePass = 8192;
-struct LnPlan { bool one_pass; int team, block, groups, pieces; };
+struct LnPlan { bool one_pass; int team, groups, pieces; };
 static LnPlan ln_plan(int rows, size_t n, int v)
 {
     LnPlan w = {};
     w.one_pass = n <= kLnOnePass;
     if (w.one_pass) {
         w.team = n <= 256 ? 32 : n <= 1024 ? 128 : n <= 2048 ? 256 : n <= 4096 ? 512 : 1024;
-        w.block = w.team <= 512 ? 512 : 1024;
-        const int teams = w.block / w.team;
-        w.groups = min((rows + teams - 1) / teams, sm_count() * (1024 / w.block));
+        // One block where each team then has four rows at most: it writes the gradients itself.
+        const int teams = kLnBlock / w.team;
+        w.groups = rows <= 4 * teams ? 1 : min((rows + teams - 1) / teams, sm_count());
     } else {
         const size_t slices = (n + (size_t)kLnSlice * v - 1) / ((size_t)kLnSlice * v);
         w.pieces = (int)slices * (kLnSlice / 32);
@@ -531,16 +693,32 @@ static int ln_backward_launch(LnBackward<T> p, float *dgamma, float *dbeta, int 
     p.pieces = w.pieces;
     p.row_part = reinterpret_cast<float2 *>(workspace);
     p.part = reinterpret_cast<float *>(workspace + align_up((size_t)p.rows * w.pieces * sizeof(float2), 16));
+    p.dgamma = dgamma;
+    p.dbeta = dbeta;
+    p.accumulate = accumulate;
     if (w.one_pass) {
-        const Launch launch((unsigned)w.groups, (unsigned)w.block, 0, s);
+        int r = status_word(&p.status);
+        if (r) return r;
+        const int teams = kLnBlock / w.team;
+        p.dy_bytes = (uint32_t)align_up(p.n * sizeof(T) + 16, 16);
+        p.x_bytes = p.codes ? (uint32_t)(p.blocks * kCkptBlock) : p.dy_bytes;
+        p.depth = min(kLnMostDepth, (int)(kLnRing / (teams * (p.dy_bytes + p.x_bytes))));      // three at least: 8192 values of 4 bytes, twice
+        const uint32_t smem = max((uint32_t)(teams * p.depth) * (p.dy_bytes + p.x_bytes), w.team < kLnBlock ? 32768u : 0u);
+#define B200_LN_ROWS(TEAM)                                                                                                                           \
+    do {                                                                                                                                             \
+        B200_CUDA(cudaFuncSetAttribute(ln_backward_rows_kernel<T, V, TEAM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kLnRing));             \
+        Launch((unsigned)w.groups, kLnBlock, smem, s)(ln_backward_rows_kernel<T, V, TEAM>, p);                                                       \
+    } while (0)
         switch (w.team) {
-        case 32: launch(ln_backward_rows_kernel<T, V, 32, 512>, p); break;
-        case 128: launch(ln_backward_rows_kernel<T, V, 128, 512>, p); break;
-        case 256: launch(ln_backward_rows_kernel<T, V, 256, 512>, p); break;
-        case 512: launch(ln_backward_rows_kernel<T, V, 512, 512>, p); break;
-        default: launch(ln_backward_rows_kernel<T, V, 1024, 1024>, p); break;
+        case 32: B200_LN_ROWS(32); break;
+        case 128: B200_LN_ROWS(128); break;
+        case 256: B200_LN_ROWS(256); break;
+        case 512: B200_LN_ROWS(512); break;
+        default: B200_LN_ROWS(1024); break;
         }
+#undef B200_LN_ROWS
         B200_LAUNCH_CHECK();
+        if (w.groups == 1) return B200_OK;
     } else {
         Launch(dim3((unsigned)(w.pieces / (kLnSlice / 32)), (unsigned)w.groups), kLnSlice, 0, s)(ln_backward_columns_kernel<T, V>, p);
         B200_LAUNCH_CHECK();
@@ -548,7 +726,9 @@ static int ln_backward_launch(LnBackward<T> p, float *dgamma, float *dbeta, int 
         B200_LAUNCH_CHECK();
     }
     if (p.weights) {
-        Launch((unsigned)((2 * p.n + 31) / 32), 256, 0, s)(ln_backward_join_kernel, dgamma, dbeta, p.part, p.groups, p.n, accumulate);
+        // many groups (blocks of the one-pass form) or many columns
+        if (p.groups > 16) Launch((unsigned)((2 * p.n + 31) / 32), 1024, 0, s)(ln_backward_join_kernel<32>, dgamma, dbeta, p.part, p.groups, p.n, accumulate);
+        else Launch((unsigned)((2 * p.n + 1023) / 1024), 1024, 0, s)(ln_backward_join_kernel<1>, dgamma, dbeta, p.part, p.groups, p.n, accumulate);
         B200_LAUNCH_CHECK();
     }
     return B200_OK;
@@ -624,7 +804,7 @@ int b200_ln_backward(void *dx, float *dgamma, float *dbeta, const void *dy, cons
 #define B200_LN_BWD(T)                                                                                                                               \
     do {                                                                                                                                             \
         const LnBackward<T> p = {(T *)dx, (const T *)dy, (const T *)x, mean, rstd, codes, exponents, gamma, rows, n, ckpt8_blocks(n), dy_pitch,      \
-                                 x_pitch, dx_pitch, create_delta_weight != 0, nullptr, 0, nullptr, 0};                                               \
+                                 x_pitch, dx_pitch, create_delta_weight != 0};                                             \
         return wide ? ln_backward_launch<T, kWide<T>>(p, dgamma, dbeta, accumulate, (char *)workspace, ST(stream))                                   \
                     : ln_backward_launch<T, 1>(p, dgamma, dbeta, accumulate, (char *)workspace, ST(stream));                                         \
     } while (0)

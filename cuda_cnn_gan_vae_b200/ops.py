@@ -71,24 +71,32 @@ def geom(in_z, in_y, in_x, kernel_amount, kernel_x, kernel_y, stride_x, stride_y
 # ---- layer normalisation and 8-bit checkpoints: activations in fp32, bf16 or fp16, as matrices of rows --------------------------
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+
+
+def _stream_id():
+    """The current stream of the current device as a number (a call of a few microseconds is made of little else)."""
+    return torch._C._cuda_getCurrentRawStream(_device())
 
 
 def _rows(x, name="tensor"):
     """(type code, rows, values in a row, pitch) of an activation tensor: its first dimension is the rows, the others (dense)
     are a row.  A 2-D tensor may have any pitch between its rows."""
-    if not (isinstance(x, torch.Tensor) and x.is_cuda and x.dtype in _TYPES and x.dim() >= 1):
+    kind = _TYPES.get(x.dtype) if isinstance(x, torch.Tensor) else None
+    if kind is None or not x.is_cuda:
         raise B200Error(2, f"{name} must be an fp32, bf16 or fp16 CUDA tensor")
-    if x.device.index != torch.cuda.current_device():
-        raise B200Error(2, f"{name} is on {x.device}, the current device is cuda:{torch.cuda.current_device()}")
-    rows = x.shape[0]
-    if x.dim() == 2 and x.shape[1]:
-        n, pitch = x.shape[1], x.stride(0)
-        if (x.stride(1) == 1 or n == 1) and (pitch >= n or rows <= 1):
-            return _TYPES[x.dtype], rows, n, max(pitch, n)
-    if not x.is_contiguous():
+    if x.get_device() != _device():
+        raise B200Error(2, f"{name} is on {x.device}, the current device is cuda:{_device()}")
+    shape = x.shape
+    if len(shape) == 2 and shape[1]:
+        rows, n = shape
+        pitch, inner = x.stride()
+        if (inner == 1 or n == 1) and (pitch >= n or rows <= 1):
+            return kind, rows, n, pitch if pitch > n else n
+    if not shape or not x.is_contiguous():
         raise B200Error(2, f"{name} must be contiguous, or a matrix of contiguous rows")
-    n = x[0].numel() if rows else int(torch.Size(x.shape[1:]).numel())
-    return _TYPES[x.dtype], rows, n, n
+    n = torch.Size(shape[1:]).numel()
+    return kind, shape[0], n, n
 
 
 def _param(x, n, name):
@@ -96,8 +104,8 @@ def _param(x, n, name):
     _t(x, name)
     if x.numel() != n:
         raise B200Error(1, f"{name} must have {n} elements")
-    if x.device.index != torch.cuda.current_device():
-        raise B200Error(2, f"{name} is on {x.device}, the current device is cuda:{torch.cuda.current_device()}")
+    if x.get_device() != _device():
+        raise B200Error(2, f"{name} is on {x.device}, the current device is cuda:{_device()}")
     return x
 
 
@@ -118,16 +126,15 @@ class Checkpoint8:
     __slots__ = ("codes", "exponents", "rows", "n")
 
     def __init__(self, codes, exponents, n):
-        blocks = (n + 31) // 32
         if not (codes.is_cuda and exponents.is_cuda and codes.dtype == torch.int8 and exponents.dtype == torch.uint8 and
                 codes.is_contiguous() and exponents.is_contiguous()):
             raise B200Error(2, "codes and exponents must be contiguous int8 and uint8 CUDA tensors")
-        if codes.device != exponents.device or codes.device.index != torch.cuda.current_device():
+        if not codes.get_device() == exponents.get_device() == _device():
             raise B200Error(2, "codes and exponents must be on the current device")
-        if n < 1 or codes.dim() != 2 or exponents.dim() != 2 or codes.shape[1] != 32 * blocks or exponents.shape[1] != blocks or \
-                codes.shape[0] != exponents.shape[0]:
+        blocks, rows = (n + 31) // 32, codes.shape[0]
+        if n < 1 or codes.shape != (rows, 32 * blocks) or exponents.shape != (rows, blocks):
             raise B200Error(1, "codes must be [rows, 32 * blocks] and exponents [rows, blocks], blocks = ceil(n / 32)")
-        self.codes, self.exponents, self.rows, self.n = codes, exponents, codes.shape[0], n
+        self.codes, self.exponents, self.rows, self.n = codes, exponents, rows, n
 
     @classmethod
     def empty(cls, rows, n, device="cuda"):
@@ -145,14 +152,14 @@ class Checkpoint8:
         """Keeps x.  keep_sign: a negative value never becomes 0 (the derivative of ReLU and LeakyReLU is then exact)."""
         kind, rows, n, pitch = self._match(x, "x")
         _check(load().b200_ckpt8_store(self.codes.data_ptr(), self.exponents.data_ptr(), x.data_ptr(), kind, rows, n, pitch,
-                                       int(keep_sign), _stream()))
+                                       int(keep_sign), _stream_id()))
         return self
 
     def load(self, output):
         """The kept values into `output` (fp32, bf16 or fp16), which is returned."""
         kind, rows, n, pitch = self._match(output, "output")
         _check(load().b200_ckpt8_load(output.data_ptr(), self.codes.data_ptr(), self.exponents.data_ptr(), kind, rows, n, pitch,
-                                      _stream()))
+                                      _stream_id()))
         return output
 
 
@@ -475,7 +482,7 @@ class CTensorApplyFunc:
             kind, rows, n, pitch = z._match(output, "output")
             e = _like(error, "error", (kind, rows, n), "output")
             _check(load().b200_ckpt8_activation_backward(output.data_ptr(), z.codes.data_ptr(), z.exponents.data_ptr(), error.data_ptr(),
-                                                         kind, rows, n, pitch, e[3], ACT[func], leaky_slope, _stream()))
+                                                         kind, rows, n, pitch, e[3], ACT[func], leaky_slope, _stream_id()))
             return
         _t(output), _t(z), _t(error)
         _check(load().b200_activation_backward(_ptr(output), _ptr(z), _ptr(error), z.numel(), ACT[func], leaky_slope, _stream()))
@@ -513,7 +520,7 @@ def _workspace(size, given, name):
     workspaces of captured graphs apart)."""
     if given is None:
         return torch.empty(max(size, 16), dtype=torch.uint8, device="cuda"), max(size, 16)
-    if not (isinstance(given, torch.Tensor) and given.is_cuda and given.is_contiguous() and given.device.index == torch.cuda.current_device()):
+    if not (isinstance(given, torch.Tensor) and given.is_cuda and given.is_contiguous() and given.get_device() == _device()):
         raise B200Error(2, f"{name}: the workspace must be a contiguous tensor on the current device")
     return given, given.numel() * given.element_size()
 
@@ -535,7 +542,7 @@ def ln_forward(x, gamma, beta, eps=1e-6, y=None, mean=None, rstd=None, checkpoin
             raise B200Error(1, f"the checkpoint must have {rows} rows of {n} values")
         codes, exponents = checkpoint.codes.data_ptr(), checkpoint.exponents.data_ptr()
     _check(load().b200_ln_forward(y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), codes, exponents, x.data_ptr(), gamma.data_ptr(),
-                                  beta.data_ptr(), kind, rows, n, pitch, y_pitch, eps, _stream()))
+                                  beta.data_ptr(), kind, rows, n, pitch, y_pitch, eps, _stream_id()))
     return dict(y=y, mean=mean, rstd=rstd)
 
 
@@ -562,7 +569,7 @@ def ln_backward(dy, x, mean, rstd, gamma, dgamma, dbeta, create_delta_weight=Tru
     workspace, size = _workspace(load().b200_ln_backward_workspace(rows, n), workspace, "ln_backward")
     _check(load().b200_ln_backward(dx.data_ptr(), dg, db, dy.data_ptr(), x_ptr, mean_ptr, rstd.data_ptr(), codes, exponents, gamma.data_ptr(),
                                    kind, rows, n, dx_pitch, dy_pitch, x_pitch, int(create_delta_weight), int(accumulate),
-                                   workspace.data_ptr(), size, _stream()))
+                                   workspace.data_ptr(), size, _stream_id()))
     return dx
 
 
@@ -578,7 +585,7 @@ def checkpoint_wgrad(dweight, dbias, delta, checkpoint, accumulate=True, workspa
     workspace, size = _workspace(load().b200_ckpt8_wgrad_workspace(kind, rows, out, checkpoint.n, delta.data_ptr(), pitch), workspace, "checkpoint_wgrad")
     _check(load().b200_ckpt8_wgrad(dweight.data_ptr(), dbias.data_ptr() if dbias is not None else None, int(accumulate), delta.data_ptr(),
                                    checkpoint.codes.data_ptr(), checkpoint.exponents.data_ptr(), kind, rows, out, checkpoint.n, pitch,
-                                   workspace.data_ptr(), size, _stream()))
+                                   workspace.data_ptr(), size, _stream_id()))
 
 
 def vae_forward(mu, logvar, eps, want_kl=True):
