@@ -88,9 +88,13 @@ template <int V> __device__ __forceinline__ CkptCodes<V> ckpt8_get(const int8_t 
 }
 template <int V> __device__ __forceinline__ void ckpt8_values(float *f, CkptCodes<V> c, uint32_t b)
 {
-    const float unit = ckpt8_unit(b);
+    // the byte u = q + 128 under the exponent of 2^23 is the float 2^23 + u: no conversion instruction; the step may be subnormal
+    const float step = ckpt8_unit(b) * 0.015625f;
 #pragma unroll
-    for (int i = 0; i < V; i++) f[i] = ckpt8_value(V == 1 ? (int)c.w[0] : (int)(int8_t)(c.w[i / 4] >> (8 * (i & 3))), unit);
+    for (int i = 0; i < V; i++) {
+        const uint32_t u = __byte_perm(c.w[i / 4] ^ 0x80808080u, 0x4b000000u, 0x7540 | (i & 3));
+        f[i] = (__uint_as_float(u) - 8388736.f) * step;
+    }
 }
 
 }  // namespace b200

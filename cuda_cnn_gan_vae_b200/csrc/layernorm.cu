@@ -26,28 +26,75 @@ __device__ __forceinline__ float warp_total(float v)
     return v;
 }
 
-// Sums over the THREADS threads of a team (a warp, or whole warps that share named barrier `id`); every thread receives them.
-// `scratch` holds N floats per warp of the team and is free again after the call.
-template <int THREADS, int N>
-__device__ __forceinline__ void team_total(float *v, float *scratch, int id)
+// Two fp32 operations in one instruction
+__device__ __forceinline__ float2 add2(float2 a, float2 b)
 {
-#pragma unroll
-    for (int k = 0; k < N; k++) v[k] = warp_total(v[k]);
+    float2 d;
+    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b)
+{
+    float2 d;
+    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
+{
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+
+// Sum over the THREADS threads of a team (a warp, or whole warps that share named barrier `id`); every thread receives it.
+// `scratch` holds a float per warp of the team and is free again after the call.
+template <int THREADS>
+__device__ __forceinline__ float team_total(float v, float *scratch, int id)
+{
+    v = warp_total(v);
     if constexpr (THREADS > 32) {
         constexpr int kWarps = THREADS / 32;
         const int lane = threadIdx.x & 31, warp = (threadIdx.x % THREADS) >> 5;
-        if (lane == 0) {
-#pragma unroll
-            for (int k = 0; k < N; k++) scratch[k * kWarps + warp] = v[k];
-        }
+        if (lane == 0) scratch[warp] = v;
         asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(THREADS) : "memory");
-#pragma unroll
-        for (int k = 0; k < N; k++) {
-            v[k] = lane < kWarps ? scratch[k * kWarps + lane] : 0.f;
-            v[k] = warp_total(v[k]);
-        }
+        v = warp_total(lane < kWarps ? scratch[lane] : 0.f);
         asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(THREADS) : "memory");
     }
+    return v;
+}
+
+// Two sums over a warp: the lower lanes finish the first, the upper ones the second
+__device__ __forceinline__ float2 warp_totals(float2 v)
+{
+    const bool upper = threadIdx.x & 16;
+    float mine = upper ? v.y : v.x;
+    mine += __shfl_xor_sync(0xffffffffu, upper ? v.x : v.y, 16);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    return make_float2(__shfl_sync(0xffffffffu, mine, 0), __shfl_sync(0xffffffffu, mine, 16));
+}
+// Two sums over a team with one barrier: the caller alternates between two `scratch` areas of a float2 per warp
+template <int THREADS>
+__device__ __forceinline__ float2 team_totals(float2 v, float2 *scratch, int id)
+{
+    v = warp_totals(v);
+    if constexpr (THREADS > 32) {
+        constexpr int kWarps = THREADS / 32;
+        const int lane = threadIdx.x & 31, warp = (threadIdx.x % THREADS) >> 5;
+        if (lane == 0) scratch[warp] = v;
+        asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(THREADS) : "memory");
+        if constexpr (kWarps <= 8) {
+            v = scratch[0];
+#pragma unroll
+            for (int k = 1; k < kWarps; k++) v = add2(v, scratch[k]);
+        } else {
+            v = warp_totals(lane < kWarps ? scratch[lane] : make_float2(0.f, 0.f));
+        }
+    }
+    return v;
 }
 
 // ---- forward -----------------------------------------------------------------------------------------------------------------
@@ -125,7 +172,7 @@ __global__ void __launch_bounds__(BLOCK, 1024 / BLOCK) ln_forward_kernel(const _
 #pragma unroll
             for (int j = 0; j < V; j++) s += v[k][j];
         }
-        team_total<TEAM, 1>(&s, scratch[team], 1 + team);
+        s = team_total<TEAM>(s, scratch[team], 1 + team);
         float mu = s / (CLUSTER ? fmaxf(mine, 1.f) : mine);
 #pragma unroll
         for (int k = 0; k < K; k++) {
@@ -135,7 +182,7 @@ __global__ void __launch_bounds__(BLOCK, 1024 / BLOCK) ln_forward_kernel(const _
                 for (int j = 0; j < V; j++) { const float d = v[k][j] - mu; q = fmaf(d, d, q); }
             }
         }
-        team_total<TEAM, 1>(&q, scratch[team], 1 + team);
+        q = team_total<TEAM>(q, scratch[team], 1 + team);
         if constexpr (CLUSTER) {
             // deviations about the mean of all: those about the share's own mean, and its distance
             cg::cluster_group cluster = cg::this_cluster();
@@ -201,9 +248,7 @@ __global__ void __launch_bounds__(512) ln_forward_long_kernel(const __grid_const
                     }
                 }
             }
-            float v = (s[0] + s[1]) + (s[2] + s[3]);
-            team_total<512, 1>(&v, scratch, 1);
-            return v;
+            return team_total<512>((s[0] + s[1]) + (s[2] + s[3]), scratch, 1);
         };
         float mu = total([](float v) { return v; }) / fmaxf(mine, 1.f);
         float q = total([&](float v) { const float d = v - mu; return d * d; });
@@ -317,13 +362,13 @@ __device__ __forceinline__ void ln_values(const LnBackward<T> &p, const LnRaw<T,
     for (int j = 0; j < V; j++) dy[j] = to_float(in.dy.v[j]);
 }
 
-// Rows of up to 8192 values in one pass: a team holds a row, a thread the same eight columns of every row, so gamma stays in
+// Rows of up to 8192 values in one pass: a team holds a row, a thread the same sixteen columns of every row, so gamma stays in
 // registers and dgamma, dbeta are summed there; the teams of a block join theirs in shared memory, the blocks (one per SM) in a
 // second kernel.  Rows come into a ring of slots in shared memory by bulk copies, several rows ahead: with loads into
 // registers, two blocks an SM, 16384 x 2048 bf16 took 91 us.  A bulk copy moves whole 16-byte pieces; the values before the first and
 // after the last of a row that starts anywhere (at most seven each) are loaded by their threads a row ahead.
-constexpr int kLnBack = 8;
-constexpr int kLnBlock = 1024;
+constexpr int kLnBack = 16;
+constexpr int kLnBlock = 512;
 constexpr uint32_t kLnRing = 198656;
 constexpr int kLnMostDepth = 8;
 
@@ -353,7 +398,7 @@ __global__ void __launch_bounds__(kLnBlock, 1) ln_backward_rows_kernel(const __g
 {
     constexpr int K = kLnBack / V, kTeams = kLnBlock / TEAM, kColumns = TEAM * kLnBack;
     extern __shared__ __align__(128) uint8_t ring[];
-    __shared__ float scratch[kTeams][2 * TEAM / 32];
+    __shared__ float2 scratch[kTeams][2][TEAM / 32];
     __shared__ uint8_t exps[kTeams][2][kColumns / kCkptBlock];
     __shared__ __align__(8) uint64_t bars[kTeams][kLnMostDepth];
     const int t = threadIdx.x % TEAM, team = threadIdx.x / TEAM, n = (int)p.n, depth = p.depth;
@@ -393,45 +438,63 @@ __global__ void __launch_bounds__(kLnBlock, 1) ln_backward_rows_kernel(const __g
     if (t == 0) {
         for (int d = 0, at = row; d < depth && at < p.rows; d++, at += step) issue(at, d);
     }
-    // what does not come by bulk copies, a row ahead: statistics, exponents, the ends of unaligned rows (this thread's column
-    // among the first seven, and the one among the last)
+    // What does not come by bulk copies, a row ahead: statistics, and of rows of single values the first seven and the last
+    // seven (this thread's column among the first, and the one among the last).
+    const T *dy_next = p.dy + (size_t)row * p.dy_pitch, *x_next = p.x + (size_t)row * p.x_pitch;
+    T *dx_row = p.dx + (size_t)row * p.dx_pitch;
+    const size_t dy_step = (size_t)step * p.dy_pitch, x_step = (size_t)step * p.x_pitch, dx_step = (size_t)step * p.dx_pitch;
     float next_mu = 0.f, next_r = 0.f, head_dy = 0.f, head_x = 0.f, tail_dy = 0.f, tail_x = 0.f;
-    const int tail_column = V == 1 ? ((n - 1 - t) / TEAM) * TEAM + t : 0;
-    const bool has_head = V == 1 && t < 7 && t < n, has_tail = V == 1 && t < n && tail_column >= n - 7;
+    uint32_t next_dy_at = 0, next_x_at = 0;                  // the next row's place in its slot
+    const int tail_k = V == 1 && t < n ? (n - 1 - t) / TEAM : -1, tail_column = tail_k * TEAM + t;
+    const bool has_head = V == 1 && t < 7 && t < n, has_tail = V == 1 && tail_k >= 0 && tail_column >= n - 7;
     auto ahead = [&](int at) {
         next_r = p.rstd[at];
-        next_mu = p.mean ? p.mean[at] : 0.f;
-        if (has_head) {
-            head_dy = to_float(p.dy[(size_t)at * p.dy_pitch + t]);
-            if (!p.codes) head_x = to_float(p.x[(size_t)at * p.x_pitch + t]);
+        if (p.mean) next_mu = p.mean[at];
+        if (V == 1) {
+            next_dy_at = (uint32_t)(reinterpret_cast<uintptr_t>(dy_next) & 15);
+            next_x_at = p.dy_bytes + (p.codes ? 0u : (uint32_t)(reinterpret_cast<uintptr_t>(x_next) & 15));
+            if (has_head) {
+                head_dy = to_float(dy_next[t]);
+                if (!p.codes) head_x = to_float(x_next[t]);
+            }
+            if (has_tail) {
+                tail_dy = to_float(dy_next[tail_column]);
+                if (!p.codes) tail_x = to_float(x_next[tail_column]);
+            }
         }
-        if (has_tail) {
-            tail_dy = to_float(p.dy[(size_t)at * p.dy_pitch + tail_column]);
-            if (!p.codes) tail_x = to_float(p.x[(size_t)at * p.x_pitch + tail_column]);
-        }
+        dy_next += dy_step;
+        x_next += x_step;
     };
     // exponents: into a register two rows ahead, into shared memory one row ahead
     const bool has_exp = p.codes && t < (int)p.blocks;
+    const uint8_t *exp_next = p.exponents + (size_t)row * p.blocks + t;
+    const size_t exp_step = (size_t)step * p.blocks;
     uint8_t next_exp = 0;
     int turn = 0, limit = 1000000;
     if (row < p.rows) {
         ahead(row);
         if (has_exp) {
-            exps[team][0][t] = p.exponents[(size_t)row * p.blocks + t];
-            if (row + step < p.rows) next_exp = p.exponents[(size_t)(row + step) * p.blocks + t];
+            exps[team][0][t] = *exp_next;
+            exp_next += exp_step;
+            if (row + step < p.rows) next_exp = *exp_next;
         }
     }
     team_sync<TEAM>(1 + team);
 
-    float gamma[K][V], dgamma[K][V], dbeta[K][V];
+    constexpr int kPairs = kLnBack / 2;                      // values 2i and 2i + 1 of the thread's sixteen
+    float2 gamma[kPairs], dgamma[kPairs], dbeta[kPairs];
     bool in[K];
 #pragma unroll
-    for (int k = 0; k < K; k++) {
-        const int col = (k * TEAM + t) * V;
-        in[k] = col < n;
+    for (int k = 0; k < K; k++) in[k] = (k * TEAM + t) * V < n;
 #pragma unroll
-        for (int j = 0; j < V; j++) { gamma[k][j] = in[k] ? __ldg(p.gamma + col + j) : 0.f; dgamma[k][j] = dbeta[k][j] = 0.f; }
+    for (int i = 0; i < kLnBack; i++) {
+        const float g = in[i / V] ? __ldg(p.gamma + (i / V * TEAM + t) * V + i % V) : 0.f;
+        if (i & 1) gamma[i / 2].y = g;
+        else gamma[i / 2].x = g;
     }
+#pragma unroll
+    for (int i = 0; i < kPairs; i++) dgamma[i] = dbeta[i] = make_float2(0.f, 0.f);
+    const float inverse_n = 1.0f / (float)n;
     int slot = 0;
     uint32_t phase = 0;
     for (; row < p.rows; row += step, turn ^= 1) {
@@ -443,100 +506,90 @@ __global__ void __launch_bounds__(kLnBlock, 1) ln_backward_rows_kernel(const __g
                 break;
             }
         }
-        const uint8_t *src = mine + (size_t)slot * slot_bytes;
-        const T *dy_row = p.dy + (size_t)row * p.dy_pitch, *x_row = p.x + (size_t)row * p.x_pitch;
-        const T *dy_in = reinterpret_cast<const T *>(src + (reinterpret_cast<uintptr_t>(dy_row) & 15));
-        const T *x_in = reinterpret_cast<const T *>(src + p.dy_bytes + (p.codes ? 0 : (reinterpret_cast<uintptr_t>(x_row) & 15)));
+        const uint8_t *src = mine + (uint32_t)slot * slot_bytes;
+        const T *dy_in = reinterpret_cast<const T *>(src + next_dy_at);
+        const T *x_in = reinterpret_cast<const T *>(src + (V == 1 ? next_x_at : p.dy_bytes));
         const int8_t *code_in = reinterpret_cast<const int8_t *>(src + p.dy_bytes);
-        int dy_first = 0, dy_last = n, x_first = 0, x_last = n;
-        if (V == 1) {
-            whole_pieces(dy_row, n, dy_first, dy_last);
-            if (!p.codes) whole_pieces(x_row, n, x_first, x_last);
-        }
         const float r = next_r, mu = next_mu;
-        float dy[K][V], xh[K][V], s[2] = {0.f, 0.f};
+        float dy[kLnBack], xh[kLnBack];
 #pragma unroll
         for (int k = 0; k < K; k++) {
             const int col = (k * TEAM + t) * V;
+#pragma unroll
+            for (int j = 0; j < V; j++) dy[k * V + j] = xh[k * V + j] = 0.f;
             if (in[k]) {
                 const Pack<T, V> a = load_pack<T, V>(dy_in + col);
 #pragma unroll
-                for (int j = 0; j < V; j++) dy[k][j] = to_float(a.v[j]);
-                if (V == 1) dy[k][0] = col < dy_first && col < 7 ? head_dy : col >= dy_last ? tail_dy : dy[k][0];
+                for (int j = 0; j < V; j++) dy[k * V + j] = to_float(a.v[j]);
+                if (V == 1 && k == 0 && has_head) dy[0] = head_dy;
+                if (V == 1 && has_tail && k == tail_k) dy[k] = tail_dy;
                 if (p.codes) {
-                    ckpt8_values<V>(xh[k], ckpt8_get<V>(code_in + col), exps[team][turn][col / kCkptBlock]);
+                    ckpt8_values<V>(xh + k * V, ckpt8_get<V>(code_in + col), exps[team][turn][col / kCkptBlock]);
                 } else {
                     const Pack<T, V> b = load_pack<T, V>(x_in + col);
 #pragma unroll
-                    for (int j = 0; j < V; j++) xh[k][j] = to_float(b.v[j]);
-                    if (V == 1) xh[k][0] = col < x_first && col < 7 ? head_x : col >= x_last ? tail_x : xh[k][0];
+                    for (int j = 0; j < V; j++) xh[k * V + j] = to_float(b.v[j]);
+                    if (V == 1 && k == 0 && has_head) xh[0] = head_x;
+                    if (V == 1 && has_tail && k == tail_k) xh[k] = tail_x;
 #pragma unroll
-                    for (int j = 0; j < V; j++) xh[k][j] = (xh[k][j] - mu) * r;
+                    for (int j = 0; j < V; j++) xh[k * V + j] = (xh[k * V + j] - mu) * r;
                 }
-            } else {
-#pragma unroll
-                for (int j = 0; j < V; j++) dy[k][j] = xh[k][j] = 0.f;
             }
+        }
+        float2 g[kPairs], s1 = make_float2(0.f, 0.f), s2 = s1;
 #pragma unroll
-            for (int j = 0; j < V; j++) {
-                dgamma[k][j] = fmaf(dy[k][j], xh[k][j], dgamma[k][j]);
-                dbeta[k][j] += dy[k][j];
-                dy[k][j] *= gamma[k][j];                    // g
-                s[0] += dy[k][j];
-                s[1] = fmaf(dy[k][j], xh[k][j], s[1]);
-            }
+        for (int i = 0; i < kPairs; i++) {
+            const float2 d = make_float2(dy[2 * i], dy[2 * i + 1]), h = make_float2(xh[2 * i], xh[2 * i + 1]);
+            dgamma[i] = fma2(d, h, dgamma[i]);
+            dbeta[i] = add2(dbeta[i], d);
+            g[i] = mul2(d, gamma[i]);
+            s1 = add2(s1, g[i]);
+            s2 = fma2(g[i], h, s2);
         }
         if (has_exp) {
             exps[team][turn ^ 1][t] = next_exp;
-            if (row + 2ll * step < p.rows) next_exp = p.exponents[(size_t)(row + 2 * step) * p.blocks + t];
+            exp_next += exp_step;
+            if (row + 2ll * step < p.rows) next_exp = *exp_next;
         }
         if (row + step < p.rows) ahead(row + step);
-        team_total<TEAM, 2>(s, scratch[team], 1 + team);    // and with it: every thread has read the slot, and wrote its exponents
+        // after the barrier in here every thread has read the slot and written its exponents
+        const float2 s = team_totals<TEAM>(make_float2(s1.x + s1.y, s2.x + s2.y), scratch[team][turn], 1 + team);
         if (TEAM == 32) __syncwarp();
         if (t == 0 && row + (long long)depth * step < p.rows) issue(row + depth * step, slot);
         if (++slot == depth) { slot = 0; phase ^= 1u; }
-        const float c1 = s[0] / (float)n, c2 = s[1] / (float)n;
-        T *dx_row = p.dx + (size_t)row * p.dx_pitch;
+        const float c1 = s.x * inverse_n, c2 = s.y * inverse_n;
+        float dx[kLnBack];
 #pragma unroll
-        for (int k = 0; k < K; k++) {
-            if (!in[k]) continue;
-            float dx[V];
-#pragma unroll
-            for (int j = 0; j < V; j++) dx[j] = r * (dy[k][j] - c1 - xh[k][j] * c2);
-            store_pack<T, V>(dx_row + (k * TEAM + t) * V, dx);
+        for (int i = 0; i < kPairs; i++) {
+            const float2 d = add2(g[i], make_float2(-c1, -c1));
+            const float2 v = mul2(fma2(make_float2(xh[2 * i], xh[2 * i + 1]), make_float2(-c2, -c2), d), make_float2(r, r));
+            dx[2 * i] = v.x;
+            dx[2 * i + 1] = v.y;
         }
+#pragma unroll
+        for (int k = 0; k < K; k++)
+            if (in[k]) store_pack<T, V>(dx_row + (k * TEAM + t) * V, dx + k * V);
+        dx_row += dx_step;
     }
     if (limit == 0) {                                       // copies still under way get time to land before the block ends
         for (int k = 0; k < 1000; k++) __nanosleep(200);
     }
     if (!p.weights) return;
-    // the teams' sums, pair by pair (the ring is free: every copy has been waited for)
+    // the teams' sums, two by two (the ring is free: every copy has been waited for)
     __syncthreads();
-    float *tree = reinterpret_cast<float *>(ring);
+    float2 *tree = reinterpret_cast<float2 *>(ring);
 #pragma unroll
     for (int half = kTeams / 2; half > 0; half /= 2) {
         if (team >= half && team < 2 * half) {
-            float *a = tree + (size_t)(team - half) * 2 * kColumns;
+            float2 *a = tree + (size_t)(team - half) * kColumns;
 #pragma unroll
-            for (int k = 0; k < K; k++) {
-#pragma unroll
-                for (int j = 0; j < V; j++) {
-                    a[(k * TEAM + t) * V + j] = dgamma[k][j];
-                    a[kColumns + (k * TEAM + t) * V + j] = dbeta[k][j];
-                }
-            }
+            for (int i = 0; i < kPairs; i++) { a[i * TEAM + t] = dgamma[i]; a[(kPairs + i) * TEAM + t] = dbeta[i]; }
         }
         __syncthreads();
         if (team < half) {
-            const float *a = tree + (size_t)team * 2 * kColumns;
+            const float2 *a = tree + (size_t)team * kColumns;
 #pragma unroll
-            for (int k = 0; k < K; k++) {
-#pragma unroll
-                for (int j = 0; j < V; j++) {
-                    dgamma[k][j] += a[(k * TEAM + t) * V + j];
-                    dbeta[k][j] += a[kColumns + (k * TEAM + t) * V + j];
-                }
-            }
+            for (int i = 0; i < kPairs; i++) { dgamma[i] = add2(dgamma[i], a[i * TEAM + t]); dbeta[i] = add2(dbeta[i], a[(kPairs + i) * TEAM + t]); }
         }
         __syncthreads();
     }
@@ -544,14 +597,12 @@ __global__ void __launch_bounds__(kLnBlock, 1) ln_backward_rows_kernel(const __g
     float *out_g = p.groups == 1 ? p.dgamma : p.part + (size_t)blockIdx.x * 2 * n, *out_b = p.groups == 1 ? p.dbeta : out_g + n;
     const bool add = p.groups == 1 && p.accumulate;
 #pragma unroll
-    for (int k = 0; k < K; k++) {
-        if (!in[k]) continue;
-        const int col = (k * TEAM + t) * V;
-#pragma unroll
-        for (int j = 0; j < V; j++) {
-            out_g[col + j] = add ? out_g[col + j] + dgamma[k][j] : dgamma[k][j];
-            out_b[col + j] = add ? out_b[col + j] + dbeta[k][j] : dbeta[k][j];
-        }
+    for (int i = 0; i < kLnBack; i++) {
+        if (!in[i / V]) continue;
+        const int col = (i / V * TEAM + t) * V + i % V;
+        const float vg = i & 1 ? dgamma[i / 2].y : dgamma[i / 2].x, vb = i & 1 ? dbeta[i / 2].y : dbeta[i / 2].x;
+        out_g[col] = add ? out_g[col] + vg : vg;
+        out_b[col] = add ? out_b[col] + vb : vb;
     }
 }
 
@@ -590,9 +641,8 @@ __global__ void __launch_bounds__(kLnSlice) ln_backward_columns_kernel(const __g
                     s2 = fmaf(g, xh[j], s2);
                 }
             }
-            s1 = warp_total(s1);
-            s2 = warp_total(s2);
-            if (lane == 0) p.row_part[(size_t)(row + u) * p.pieces + piece] = make_float2(s1, s2);
+            const float2 both = warp_totals(make_float2(s1, s2));
+            if (lane == 0) p.row_part[(size_t)(row + u) * p.pieces + piece] = both;
         }
     }
     if (!p.weights || !in) return;
@@ -605,9 +655,10 @@ template <typename T, int V>
 __global__ void __launch_bounds__(256) ln_backward_apply_kernel(const __grid_constant__ LnBackward<T> p)
 {
     constexpr int K = 4;
-    __shared__ float scratch[16];
+    __shared__ float2 scratch[2][8];
     grid_dependency_wait();
-    for (int row = blockIdx.y; row < p.rows; row += gridDim.y) {
+    int turn = 0;
+    for (int row = blockIdx.y; row < p.rows; row += gridDim.y, turn ^= 1) {
         LnRaw<T, V> raw[K];
         const size_t base = (size_t)blockIdx.x * 256 * K * V;
 #pragma unroll
@@ -615,14 +666,10 @@ __global__ void __launch_bounds__(256) ln_backward_apply_kernel(const __grid_con
             const size_t col = base + (size_t)(k * 256 + threadIdx.x) * V;
             if (col < p.n) ln_load<T, V>(p, row, col, raw[k]);
         }
-        float s[2] = {0.f, 0.f};
-        for (int i = threadIdx.x; i < p.pieces; i += 256) {
-            const float2 v = p.row_part[(size_t)row * p.pieces + i];
-            s[0] += v.x;
-            s[1] += v.y;
-        }
-        team_total<256, 2>(s, scratch, 1);
-        const float c1 = s[0] / (float)p.n, c2 = s[1] / (float)p.n, mu = p.mean ? p.mean[row] : 0.f, r = p.rstd[row];
+        float2 s = make_float2(0.f, 0.f);
+        for (int i = threadIdx.x; i < p.pieces; i += 256) s = add2(s, p.row_part[(size_t)row * p.pieces + i]);
+        s = team_totals<256>(s, scratch[turn], 1);
+        const float c1 = s.x / (float)p.n, c2 = s.y / (float)p.n, mu = p.mean ? p.mean[row] : 0.f, r = p.rstd[row];
 #pragma unroll
         for (int k = 0; k < K; k++) {
             const size_t col = base + (size_t)(k * 256 + threadIdx.x) * V;
@@ -671,10 +718,10 @@ static LnPlan ln_plan(int rows, size_t n, int v)
     LnPlan w = {};
     w.one_pass = n <= kLnOnePass;
     if (w.one_pass) {
-        w.team = n <= 256 ? 32 : n <= 1024 ? 128 : n <= 2048 ? 256 : n <= 4096 ? 512 : 1024;
-        // One block where each team then has four rows at most: it writes the gradients itself.
+        w.team = n <= 512 ? 32 : n <= 1024 ? 64 : n <= 2048 ? 128 : n <= 4096 ? 256 : 512;
+        // One block where each team then has eight rows at most: it writes the gradients itself.
         const int teams = kLnBlock / w.team;
-        w.groups = rows <= 4 * teams ? 1 : min((rows + teams - 1) / teams, sm_count());
+        w.groups = rows <= 8 * teams ? 1 : min((rows + teams - 1) / teams, sm_count());
     } else {
         const size_t slices = (n + (size_t)kLnSlice * v - 1) / ((size_t)kLnSlice * v);
         w.pieces = (int)slices * (kLnSlice / 32);
@@ -711,10 +758,10 @@ static int ln_backward_launch(LnBackward<T> p, float *dgamma, float *dbeta, int 
     } while (0)
         switch (w.team) {
         case 32: B200_LN_ROWS(32); break;
+        case 64: B200_LN_ROWS(64); break;
         case 128: B200_LN_ROWS(128); break;
         case 256: B200_LN_ROWS(256); break;
-        case 512: B200_LN_ROWS(512); break;
-        default: B200_LN_ROWS(1024); break;
+        default: B200_LN_ROWS(512); break;
         }
 #undef B200_LN_ROWS
         B200_LAUNCH_CHECK();
