@@ -528,6 +528,11 @@ ckpt8_wgrad_tc_kernel(const __grid_constant__ CUtensorMap codes_map, const __gri
             const int row0 = rank * 128 + warp * 32, o0 = w.mt * kPairTile + row0;
             const size_t i0 = (size_t)w.nt * kPairTile;
             const uint32_t src = tmem + (uint32_t)acc * 256u + ((uint32_t)(warp * 32) << 16);
+            // where nothing is ragged: 16 bytes a thread, eight threads on 128 bytes of a row, four rows at a time
+            const size_t pitch = w.unit >= 0 ? (size_t)kPairTile : p.in;
+            const bool even = w.unit >= 0 || (p.vector_out && o0 + 32 <= p.out && i0 + kPairTile <= p.in);
+            float *corner = w.unit >= 0 ? p.partial + (size_t)w.unit * kUnitFloats + (size_t)row0 * kPairTile : p.dweight + (size_t)o0 * p.in + i0;
+            corner += (size_t)sub * pitch + quad;
             for (int col = 0; col < kPairTile; col += 32) {
                 uint32_t v[32];
                 ptx::tmem_ld16_issue(src + col, v);
@@ -543,30 +548,28 @@ ckpt8_wgrad_tc_kernel(const __grid_constant__ CUtensorMap codes_map, const __gri
 #pragma unroll
                 for (int k = 0; k < 32; k += 4) *reinterpret_cast<uint4 *>(mine + lane * kPitch + k) = make_uint4(v[k], v[k + 1], v[k + 2], v[k + 3]);
                 __syncwarp();
-                const size_t i = i0 + col + quad;
+                if (even) {
+                    float4 x[8];
 #pragma unroll
-                for (int k = 0; k < 32; k += 4) {
-                    const int rr = k + sub;
-                    const float4 x = *reinterpret_cast<const float4 *>(mine + rr * kPitch + quad);
-                    float *dst;
-                    bool wide;
-                    if (w.unit >= 0) {
-                        dst = p.partial + (size_t)w.unit * kUnitFloats + (size_t)(row0 + rr) * kPairTile + col + quad;
-                        wide = true;
-                    } else {
-                        if (o0 + rr >= p.out) continue;
-                        dst = p.dweight + (size_t)(o0 + rr) * p.in + i;
-                        wide = p.vector_out && i + 4 <= p.in;
+                    for (int k = 0; k < 8; k++) x[k] = *reinterpret_cast<const float4 *>(mine + (4 * k + sub) * kPitch + quad);
+                    float *dst = corner + col;
+                    if (add) {
+                        float4 old[8];
+#pragma unroll
+                        for (int k = 0; k < 8; k++) old[k] = *reinterpret_cast<const float4 *>(dst + (size_t)(4 * k) * pitch);
+#pragma unroll
+                        for (int k = 0; k < 8; k++) { x[k].x += old[k].x; x[k].y += old[k].y; x[k].z += old[k].z; x[k].w += old[k].w; }
                     }
-                    if (wide) {
-                        float4 y = x;
-                        if (add) {
-                            const float4 old = *reinterpret_cast<const float4 *>(dst);
-                            y.x += old.x; y.y += old.y; y.z += old.z; y.w += old.w;
-                        }
-                        *reinterpret_cast<float4 *>(dst) = y;
-                    } else {
+#pragma unroll
+                    for (int k = 0; k < 8; k++) *reinterpret_cast<float4 *>(dst + (size_t)(4 * k) * pitch) = x[k];
+                } else {
+                    const size_t i = i0 + col + quad;
+                    for (int k = 0; k < 8; k++) {
+                        const int rr = 4 * k + sub;
+                        if (o0 + rr >= p.out) break;
+                        const float4 x = *reinterpret_cast<const float4 *>(mine + rr * kPitch + quad);
                         const float y[4] = {x.x, x.y, x.z, x.w};
+                        float *dst = corner + col + (size_t)(4 * k) * pitch;
 #pragma unroll
                         for (int m = 0; m < 4; m++)
                             if (i + m < p.in) dst[m] = add ? dst[m] + y[m] : y[m];
