@@ -363,8 +363,10 @@ ckpt8_wgrad_tc_kernel(const __grid_constant__ CUtensorMap codes_map, const __gri
             }
             if (!more) break;
             if (ok) {
-                if (lane == 0) ok = wait_bar(raw_full_bar(rs), rphase, abort_flag, p.status, 0x800u + B200_E_TIMEOUT);
-                ok = __shfl_sync(0xffffffffu, ok, 0);
+                // All lanes wait: where one waits and the others stand by, the warp stays divided after it and does the stage's work
+                // twice (fp32, 8192 x 4096 x 4096: 1320 us in place of 804; bf16 328 in place of 271).
+                ok = wait_bar(raw_full_bar(rs), rphase, abort_flag, p.status, 0x800u + B200_E_TIMEOUT);
+                ok = __all_sync(0xffffffffu, ok);
                 const uint8_t *raw = smem + S::kRing + (uint32_t)rs * S::kRaw;
                 // Chunks 2c and 2c + 1 of a row's sixteen.  The threads of the row's second half take theirs in the other order, so that
                 // no two of a store meet in a bank.
@@ -381,8 +383,8 @@ ckpt8_wgrad_tc_kernel(const __grid_constant__ CUtensorMap codes_map, const __gri
                         __syncwarp();
                         if (lane == 0) ptx::mbar_arrive(raw_empty_bar(rs));
                     }
-                    if (lane == 0) ok = wait_bar(empty_bar(stage), phase ^ 1u, abort_flag, p.status, 0x900u + B200_E_TIMEOUT);
-                    ok = __shfl_sync(0xffffffffu, ok, 0);
+                    ok = wait_bar(empty_bar(stage), phase ^ 1u, abort_flag, p.status, 0x900u + B200_E_TIMEOUT);
+                    ok = __all_sync(0xffffffffu, ok);
                 }
                 if (ok) {
                     uint8_t *tile = smem + (uint32_t)stage * S::kStage;
@@ -439,8 +441,8 @@ ckpt8_wgrad_tc_kernel(const __grid_constant__ CUtensorMap codes_map, const __gri
                         // the bias gradient sums delta from the operand tile, which is not loaded again until every warp of the group has
                         // arrived here
                         if (bias) {
-                            if (lane == 0) ok = wait_bar(full_bar(stage), phase, abort_flag, p.status, 0xa00u + B200_E_TIMEOUT);
-                            ok = __shfl_sync(0xffffffffu, ok, 0);
+                            ok = wait_bar(full_bar(stage), phase, abort_flag, p.status, 0xa00u + B200_E_TIMEOUT);
+                            ok = __all_sync(0xffffffffu, ok);
                             if (ok) {
 #pragma unroll
                                 for (int k = 0; k < S::kDeltaPasses; k++) {
@@ -521,9 +523,8 @@ ckpt8_wgrad_tc_kernel(const __grid_constant__ CUtensorMap codes_map, const __gri
             const WorkItem w = at.w;
             const bool add = !w.first || (w.unit < 0 && p.accumulate);
             const int acc = n % kAccumulators;
-            bool ok = lane == 0 ? wait_bar(tfull_bar(acc), (uint32_t)(n / kAccumulators) & 1u, abort_flag, p.status, 0x400u + B200_E_TIMEOUT) : true;
-            ok = __shfl_sync(0xffffffffu, ok, 0);
-            if (!ok) break;
+            const bool ok = wait_bar(tfull_bar(acc), (uint32_t)(n / kAccumulators) & 1u, abort_flag, p.status, 0x400u + B200_E_TIMEOUT);
+            if (!__all_sync(0xffffffffu, ok)) break;
             ptx::tc_fence_after();
             const int row0 = rank * 128 + warp * 32, o0 = w.mt * kPairTile + row0;
             const size_t i0 = (size_t)w.nt * kPairTile;
