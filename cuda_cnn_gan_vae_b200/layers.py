@@ -112,15 +112,19 @@ class NetLayerBackConvolution(NetLayerConvolution):
 class NetLayerLinear(_Layer):
     """netlayer/cnetlayerlinear.cu.h: Forward :262 (H = W*x + B per sample), TrainingBackward :415 (prev error =
     W^T*delta; dW += sum over samples of delta*x^T; dB += sum of delta).  The three products are one GEMM each over the
-    whole batch; the reference's [batch, out, in] scratch of per-sample outer products is not materialised."""
+    whole batch; the reference's [batch, out, in] scratch of per-sample outer products is not materialised.
 
-    def __init__(self, in_shape, batch, neurons):
+    checkpoint8: the layer keeps its input in 8 bits (ops.Checkpoint8) and forms its weight and bias gradients from that; the
+    tensor it was given is not needed after Forward."""
+
+    def __init__(self, in_shape, batch, neurons, checkpoint8=False):
         self.in_shape, self.batch, self.neurons = tuple(in_shape), batch, neurons
         self.n_in = int(np.prod(in_shape))
         self.out_shape = (1, neurons, 1)
         self.H = torch.empty((batch, 1, neurons, 1), device="cuda")
         self.prev_error = torch.empty((batch,) + self.in_shape, device="cuda")
-        self.tmp_dw = torch.empty((1, 1, neurons, self.n_in), device="cuda")
+        self.kept = ops.Checkpoint8.empty(batch, self.n_in) if checkpoint8 else None
+        self.tmp_dw = None if checkpoint8 else torch.empty((1, 1, neurons, self.n_in), device="cuda")
 
     def param_shapes(self):
         return {"w": (1, 1, self.neurons, self.n_in), "b": (1, 1, self.neurons, 1)}
@@ -130,7 +134,10 @@ class NetLayerLinear(_Layer):
         self.w["b"].zero_()
 
     def Forward(self, x):
-        self.x = x
+        if self.kept is not None:
+            self.kept.store(x.view(self.batch, self.n_in))
+        else:
+            self.x = x
         ops.CTensorMath.Mul(self.H, self.w["w"], x.view(self.batch, 1, self.n_in, 1))
         ops.CTensorMath.Add(self.H, self.H, self.w["b"])
         return self.H
@@ -139,7 +146,9 @@ class NetLayerLinear(_Layer):
         delta = delta.view(self.batch, 1, self.neurons, 1)
         if need_prev:
             ops.CTensorMath.TransponseMul(self.prev_error.view(self.batch, 1, self.n_in, 1), self.w["w"], delta)
-        if create_delta_weight:
+        if create_delta_weight and self.kept is not None:
+            ops.checkpoint_wgrad(self.g["w"], self.g["b"], delta.view(self.batch, self.neurons), self.kept)
+        elif create_delta_weight:
             # sum_b delta_b * x_b^T = D^T * X with D = [batch, out] and X = [batch, in] as stored
             ops.CTensorMath.TransponseMul(self.tmp_dw, delta.view(1, 1, self.batch, self.neurons), self.x.view(1, 1, self.batch, self.n_in))
             ops.CTensorMath.Add(self.g["w"], self.g["w"], self.tmp_dw)
@@ -149,7 +158,10 @@ class NetLayerLinear(_Layer):
 
 class NetLayerFunction(_Layer):
     """netlayer/cnetlayerfunction.cu.h: Forward applies the neuron function; SetOutputError :347-358 forms
-    delta = f'(layer input) * error, which TrainingBackward hands to the previous layer."""
+    delta = f'(layer input) * error, which TrainingBackward hands to the previous layer.
+
+    checkpoint8: the layer keeps its input in 8 bits, signs kept, so that the errors below ReLU and LeakyReLU are those of the
+    tensor itself and the other functions' are taken at the kept values.  Such a layer is not folded into a convolution layer."""
 
     # folded = "into_next": the convolution layer behind applies the function while it packs its input (Forward here only
     # remembers its input; H is written by that layer when `materialise` is set); folded = "into_prev": the convolution layer
@@ -157,13 +169,18 @@ class NetLayerFunction(_Layer):
     folded = None
     materialise = True
 
-    def __init__(self, in_shape, batch, func, leaky_slope=0.1):
+    def __init__(self, in_shape, batch, func, leaky_slope=0.1, checkpoint8=False):
         self.in_shape = self.out_shape = tuple(in_shape)
         self.batch, self.func, self.slope = batch, func, leaky_slope
+        self.kept = ops.Checkpoint8.empty(batch, int(np.prod(self.in_shape))) if checkpoint8 else None
         self.H = torch.empty((batch,) + self.in_shape, device="cuda")
         self.delta = torch.empty((batch,) + self.in_shape, device="cuda")
 
     def Forward(self, x):
+        if self.kept is not None:
+            self.kept.store(x.view(self.batch, -1), keep_sign=True)
+            ops.CTensorApplyFunc.Apply(self.H, x, self.func, self.slope)
+            return self.H
         if self.folded == "into_prev":
             return self.H                   # written by the convolution layer in front; self.x was set by Net
         self.x = x
@@ -173,7 +190,7 @@ class NetLayerFunction(_Layer):
         return self.H
 
     def TrainingBackward(self, error, create_delta_weight=True, need_prev=True):
-        ops.CTensorApplyFunc.Backward(self.delta, self.x, error, self.func, self.slope)
+        ops.CTensorApplyFunc.Backward(self.delta, self.x if self.kept is None else self.kept, error, self.func, self.slope)
         return self.delta
 
 
@@ -230,6 +247,48 @@ class NetLayerBatchNormalizationFunction(NetLayerBatchNormalization):
         _check(load().b200_bn_act_backward(_ptr(self.prev_error), _ptr(self.g["gamma"]), _ptr(self.g["beta"]), _ptr(error), _ptr(self.xhat),
                                            _ptr(self.ivar), _ptr(self.w["gamma"]), _ptr(self.w["beta"]), self.batch, self.n,
                                            int(create_delta_weight), ACT[self.func], self.slope, _stream()))
+        return self.prev_error
+
+
+class NetLayerLayerNormalization(_Layer):
+    """Layer normalisation: statistics of each sample itself (batch normalisation mixes the samples of a batch, which a gradient
+    penalty per sample or a batch of one does not allow).  dims: how many of the dimensions (Z, Y, X) are normalised together, from
+    the last: 3 the whole sample, 2 every plane, 1 every row of X.  No reference counterpart.
+
+    checkpoint8: the normalised values are kept in 8 bits for the way back instead of the layer's input, which is not
+    needed after Forward."""
+
+    def __init__(self, in_shape, batch, dims=3, eps=1e-6, checkpoint8=False):
+        self.in_shape = self.out_shape = tuple(in_shape)
+        if dims not in (1, 2, 3):
+            raise ops.B200Error(2, "layer normalisation is over 1, 2 or 3 dimensions")
+        self.batch, self.eps = batch, eps
+        self.norm_shape = (1,) * (4 - dims) + self.in_shape[3 - dims:]
+        self.n = int(np.prod(self.norm_shape))
+        self.rows = batch * int(np.prod(self.in_shape)) // self.n
+        self.H, self.prev_error = (torch.empty((batch,) + self.in_shape, device="cuda") for _ in range(2))
+        self.mean, self.rstd = (torch.empty(self.rows, device="cuda") for _ in range(2))
+        self.kept = ops.Checkpoint8.empty(self.rows, self.n) if checkpoint8 else None
+        self.workspace = torch.empty(max(16, load().b200_ln_backward_workspace(self.rows, self.n)), dtype=torch.uint8, device="cuda")
+
+    def param_shapes(self):
+        return {"gamma": self.norm_shape, "beta": self.norm_shape}
+
+    def init(self, rng):
+        self.w["gamma"].fill_(1.0)
+        self.w["beta"].zero_()
+
+    def Forward(self, x):
+        if self.kept is None:
+            self.x = x
+        ops.ln_forward(x.view(self.rows, self.n), self.w["gamma"], self.w["beta"], self.eps, y=self.H.view(self.rows, self.n),
+                       mean=self.mean, rstd=self.rstd, checkpoint=self.kept)
+        return self.H
+
+    def TrainingBackward(self, delta, create_delta_weight=True, need_prev=True):
+        ops.ln_backward(delta.view(self.rows, self.n), self.x.view(self.rows, self.n) if self.kept is None else self.kept, self.mean,
+                        self.rstd, self.w["gamma"], self.g["gamma"], self.g["beta"], create_delta_weight,
+                        dx=self.prev_error.view(self.rows, self.n), workspace=self.workspace)
         return self.prev_error
 
 
@@ -340,22 +399,29 @@ class Net:
     TrainingResetDeltaWeight, Forward of all layers, SetOutputError on the last, TrainingBackward in reverse order,
     TrainingUpdateWeight) on four arenas: weights, gradients, Adam m and v."""
 
-    def __init__(self, in_shape, batch, spec, seed=0, peer=False, channel=0, fold=True):
+    def __init__(self, in_shape, batch, spec, seed=0, peer=False, channel=0, fold=True, checkpoint8=False):
         """spec: list of (class, kwargs).  The input of layer i is the output of layer i-1.
         peer: True, or a PeerBuffer shared with other nets.  With several ranks, the weight and gradient arenas are placed in
         the PeerBuffer (memory every rank maps), and
         TrainingUpdateWeight(fused=True) runs the library's reduce-scatter + Adam + all-gather kernel on `channel`.
-        fold: function layers next to a convolution layer are folded into that layer's Forward (see fold_functions)."""
+        fold: function layers next to a convolution layer are folded into that layer's Forward (see fold_functions).
+        checkpoint8: the Linear, function and layer-normalisation layers keep what their backward passes need in 8 bits.  A net of
+        only such layers then holds two output tensors and two error tensors in all, used in turn by its layers, in place
+        of two for each."""
         self.batch, self.in_shape = batch, tuple(in_shape)
         self.layers, shape = [], tuple(in_shape)
         for cls, kw in spec:
             if cls == "reshape":             # ReinterpretSize of the previous output (cuda/ctensor.cu.h): no data moves
                 shape = tuple(kw)
                 continue
+            if checkpoint8 and cls in (NetLayerLinear, NetLayerFunction, NetLayerLayerNormalization):
+                kw = dict(kw, checkpoint8=True)
             layer = cls(shape, batch, **kw)
             self.layers.append(layer)
             shape = layer.out_shape
         self.out_shape = shape
+        if self.layers and all(getattr(layer, "kept", None) is not None for layer in self.layers):
+            self.share_tensors()
         self.fold_functions(fold)
         shapes = {}
         for i, layer in enumerate(self.layers):
@@ -396,7 +462,7 @@ class Net:
         if not enable or os.environ.get("B200CONV_FOLD") == "0":          # tuning aid: B200CONV_FOLD=0 keeps every layer separate
             return
         for i, layer in enumerate(self.layers):
-            if not isinstance(layer, NetLayerFunction):
+            if not isinstance(layer, NetLayerFunction) or layer.kept is not None:
                 continue
             prev_l = self.layers[i - 1] if i > 0 else None
             next_l = self.layers[i + 1] if i + 1 < len(self.layers) else None
@@ -407,6 +473,19 @@ class Net:
                 layer.folded, prev_l.after = "into_prev", layer
             elif isinstance(next_l, conv) and next_l.in_shape == layer.out_shape:
                 layer.folded, layer.materialise, next_l.before = "into_next", materialise, layer
+
+    def share_tensors(self):
+        """Two output tensors and two error tensors for all layers (each of which keeps what it needs in a checkpoint): layer i
+        reads the one that layer i - 1 wrote and writes the other."""
+        def shared(count):
+            return [torch.empty(max([count(layer) for layer in self.layers[k::2]], default=0), device="cuda") for k in range(2)]
+        outs = shared(lambda layer: self.batch * int(np.prod(layer.out_shape)))
+        errors = shared(lambda layer: self.batch * int(np.prod(layer.in_shape)))
+        for i, layer in enumerate(self.layers):
+            layer.H = outs[i % 2][:layer.H.numel()].view(layer.H.shape)
+            name = "delta" if isinstance(layer, NetLayerFunction) else "prev_error"
+            old = getattr(layer, name)
+            setattr(layer, name, errors[i % 2][:old.numel()].view(old.shape))
 
     @property
     def parameter_count(self):

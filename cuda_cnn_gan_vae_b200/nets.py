@@ -7,7 +7,7 @@ import torch
 from . import ops
 from .lib import load
 from .layers import (AdamCorrections, Net, NetLayerBackConvolution, NetLayerBatchNormalization, NetLayerBatchNormalizationFunction,
-                     NetLayerConvolution, NetLayerFunction, NetLayerLinear, NetLayerMaxPooling, NetLayerUpSampling)
+                     NetLayerConvolution, NetLayerFunction, NetLayerLayerNormalization, NetLayerLinear, NetLayerMaxPooling, NetLayerUpSampling)
 
 
 def _bn_function(spec, fused, leaky_slope):
@@ -34,15 +34,24 @@ def dcgan_generator(batch, noise=100, base=512, widths=(256, 128, 64, 3), leaky_
     return Net((1, noise, 1), batch, spec, seed=seed, peer=peer, channel=channel)
 
 
-def dcgan_discriminator(batch, image=(3, 64, 64), widths=(64, 128, 256, 512), leaky_slope=0.2, seed=3, fused=False, peer=False, channel=0):
-    """image -> 4x4 stride-2 convolutions with batch normalisation and LeakyReLU -> Linear to one logit -> sigmoid."""
+def dcgan_discriminator(batch, image=(3, 64, 64), widths=(64, 128, 256, 512), leaky_slope=0.2, seed=3, fused=False, peer=False, channel=0,
+                        norm="batch", checkpoint8=False):
+    """image -> 4x4 stride-2 convolutions with batch normalisation and LeakyReLU -> Linear to one logit -> sigmoid.
+    norm="layer": every sample normalised by itself (a discriminator's answer to one image must not depend on the others
+    under a gradient penalty per sample).  checkpoint8: as in Net."""
+    if norm not in ("batch", "layer"):
+        raise ops.B200Error(2, "norm must be 'batch' or 'layer'")
     spec = []
     for width in widths:
         spec.append((NetLayerConvolution, dict(kernel_amount=width, kernel_size=4, stride=2, padding=1)))
-        _bn_function(spec, fused, leaky_slope)
+        if norm == "batch":
+            _bn_function(spec, fused, leaky_slope)
+        else:
+            spec.append((NetLayerLayerNormalization, {}))
+            spec.append((NetLayerFunction, dict(func="leaky_relu", leaky_slope=leaky_slope)))
     spec.append((NetLayerLinear, dict(neurons=1)))
     spec.append((NetLayerFunction, dict(func="sigmoid")))
-    return Net(image, batch, spec, seed=seed, peer=peer, channel=channel)
+    return Net(image, batch, spec, seed=seed, peer=peer, channel=channel, checkpoint8=checkpoint8)
 
 
 class DCGANStep:
@@ -186,12 +195,14 @@ class VAEStep:
     2(x_hat - x)/numel at the output plus the Kullback-Leibler terms at the heads (:424-460); backward through all four
     nets with weight gradients, one all-reduce per gradient arena, Adam on every net."""
 
-    def __init__(self, batch, world=1, image=(3, 128, 128), widths=(32, 64, 128, 256), latent=256, kl_speed=1.0, leaky_slope=0.1):
+    def __init__(self, batch, world=1, image=(3, 128, 128), widths=(32, 64, 128, 256), latent=256, kl_speed=1.0, leaky_slope=0.1,
+                 checkpoint8=False):
+        """checkpoint8: the two heads keep the features they read in 8 bits for their weight gradients."""
         self.batch, self.world, self.kl_speed = batch, world, kl_speed
         self.encoder = vae_encoder(batch, image, widths, leaky_slope)
         feat = self.encoder.out_shape
-        self.mu = Net(feat, batch, [(NetLayerLinear, dict(neurons=latent))], seed=6)
-        self.logvar = Net(feat, batch, [(NetLayerLinear, dict(neurons=latent))], seed=7)
+        self.mu = Net(feat, batch, [(NetLayerLinear, dict(neurons=latent))], seed=6, checkpoint8=checkpoint8)
+        self.logvar = Net(feat, batch, [(NetLayerLinear, dict(neurons=latent))], seed=7, checkpoint8=checkpoint8)
         self.decoder = vae_decoder(batch, latent, feat, tuple(widths[-2::-1]) + (image[0],), leaky_slope)
         assert self.decoder.out_shape == tuple(image), (self.decoder.out_shape, image)
         self.nets = (self.encoder, self.mu, self.logvar, self.decoder)

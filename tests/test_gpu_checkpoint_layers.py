@@ -1,0 +1,242 @@
+"""Layers that normalise per sample and layers that keep what they need in 8 bits, run together as a net trains them."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+from tests import ckpt8_util as cu  # noqa: E402
+
+
+@pytest.fixture(autouse=True)
+def ops():
+    from cuda_cnn_gan_vae_b200 import ops as o
+    yield o
+    o.set_precision(o.TF32X3)
+
+
+def dense(batch, checkpoint8, share=True, widths=(96, 130, 64), inputs=200, func="leaky_relu"):
+    from cuda_cnn_gan_vae_b200.layers import Net, NetLayerFunction, NetLayerLayerNormalization, NetLayerLinear
+    spec = []
+    for w in widths:
+        spec += [(NetLayerLinear, dict(neurons=w)), (NetLayerLayerNormalization, {}), (NetLayerFunction, dict(func=func, leaky_slope=0.2))]
+    spec.append((NetLayerLinear, dict(neurons=7)))
+    keep = Net.share_tensors
+    if not share:
+        Net.share_tensors = lambda self: None
+    try:
+        return Net((1, inputs, 1), batch, spec, seed=1, checkpoint8=checkpoint8)
+    finally:
+        Net.share_tensors = keep
+
+
+def rel(a, b):
+    a, b = a.double(), b.double()
+    return float((a - b).norm() / b.norm())
+
+
+def wide_dense(net, x, error, slope=0.2, kept=None):
+    """Gradients of sum(error * net(x)) in 64 bits by torch's autograd; kept: a list that receives what each layer reads."""
+    from cuda_cnn_gan_vae_b200.layers import NetLayerFunction, NetLayerLayerNormalization, NetLayerLinear
+    params = [{k: v.detach().double().requires_grad_() for k, v in layer.w.items()} if layer.param_shapes() else {} for layer in net.layers]
+    x = x.double().reshape(net.batch, -1).requires_grad_()
+    y = x
+    for layer, w in zip(net.layers, params):
+        if isinstance(layer, NetLayerLinear):
+            y = y @ w["w"].view(layer.neurons, -1).t() + w["b"].view(-1)
+        elif isinstance(layer, NetLayerLayerNormalization):
+            mu = y.mean(1, keepdim=True)
+            y = (y - mu) / ((y - mu).square().mean(1, keepdim=True) + layer.eps).sqrt() * w["gamma"].view(-1) + w["beta"].view(-1)
+        elif isinstance(layer, NetLayerFunction):
+            y = torch.where(y >= 0, y, slope * y)
+    (y * error.double().reshape(net.batch, -1)).sum().backward()
+    return y, x.grad, [{k: v.grad for k, v in w.items()} for w in params]
+
+
+@pytest.mark.parametrize("batch", [1, 5, 64])
+def test_net_with_layer_normalisation_against_autograd(ops, batch):
+    """Without checkpoints: 3xTF32 products are off by about 2^-21 of their terms, each layer's gradient by a few of those."""
+    net = dense(batch, False)
+    x, error = torch.randn(batch, 1, 200, 1, device="cuda"), torch.randn(batch, 1, 7, 1, device="cuda")
+    net.TrainingResetDeltaWeight()
+    y = net.Forward(x)
+    dx = net.TrainingBackward(error, True, need_input_error=True)
+    ops.stream_status()
+    want_y, want_dx, want = wide_dense(net, x, error)
+    assert rel(y.view(batch, -1), want_y) < 1e-4
+    assert rel(dx.view(batch, -1), want_dx) < 1e-4
+    for layer, w in zip(net.layers, want):
+        for name, g in w.items():
+            assert rel(layer.g[name].view(-1), g.view(-1)) < 1e-4, name
+
+
+@pytest.mark.parametrize("func", ["leaky_relu", "tanh", "sigmoid"])
+@pytest.mark.parametrize("batch", [1, 5, 64])
+def test_net_with_checkpoints(ops, batch, func):
+    """The forward pass is that of the net without checkpoints, bit for bit.  A kept value is off by at most 1/127 of its block's
+    largest, a normal one's rms by about 1 % of the tensor's; errors and gradients pass through three such tensors of
+    each kind on their way, so 2-norms within 10 %, and not equal."""
+    plain, kept = dense(batch, False, func=func), dense(batch, True, func=func)
+    x, error = torch.randn(batch, 1, 200, 1, device="cuda"), torch.randn(batch, 1, 7, 1, device="cuda")
+    outs = []
+    for net in (plain, kept):
+        net.TrainingResetDeltaWeight()
+        outs.append((net.Forward(x).clone(), net.TrainingBackward(error, True, need_input_error=True).clone()))
+    ops.stream_status()
+    assert torch.equal(outs[0][0], outs[1][0])
+    assert 0 < rel(outs[1][1], outs[0][1]) < 0.1
+    for a, b in zip(plain.layers, kept.layers):
+        for name in a.param_shapes():
+            assert rel(b.g[name], a.g[name]) < 0.1, name
+    # the last layer's bias gradient reads no kept value at all
+    assert rel(kept.layers[-1].g["b"], plain.layers[-1].g["b"]) < 1e-6
+
+
+def test_shared_tensors_change_nothing_and_inputs_may_go(ops):
+    """Two output and two error tensors for the whole net: the same bits as tensors for every layer; and the net's input may be
+    overwritten once Forward has returned."""
+    apart, shared = dense(33, True, share=False), dense(33, True)
+    assert len({layer.H.data_ptr() for layer in shared.layers}) == 2 and len({layer.H.data_ptr() for layer in apart.layers}) == 10
+    x, error = torch.randn(33, 1, 200, 1, device="cuda"), torch.randn(33, 1, 7, 1, device="cuda")
+    for turn in range(2):
+        outs = []
+        for net in (apart, shared):
+            inp = x.clone()
+            net.TrainingResetDeltaWeight()
+            y = net.Forward(inp).clone()
+            inp.fill_(float("nan"))
+            dx = net.TrainingBackward(error, True, need_input_error=True).clone()
+            outs.append((y, dx, net.grads.buffer.clone()))
+        for a, b in zip(*outs):
+            assert torch.equal(a, b) and torch.isfinite(a).all()
+        x = x * 1.5
+    # 33 bytes for 32 values
+    layer = shared.layers[3]
+    assert layer.kept.codes.numel() + layer.kept.exponents.numel() <= 33 * (96 * 33 // 32)
+
+
+def test_function_layer_with_kept_signs_is_exact(ops):
+    from cuda_cnn_gan_vae_b200.layers import NetLayerFunction
+    for func in ("relu", "leaky_relu"):
+        a, b = NetLayerFunction((3, 9, 11), 4, func), NetLayerFunction((3, 9, 11), 4, func, checkpoint8=True)
+        x, e = torch.randn(4, 3, 9, 11, device="cuda"), torch.randn(4, 3, 9, 11, device="cuda")
+        x[0] *= 1e-7
+        assert torch.equal(a.Forward(x), b.Forward(x))
+        assert torch.equal(a.TrainingBackward(e), b.TrainingBackward(e))
+
+
+@pytest.mark.parametrize("dims", [1, 2, 3])
+@pytest.mark.parametrize("checkpoint8", [False, True])
+def test_layer_normalisation_dims(ops, dims, checkpoint8):
+    from cuda_cnn_gan_vae_b200.dp import GradArena
+    from cuda_cnn_gan_vae_b200.layers import NetLayerLayerNormalization
+    layer = NetLayerLayerNormalization((3, 10, 12), 4, dims=dims, checkpoint8=checkpoint8)
+    w, g = GradArena(layer.param_shapes(), "cuda"), GradArena(layer.param_shapes(), "cuda")
+    layer.bind(w.views, g.views)
+    r = np.random.default_rng(dims)
+    for v in w.views.values():
+        v.copy_(torch.from_numpy(r.normal(1, 0.2, tuple(v.shape)).astype(np.float32)))
+    g.buffer.zero_()
+    x = torch.from_numpy(r.normal(1, 2, (4, 3, 10, 12)).astype(np.float32)).cuda()
+    d = torch.from_numpy(r.normal(0, 1, (4, 3, 10, 12)).astype(np.float32)).cuda()
+    y, dx = layer.Forward(x), layer.TrainingBackward(d)
+    ops.stream_status()
+    axes = tuple(range(4 - dims, 4))
+    X, D = x.double().requires_grad_(), d.double()
+    G, B = (w.views[k].double().requires_grad_() for k in ("gamma", "beta"))
+    mu = X.mean(axes, keepdim=True)
+    Y = (X - mu) / ((X - mu).square().mean(axes, keepdim=True) + 1e-6).sqrt() * G + B
+    (Y * D).sum().backward()
+    tol = 0.03 if checkpoint8 else 1e-5
+    assert rel(y, Y) < 1e-6 and rel(dx, X.grad) < tol and rel(g.views["gamma"], G.grad) < tol and rel(g.views["beta"], B.grad) < 1e-6
+
+
+@pytest.mark.parametrize("checkpoint8", [False, True])
+def test_discriminator_with_layer_normalisation(ops, checkpoint8):
+    """Against autograd in 64 bits; and an image's answer does not depend on the rest of the batch."""
+    from cuda_cnn_gan_vae_b200.nets import dcgan_discriminator
+    net = dcgan_discriminator(4, image=(3, 32, 32), widths=(16, 32, 48), norm="layer", checkpoint8=checkpoint8)
+    x = torch.randn(4, 3, 32, 32, device="cuda")
+    net.TrainingResetDeltaWeight()
+    y = net.Forward(x).clone()
+    dx = net.TrainingBackward(torch.ones_like(y), True, need_input_error=True)
+    ops.stream_status()
+    X = x.double().requires_grad_()
+    h, ws = X, []
+    for i in range(3):
+        conv, norm = net.layers[3 * i], net.layers[3 * i + 1]
+        w = [conv.w["kernel"].double().requires_grad_(), conv.w["bias"].double().requires_grad_(), norm.w["gamma"].double().requires_grad_(),
+             norm.w["beta"].double().requires_grad_()]
+        ws.append((w, [conv.g["kernel"], conv.g["bias"], norm.g["gamma"], norm.g["beta"]]))
+        h = torch.nn.functional.conv2d(h, w[0].view(conv.K, -1, 4, 4), w[1].view(-1), stride=2, padding=1)
+        mu = h.mean((1, 2, 3), keepdim=True)
+        h = (h - mu) / ((h - mu).square().mean((1, 2, 3), keepdim=True) + 1e-6).sqrt() * w[2] + w[3]
+        h = torch.where(h >= 0, h, 0.2 * h)
+    lin = net.layers[-2]
+    w = [lin.w["w"].double().requires_grad_(), lin.w["b"].double().requires_grad_()]
+    ws.append((w, [lin.g["w"], lin.g["b"]]))
+    out = torch.sigmoid(h.reshape(4, -1) @ w[0].view(1, -1).t() + w[1].view(-1))
+    out.sum().backward()
+    assert rel(y.view(-1), out.view(-1)) < 1e-4
+    # 3xTF32 convolutions without checkpoints; three kept tensors of each kind with them (as above)
+    tol = 0.1 if checkpoint8 else 1e-3
+    assert rel(dx, X.grad) < tol
+    for want, got in ws:
+        for a, b in zip(want, got):
+            # (a convolution's bias in front of a normalisation shifts nothing but the few values at the borders' share: its
+            # gradient is a difference of large sums, held to the size of what is summed)
+            assert float((b.view(-1).double() - a.grad.view(-1)).norm()) <= tol * max(float(a.grad.norm()), 0.05 * float(dx.double().norm()))
+    alone = net.Forward(torch.cat([x[:1], torch.randn(3, 3, 32, 32, device="cuda") * 3]))
+    assert torch.equal(alone[0], y[0])
+
+
+def test_vae_step_with_checkpointed_heads(ops):
+    """The heads' forward passes and the errors they hand down are unchanged; their weight gradients come from the kept features."""
+    from cuda_cnn_gan_vae_b200.nets import VAEStep
+    grads = []
+    x, eps = torch.rand(6, 3, 32, 32, device="cuda"), torch.randn(6, 1, 24, 1, device="cuda")
+    for checkpoint8 in (False, True):
+        step = VAEStep(6, image=(3, 32, 32), widths=(8, 16, 32), latent=24, checkpoint8=checkpoint8)
+        x_hat = step(x, eps).clone()
+        ops.stream_status()
+        grads.append((x_hat, step.feat_error.clone(), step.mu.grads.buffer.clone(), step.logvar.grads.buffer.clone()))
+    (h0, e0, m0, l0), (h1, e1, m1, l1) = grads
+    assert torch.equal(h0, h1) and torch.equal(e0, e1)
+    assert 0 < rel(m1, m0) < 0.03 and 0 < rel(l1, l0) < 0.03
+
+
+@pytest.mark.parametrize("mode", ["TF32X3", "TF32", "FP32"])
+def test_captured_training_steps(ops, mode):
+    """Whole steps (forward, backward, Adam) captured and replayed give the weights of eager ones."""
+    from cuda_cnn_gan_vae_b200.layers import AdamCorrections
+    ops.set_precision(getattr(ops, mode))
+    nets = [dense(40, True), dense(40, True)]
+    x, error = torch.randn(40, 1, 200, 1, device="cuda"), torch.randn(40, 1, 7, 1, device="cuda")
+    corr = AdamCorrections()
+
+    def step(net):
+        net.TrainingResetDeltaWeight()
+        net.Forward(x)
+        net.TrainingBackward(error)
+        net.TrainingUpdateWeight(1e-3, None, corrections=corr.device)
+    corr.set(1)
+    step(nets[0]), step(nets[1])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(nets[1])
+    for it in range(2, 5):
+        corr.set(it)
+        step(nets[0])
+        graph.replay()
+    ops.stream_status()
+    assert torch.equal(nets[0].weights.buffer, nets[1].weights.buffer) and torch.isfinite(nets[0].weights.buffer).all()
+
+
+def test_refusals(ops):
+    from cuda_cnn_gan_vae_b200.layers import NetLayerLayerNormalization
+    from cuda_cnn_gan_vae_b200.nets import dcgan_discriminator
+    with pytest.raises(ops.B200Error):
+        NetLayerLayerNormalization((3, 4, 5), 2, dims=4)
+    with pytest.raises(ops.B200Error):
+        dcgan_discriminator(2, image=(3, 32, 32), widths=(8,), norm="group")
