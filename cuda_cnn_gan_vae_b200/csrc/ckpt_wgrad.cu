@@ -692,7 +692,7 @@ static int wgrad_tc_launch(WgradParams p, const WgradPlan &w, const void *delta,
     r = tensor_map_2d(&delta_map, kind, delta, (size_t)p.out, (size_t)p.rows, delta_pitch * sizeof(T), PARTS == 1 ? 64 : 128, S::kRows, PARTS == 1);
     if (r) return r;
     p.chunk_steps = S::kChunk;
-    B200_CUDA(cudaFuncSetAttribute(ckpt8_wgrad_tc_kernel<T, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTcSmem));
+    if ((r = allow_shared<ckpt8_wgrad_tc_kernel<T, PARTS>>((int)kTcSmem))) return r;
     Launch((unsigned)w.launch_pairs * 2, kTcThreads, kTcSmem, s).cluster(2)(ckpt8_wgrad_tc_kernel<T, PARTS>, codes_map, delta_map, p);
     B200_LAUNCH_CHECK();
     if (w.splits > 1) {
@@ -736,7 +736,7 @@ int b200_ckpt8_wgrad(float *dweight, float *dbias, int accumulate, const void *d
     if (precision() != B200_FP32) {
         const WgradPlan w = wgrad_plan(wgrad_parts(type), rows, out, in);
         const bool fits = delta_fits(delta, type, delta_pitch);
-        const size_t need = b200_ckpt8_wgrad_workspace(type, rows, out, in, delta, delta_pitch);
+        const size_t need = partial_bytes(w) + (fits ? 0 : (size_t)rows * aligned_pitch(type, out) * type_size(type));
         if (need && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15))) return fail(B200_E_ARG, "the workspace must be given, aligned to 16 bytes");
         if (workspace_bytes < need) return fail(B200_E_NOMEM, "the workspace has %zu bytes, %zu are needed", workspace_bytes, need);
         WgradParams p = {};

@@ -2,6 +2,7 @@
 // scratch arena, and small launch utilities.
 #pragma once
 #include <cuda_runtime.h>
+#include <atomic>
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
@@ -92,6 +93,20 @@ struct Arena {
 int arena_reserve(size_t bytes, cudaStream_t stream);  // make sure cap >= bytes (may synchronise + reallocate)
 void *arena_take(size_t bytes);                        // bump-allocate (256-byte aligned); call after arena_reserve
 void arena_reset();
+
+// Dynamic shared memory above the default, allowed once per kernel and device (the call costs as much as a small launch).
+template <auto KERNEL>
+int allow_shared(int bytes)
+{
+    static std::atomic<unsigned long long> done{0};
+    int d = 0;
+    B200_CUDA(cudaGetDevice(&d));
+    const unsigned long long bit = 1ull << (d & 63);
+    if (done.load(std::memory_order_acquire) & bit) return B200_OK;
+    B200_CUDA(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    done.fetch_or(bit, std::memory_order_release);
+    return B200_OK;
+}
 
 inline size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 inline int ceil_div(int a, int b) { return (a + b - 1) / b; }

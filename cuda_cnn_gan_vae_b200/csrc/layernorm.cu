@@ -108,8 +108,10 @@ struct LnForward {
     const T *x;
     const float *gamma, *beta;
     int rows;
-    size_t n, x_pitch, y_pitch, share;      // share: values of a row per block (a multiple of 32 * V)
+    size_t n, x_pitch, y_pitch;
     float eps;
+    size_t share;                // long rows: values of a row per block (a multiple of V)
+    int groups;                  // and groups of rows
 };
 
 constexpr int kLnValues = 32;       // values of a row in a thread's registers
@@ -134,36 +136,26 @@ __device__ __forceinline__ void ln_put(const LnForward<T> &p, size_t row, size_t
     }
 }
 
-// A row in the registers of one team, or of CLUSTER blocks that hold a share each: read once, written once.  The blocks of a
-// cluster exchange the mean and the squared deviations of their shares through distributed shared memory, one barrier a row.
-template <typename T, int V, int TEAM, int BLOCK, bool CLUSTER>
+// A row in the registers of one team: read once, written once.
+template <typename T, int V, int TEAM, int BLOCK>
 __global__ void __launch_bounds__(BLOCK, 1024 / BLOCK) ln_forward_kernel(const __grid_constant__ LnForward<T> p)
 {
     constexpr int K = kLnValues / V, kTeams = BLOCK / TEAM;
     __shared__ float scratch[kTeams][TEAM / 32];
-    __shared__ float2 shares[2][8];
     grid_dependency_wait();
-    const int t = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
-    unsigned rank = 0, ranks = 1;
-    if constexpr (CLUSTER) { rank = cg::this_cluster().block_rank(); ranks = cg::this_cluster().num_blocks(); }
-    const size_t begin = CLUSTER ? (size_t)rank * p.share : 0;
-    const size_t end = CLUSTER ? min(begin + p.share, p.n) : p.n;
-    const float mine = CLUSTER ? (float)(begin < end ? end - begin : 0) : (float)p.n;
-    const int step = CLUSTER ? (int)(gridDim.x / ranks) : (int)gridDim.x * kTeams;
-    int turn = 0;
-    for (int row = CLUSTER ? (int)(blockIdx.x / ranks) : (int)blockIdx.x * kTeams + team; row < p.rows; row += step, turn ^= 1) {
+    const int t = threadIdx.x % TEAM, team = threadIdx.x / TEAM, n = (int)p.n;
+    for (int row = (int)blockIdx.x * kTeams + team; row < p.rows; row += (int)gridDim.x * kTeams) {
         const T *x = p.x + (size_t)row * p.x_pitch;
         float v[K][V];
 #pragma unroll
         for (int k = 0; k < K; k++) {
-            const size_t col = begin + (size_t)(k * TEAM + t) * V;
-            if (col < end) {
+            const int col = (k * TEAM + t) * V;
+#pragma unroll
+            for (int j = 0; j < V; j++) v[k][j] = 0.f;
+            if (col < n) {
                 const Pack<T, V> in = load_pack<T, V>(x + col);
 #pragma unroll
                 for (int j = 0; j < V; j++) v[k][j] = to_float(in.v[j]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < V; j++) v[k][j] = 0.f;
             }
         }
         float s = 0.f, q = 0.f;
@@ -172,117 +164,155 @@ __global__ void __launch_bounds__(BLOCK, 1024 / BLOCK) ln_forward_kernel(const _
 #pragma unroll
             for (int j = 0; j < V; j++) s += v[k][j];
         }
-        s = team_total<TEAM>(s, scratch[team], 1 + team);
-        float mu = s / (CLUSTER ? fmaxf(mine, 1.f) : mine);
+        const float mu = team_total<TEAM>(s, scratch[team], 1 + team) / (float)n;
 #pragma unroll
         for (int k = 0; k < K; k++) {
-            const size_t col = begin + (size_t)(k * TEAM + t) * V;
-            if (col < end) {
+            if ((k * TEAM + t) * V < n) {
 #pragma unroll
                 for (int j = 0; j < V; j++) { const float d = v[k][j] - mu; q = fmaf(d, d, q); }
             }
         }
-        q = team_total<TEAM>(q, scratch[team], 1 + team);
-        if constexpr (CLUSTER) {
-            // deviations about the mean of all: those about the share's own mean, and its distance
-            cg::cluster_group cluster = cg::this_cluster();
-            if (threadIdx.x < ranks) *cluster.map_shared_rank(&shares[turn][rank], threadIdx.x) = make_float2(mu, q);
-            cluster.sync();
-            float total = 0.f;
-            for (unsigned k = 0; k < ranks; k++) {
-                const size_t at = k * p.share;
-                total += shares[turn][k].x * (float)(at < p.n ? min(p.share, p.n - at) : 0);
-            }
-            mu = total / (float)p.n;
-            q = 0.f;
-            for (unsigned k = 0; k < ranks; k++) {
-                const size_t at = k * p.share;
-                const float d = shares[turn][k].x - mu;
-                q += shares[turn][k].y + d * d * (float)(at < p.n ? min(p.share, p.n - at) : 0);
-            }
-        }
-        const float r = 1.0f / sqrtf(q / (float)p.n + p.eps);
-        if (t == 0 && rank == 0) {
+        const float r = 1.0f / sqrtf(team_total<TEAM>(q, scratch[team], 1 + team) / (float)n + p.eps);
+        if (t == 0) {
             if (p.mean) p.mean[row] = mu;
             if (p.rstd) p.rstd[row] = r;
         }
 #pragma unroll
         for (int k = 0; k < K; k++) {
-            const size_t first = begin + (size_t)(k * TEAM + (t & ~31)) * V;       // of the warp
-            if (first >= end) break;
-            const size_t col = begin + (size_t)(k * TEAM + t) * V;
+            if ((k * TEAM + (t & ~31)) * V >= n) break;     // whole warps: their lanes share blocks of the checkpoint
+            const int col = (k * TEAM + t) * V;
             float xh[V];
 #pragma unroll
-            for (int j = 0; j < V; j++) xh[j] = col < end ? (v[k][j] - mu) * r : 0.f;
+            for (int j = 0; j < V; j++) xh[j] = col < n ? (v[k][j] - mu) * r : 0.f;
             ln_put<T, V>(p, row, col, xh);
         }
     }
 }
 
-// Longer rows: a cluster per row that reads its share three times (from L2 the second and third time).
-template <typename T, int V>
-__global__ void __launch_bounds__(512) ln_forward_long_kernel(const __grid_constant__ LnForward<T> p)
+// Rows that no block holds in two kernels: the statistics, then the values, read a second time (from L2 where the tensor fits there).
+// In one kernel, a cluster of eight blocks on a row, every block reads its share of gamma and beta for every row, which is twice
+// the row itself in fp32: 55 us for 128 rows of 131072 values with a checkpoint.  Here a thread of the second kernel keeps those of
+// its columns and walks down the rows.
+//
+// Statistics are joined pair by pair: values a of mean m_a and squared deviations q_a with values b give
+// m = m_a + d b / (a + b), q = q_a + q_b + d^2 a b / (a + b), d = m_b - m_a.
+struct Moments { float count, mean, q; };
+__device__ __forceinline__ Moments join(Moments a, Moments b)
 {
-    __shared__ float scratch[16];
-    __shared__ float2 shares[2][8];
+    const float count = a.count + b.count, part = count > 0.f ? b.count / count : 0.f, d = b.mean - a.mean;
+    return {count, fmaf(d, part, a.mean), a.q + b.q + d * d * a.count * part};
+}
+__device__ __forceinline__ Moments warp_join(Moments m)
+{
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const Moments other = {__shfl_xor_sync(0xffffffffu, m.count, o), __shfl_xor_sync(0xffffffffu, m.mean, o), __shfl_xor_sync(0xffffffffu, m.q, o)};
+        m = join(m, other);
+    }
+    return m;
+}
+
+constexpr int kLnShares = 8;        // blocks of a cluster
+template <typename T, int V>
+__global__ void __launch_bounds__(512, 2) ln_statistics_kernel(const __grid_constant__ LnForward<T> p)
+{
+    constexpr int U = kLnValues / V;
+    __shared__ Moments warps[16], shares[kLnShares];
     grid_dependency_wait();
     cg::cluster_group cluster = cg::this_cluster();
-    const unsigned rank = cluster.block_rank(), ranks = cluster.num_blocks();
+    const unsigned rank = cluster.block_rank();
+    const int row = (int)(blockIdx.x / kLnShares), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const size_t begin = rank * p.share, end = min(begin + p.share, p.n);
-    const float mine = (float)(begin < p.n ? end - begin : 0);
-    const int step = (int)(gridDim.x / ranks);
-    constexpr int U = 4;
-    int turn = 0;
-    for (int row = (int)(blockIdx.x / ranks); row < p.rows; row += step, turn ^= 1) {
-        const T *x = p.x + (size_t)row * p.x_pitch;
-        auto total = [&](auto f) {
-            float s[U] = {};
-            for (size_t base = begin; base < end; base += 512 * V * U) {
+    const T *x = p.x + (size_t)row * p.x_pitch;
+    Moments m = {0.f, 0.f, 0.f};
+    for (size_t base = begin; base < end; base += 512 * V * U) {
+        float v[U][V], s = 0.f, q = 0.f, count = 0.f;
 #pragma unroll
-                for (int u = 0; u < U; u++) {
-                    const size_t col = base + (size_t)(u * 512 + threadIdx.x) * V;
-                    if (col < end) {
-                        const Pack<T, V> in = load_pack<T, V>(x + col);
-#pragma unroll
-                        for (int j = 0; j < V; j++) s[u] += f(to_float(in.v[j]));
-                    }
-                }
-            }
-            return team_total<512>((s[0] + s[1]) + (s[2] + s[3]), scratch, 1);
-        };
-        float mu = total([](float v) { return v; }) / fmaxf(mine, 1.f);
-        float q = total([&](float v) { const float d = v - mu; return d * d; });
-        if (threadIdx.x < ranks) *cluster.map_shared_rank(&shares[turn][rank], threadIdx.x) = make_float2(mu, q);
-        cluster.sync();
-        float sum = 0.f;
-        for (unsigned k = 0; k < ranks; k++) {
-            const size_t at = k * p.share;
-            sum += shares[turn][k].x * (float)(at < p.n ? min(p.share, p.n - at) : 0);
-        }
-        mu = sum / (float)p.n;
-        q = 0.f;
-        for (unsigned k = 0; k < ranks; k++) {
-            const size_t at = k * p.share;
-            const float d = shares[turn][k].x - mu;
-            q += shares[turn][k].y + d * d * (float)(at < p.n ? min(p.share, p.n - at) : 0);
-        }
-        const float r = 1.0f / sqrtf(q / (float)p.n + p.eps);
-        if (threadIdx.x == 0 && rank == 0) {
-            if (p.mean) p.mean[row] = mu;
-            if (p.rstd) p.rstd[row] = r;
-        }
-        for (size_t base = begin + (threadIdx.x & ~31u) * V; base < end; base += 512 * V) {      // whole warps: they share blocks
-            const size_t col = base + (threadIdx.x & 31) * V;
-            float xh[V];
+        for (int u = 0; u < U; u++) {
+            const size_t col = base + (size_t)(u * 512 + threadIdx.x) * V;
             if (col < end) {
                 const Pack<T, V> in = load_pack<T, V>(x + col);
 #pragma unroll
-                for (int j = 0; j < V; j++) xh[j] = (to_float(in.v[j]) - mu) * r;
-            } else {
-#pragma unroll
-                for (int j = 0; j < V; j++) xh[j] = 0.f;
+                for (int j = 0; j < V; j++) v[u][j] = to_float(in.v[j]);
             }
-            ln_put<T, V>(p, row, col, xh);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (base + (size_t)(u * 512 + threadIdx.x) * V < end) {
+                count += (float)V;
+#pragma unroll
+                for (int j = 0; j < V; j++) s += v[u][j];
+            }
+        }
+        const float mu = s / fmaxf(count, 1.f);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (base + (size_t)(u * 512 + threadIdx.x) * V < end) {
+#pragma unroll
+                for (int j = 0; j < V; j++) { const float d = v[u][j] - mu; q = fmaf(d, d, q); }
+            }
+        }
+        m = join(m, {count, mu, q});
+    }
+    m = warp_join(m);
+    if (lane == 0) warps[warp] = m;
+    __syncthreads();
+    if (warp == 0) {
+        m = warp_join(lane < 16 ? warps[lane] : Moments{0.f, 0.f, 0.f});
+        if (lane == 0) *cluster.map_shared_rank(&shares[rank], 0) = m;
+    }
+    cluster.sync();
+    if (rank == 0 && threadIdx.x == 0) {
+        m = shares[0];
+#pragma unroll
+        for (int k = 1; k < kLnShares; k++) m = join(m, shares[k]);
+        p.mean[row] = m.mean;
+        p.rstd[row] = 1.0f / sqrtf(m.q / (float)p.n + p.eps);
+    }
+}
+
+constexpr int kLnSlice = 128;       // threads on a slice of columns, V each
+template <typename T, int V>
+__global__ void __launch_bounds__(kLnSlice) ln_normalise_kernel(const __grid_constant__ LnForward<T> p)
+{
+    constexpr int U = 4;
+    grid_dependency_wait();
+    const size_t first = ((size_t)blockIdx.x * kLnSlice + (threadIdx.x & ~31)) * V, col = first + (threadIdx.x & 31) * V;
+    if (first >= p.n) return;                                // whole warps: their lanes share blocks of the checkpoint
+    const bool in = col < p.n;
+    float gamma[V], beta[V];
+#pragma unroll
+    for (int j = 0; j < V; j++) { gamma[j] = in ? __ldg(p.gamma + col + j) : 0.f; beta[j] = in ? __ldg(p.beta + col + j) : 0.f; }
+    const size_t blocks = ckpt8_blocks(p.n);
+    const int begin = (int)((long long)p.rows * blockIdx.y / p.groups), end = (int)((long long)p.rows * (blockIdx.y + 1) / p.groups);
+    for (int row = begin; row < end; row += U) {
+        Pack<T, V> raw[U];
+        float mu[U], r[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (row + u >= end) break;
+            if (in) raw[u] = load_pack<T, V>(p.x + (size_t)(row + u) * p.x_pitch + col);
+            mu[u] = p.mean[row + u];
+            r[u] = p.rstd[row + u];
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (row + u >= end) break;
+            float xh[V], y[V];
+#pragma unroll
+            for (int j = 0; j < V; j++) xh[j] = in ? (to_float(raw[u].v[j]) - mu[u]) * r[u] : 0.f;
+            if (p.codes) {
+                const uint32_t b = ckpt8_exponent(ckpt8_top<V>(xh));
+                if (col < blocks * kCkptBlock) {
+                    ckpt8_put<V>(p.codes + (size_t)(row + u) * blocks * kCkptBlock + col, xh, b, false);
+                    if (col % kCkptBlock == 0) p.exponents[(size_t)(row + u) * blocks + col / kCkptBlock] = (uint8_t)b;
+                }
+            }
+            if (in) {
+#pragma unroll
+                for (int j = 0; j < V; j++) y[j] = fmaf(xh[j], gamma[j], beta[j]);
+                store_pack<T, V>(p.y + (size_t)(row + u) * p.y_pitch + col, y);
+            }
         }
     }
 }
@@ -290,22 +320,32 @@ __global__ void __launch_bounds__(512) ln_forward_long_kernel(const __grid_const
 template <typename T, int V>
 static int ln_forward_launch(LnForward<T> p, cudaStream_t s)
 {
-    constexpr size_t kBlockRow = 512 * kLnValues;
-    if (p.n <= kBlockRow) {
+    if (p.n <= 512 * kLnValues) {
         // teams of one, four or sixteen warps: 1024, 4096 or 16384 values
         const int teams = p.n <= 32 * kLnValues ? 4 : 1;
         const Launch launch((unsigned)min((p.rows + teams - 1) / teams, sm_count() * 16), p.n <= 128 * kLnValues ? 128 : 512, 0, s);
-        if (p.n <= 32 * kLnValues) launch(ln_forward_kernel<T, V, 32, 128, false>, p);
-        else if (p.n <= 128 * kLnValues) launch(ln_forward_kernel<T, V, 128, 128, false>, p);
-        else launch(ln_forward_kernel<T, V, 512, 512, false>, p);
-    } else {
-        const int ranks = p.n <= 2 * kBlockRow ? 2 : p.n <= 4 * kBlockRow ? 4 : 8;
-        p.share = align_up((p.n + ranks - 1) / ranks, 32 * V);
-        Launch launch((unsigned)(min(p.rows, sm_count() * 2) * ranks), 512, 0, s);
-        launch.cluster((unsigned)ranks);
-        if (p.n <= 8 * kBlockRow) launch(ln_forward_kernel<T, V, 512, 512, true>, p);
-        else launch(ln_forward_long_kernel<T, V>, p);
+        if (p.n <= 32 * kLnValues) launch(ln_forward_kernel<T, V, 32, 128>, p);
+        else if (p.n <= 128 * kLnValues) launch(ln_forward_kernel<T, V, 128, 128>, p);
+        else launch(ln_forward_kernel<T, V, 512, 512>, p);
+        B200_LAUNCH_CHECK();
+        return B200_OK;
     }
+    if (!p.mean || !p.rstd) return fail(B200_E_ARG, "rows of more than %d values need mean and rstd", 512 * kLnValues);
+    p.share = align_up((p.n + kLnShares - 1) / kLnShares, V);
+    const int most = 0x7fffffff / kLnShares;
+    for (int row = 0; row < p.rows; row += most) {           // a cluster per row
+        LnForward<T> part = p;
+        part.x += (size_t)row * p.x_pitch;
+        part.mean += row;
+        part.rstd += row;
+        part.rows = min(most, p.rows - row);
+        Launch(dim3((unsigned)part.rows * kLnShares), 512, 0, s).cluster(kLnShares)(ln_statistics_kernel<T, V>, part);
+        B200_LAUNCH_CHECK();
+    }
+    // about sixteen blocks of 128 threads per SM, and four rows each at least
+    const long long slices = (long long)((p.n + (size_t)kLnSlice * V - 1) / ((size_t)kLnSlice * V));
+    p.groups = (int)max(1ll, min((long long)(p.rows + 3) / 4, min(65535ll, ((long long)sm_count() * 16 + slices - 1) / slices)));
+    Launch(dim3((unsigned)slices, (unsigned)p.groups), kLnSlice, 0, s)(ln_normalise_kernel<T, V>, p);
     B200_LAUNCH_CHECK();
     return B200_OK;
 }
@@ -608,7 +648,6 @@ __global__ void __launch_bounds__(kLnBlock, 1) ln_backward_rows_kernel(const __g
 
 // Longer rows in two passes.  First: a thread owns V columns and walks a group of rows; it sums dgamma and dbeta of its columns, and
 // its warp writes the partial sums of g and g xh of each row.  Second: a block joins a row's partial sums and forms a piece of dx.
-constexpr int kLnSlice = 128;
 template <typename T, int V>
 __global__ void __launch_bounds__(kLnSlice) ln_backward_columns_kernel(const __grid_constant__ LnBackward<T> p)
 {
@@ -753,7 +792,7 @@ static int ln_backward_launch(LnBackward<T> p, float *dgamma, float *dbeta, int 
         const uint32_t smem = max((uint32_t)(teams * p.depth) * (p.dy_bytes + p.x_bytes), w.team < kLnBlock ? 32768u : 0u);
 #define B200_LN_ROWS(TEAM)                                                                                                                           \
     do {                                                                                                                                             \
-        B200_CUDA(cudaFuncSetAttribute(ln_backward_rows_kernel<T, V, TEAM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kLnRing));             \
+        if ((r = allow_shared<ln_backward_rows_kernel<T, V, TEAM>>((int)kLnRing))) return r;                                                         \
         Launch((unsigned)w.groups, kLnBlock, smem, s)(ln_backward_rows_kernel<T, V, TEAM>, p);                                                       \
     } while (0)
         switch (w.team) {
@@ -801,7 +840,7 @@ int b200_ln_forward(void *y, float *mean, float *rstd, int8_t *codes, uint8_t *e
     const bool wide = wide_rows(x, type, n, x_pitch) && wide_rows(y, type, n, y_pitch);
 #define B200_LN_FWD(T)                                                                                                                               \
     do {                                                                                                                                             \
-        const LnForward<T> p = {(T *)y, mean, rstd, codes, exponents, (const T *)x, gamma, beta, rows, n, x_pitch, y_pitch, 0, eps};                 \
+        const LnForward<T> p = {(T *)y, mean, rstd, codes, exponents, (const T *)x, gamma, beta, rows, n, x_pitch, y_pitch, eps, 0, 0};              \
         return wide ? ln_forward_launch<T, kWide<T>>(p, ST(stream)) : ln_forward_launch<T, 1>(p, ST(stream));                                        \
     } while (0)
     if (type == B200_F32) B200_LN_FWD(float);

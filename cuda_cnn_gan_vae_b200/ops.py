@@ -101,12 +101,12 @@ def _rows(x, name="tensor"):
 
 def _param(x, n, name):
     """A contiguous fp32 tensor of n elements on the current device."""
+    if isinstance(x, torch.Tensor) and x.dtype == torch.float32 and x.numel() == n and x.get_device() == _device() and x.is_contiguous():
+        return x
     _t(x, name)
     if x.numel() != n:
         raise B200Error(1, f"{name} must have {n} elements")
-    if x.get_device() != _device():
-        raise B200Error(2, f"{name} is on {x.device}, the current device is cuda:{_device()}")
-    return x
+    raise B200Error(2, f"{name} is on {x.device}, the current device is cuda:{_device()}")
 
 
 def _like(x, name, want, other):
@@ -515,11 +515,11 @@ def bn_backward(dy, xhat, ivar, gamma, dgamma, dbeta, create_delta_weight=True):
     return dx
 
 
-def _workspace(size, given, name):
+def _workspace(size, given, name, like):
     """The caller's workspace tensor, or a fresh one from torch's allocator (which orders its reuse by stream and keeps the
-    workspaces of captured graphs apart)."""
+    workspaces of captured graphs apart); `like`: an fp32 tensor on the current device."""
     if given is None:
-        return torch.empty(max(size, 16), dtype=torch.uint8, device="cuda"), max(size, 16)
+        return (like.new_empty((size + 3) // 4), size) if size else (None, 0)
     if not (isinstance(given, torch.Tensor) and given.is_cuda and given.is_contiguous() and given.get_device() == _device()):
         raise B200Error(2, f"{name}: the workspace must be a contiguous tensor on the current device")
     return given, given.numel() * given.element_size()
@@ -566,10 +566,10 @@ def ln_backward(dy, x, mean, rstd, gamma, dgamma, dbeta, create_delta_weight=Tru
     dg = db = None
     if create_delta_weight:
         dg, db = _param(dgamma, n, "dgamma").data_ptr(), _param(dbeta, n, "dbeta").data_ptr()
-    workspace, size = _workspace(load().b200_ln_backward_workspace(rows, n), workspace, "ln_backward")
+    workspace, size = _workspace(load().b200_ln_backward_workspace(rows, n), workspace, "ln_backward", gamma)
     _check(load().b200_ln_backward(dx.data_ptr(), dg, db, dy.data_ptr(), x_ptr, mean_ptr, rstd.data_ptr(), codes, exponents, gamma.data_ptr(),
                                    kind, rows, n, dx_pitch, dy_pitch, x_pitch, int(create_delta_weight), int(accumulate),
-                                   workspace.data_ptr(), size, _stream_id()))
+                                   workspace.data_ptr() if workspace is not None else None, size, _stream_id()))
     return dx
 
 
@@ -582,10 +582,10 @@ def checkpoint_wgrad(dweight, dbias, delta, checkpoint, accumulate=True, workspa
     _param(dweight, out * checkpoint.n, "dweight")
     if dbias is not None:
         _param(dbias, out, "dbias")
-    workspace, size = _workspace(load().b200_ckpt8_wgrad_workspace(kind, rows, out, checkpoint.n, delta.data_ptr(), pitch), workspace, "checkpoint_wgrad")
+    workspace, size = _workspace(load().b200_ckpt8_wgrad_workspace(kind, rows, out, checkpoint.n, delta.data_ptr(), pitch), workspace, "checkpoint_wgrad", dweight)
     _check(load().b200_ckpt8_wgrad(dweight.data_ptr(), dbias.data_ptr() if dbias is not None else None, int(accumulate), delta.data_ptr(),
                                    checkpoint.codes.data_ptr(), checkpoint.exponents.data_ptr(), kind, rows, out, checkpoint.n, pitch,
-                                   workspace.data_ptr(), size, _stream_id()))
+                                   workspace.data_ptr() if workspace is not None else None, size, _stream_id()))
 
 
 def vae_forward(mu, logvar, eps, want_kl=True):

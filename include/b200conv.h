@@ -337,7 +337,7 @@ enum { B200_F32 = 0, B200_BF16 = 1, B200_F16 = 2 };
  * captured graphs are independent as long as their workspaces are. */
 
 /* Layer normalisation of every row over its n values: y = gamma * xhat + beta, xhat = (x - mean) * rstd,
- * rstd = 1 / sqrt(variance + eps), the variance being the row's own (divided by n).  mean and rstd [rows] may be NULL.  codes
+ * rstd = 1 / sqrt(variance + eps), the variance being the row's own (divided by n).  mean and rstd [rows] may be NULL where n <= 16384.  codes
  * and exponents (both or neither): xhat is kept as an 8-bit checkpoint for b200_ln_backward.  y may be x. */
 int b200_ln_forward(void *y, float *mean, float *rstd, int8_t *codes, uint8_t *exponents, const void *x, const float *gamma,
                     const float *beta, int type, int rows, size_t n, size_t x_pitch, size_t y_pitch, float eps, void *stream);
