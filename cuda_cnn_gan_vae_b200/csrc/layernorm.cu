@@ -97,6 +97,25 @@ __device__ __forceinline__ float2 team_totals(float2 v, float2 *scratch, int id)
     return v;
 }
 
+// V parameters from column `col` on (a multiple of V); wide: they start at a 16-byte boundary
+template <int V>
+__device__ __forceinline__ void load_params(float *f, const float *p, size_t col, bool wide)
+{
+    if constexpr (V >= 4) {
+        if (wide) {
+#pragma unroll
+            for (int i = 0; i < V / 4; i++) {
+                const float4 v = __ldg(reinterpret_cast<const float4 *>(p + col) + i);
+                f[4 * i] = v.x; f[4 * i + 1] = v.y; f[4 * i + 2] = v.z; f[4 * i + 3] = v.w;
+            }
+            return;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < V; i++) f[i] = __ldg(p + col + i);
+}
+inline bool wide_params(const void *a, const void *b) { return !((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15); }
+
 // ---- forward -----------------------------------------------------------------------------------------------------------------
 
 template <typename T>
@@ -110,11 +129,10 @@ struct LnForward {
     int rows;
     size_t n, x_pitch, y_pitch;
     float eps;
+    int wide;                    // gamma and beta can be read in 16-byte pieces
     size_t share;                // long rows: values of a row per block (a multiple of V)
     int groups;                  // and groups of rows
 };
-
-constexpr int kLnValues = 32;       // values of a row in a thread's registers
 
 // writes V normalised values and keeps them; col < n may be false for lanes that fill up a block of the checkpoint
 template <typename T, int V>
@@ -129,18 +147,20 @@ __device__ __forceinline__ void ln_put(const LnForward<T> &p, size_t row, size_t
         }
     }
     if (col < p.n) {
-        float y[V];
+        float y[V], gamma[V], beta[V];
+        load_params<V>(gamma, p.gamma, col, p.wide);
+        load_params<V>(beta, p.beta, col, p.wide);
 #pragma unroll
-        for (int j = 0; j < V; j++) y[j] = fmaf(xh[j], __ldg(p.gamma + col + j), __ldg(p.beta + col + j));
+        for (int j = 0; j < V; j++) y[j] = fmaf(xh[j], gamma[j], beta[j]);
         store_pack<T, V>(p.y + row * p.y_pitch + col, y);
     }
 }
 
 // A row in the registers of one team: read once, written once.
-template <typename T, int V, int TEAM, int BLOCK>
-__global__ void __launch_bounds__(BLOCK, 1024 / BLOCK) ln_forward_kernel(const __grid_constant__ LnForward<T> p)
+template <typename T, int V, int VALUES, int TEAM, int BLOCK>
+__global__ void __launch_bounds__(BLOCK, (VALUES <= 16 ? 1536 : 1024) / BLOCK) ln_forward_kernel(const __grid_constant__ LnForward<T> p)
 {
-    constexpr int K = kLnValues / V, kTeams = BLOCK / TEAM;
+    constexpr int K = VALUES / V, kTeams = BLOCK / TEAM;
     __shared__ float scratch[kTeams][TEAM / 32];
     grid_dependency_wait();
     const int t = threadIdx.x % TEAM, team = threadIdx.x / TEAM, n = (int)p.n;
@@ -190,7 +210,7 @@ __global__ void __launch_bounds__(BLOCK, 1024 / BLOCK) ln_forward_kernel(const _
 }
 
 // Rows that no block holds in two kernels: the statistics, then the values, read a second time (from L2 where the tensor fits there).
-// In one kernel, a cluster of eight blocks on a row, every block reads its share of gamma and beta for every row, which is twice
+// In one kernel, a cluster of blocks on a row, every block reads its share of gamma and beta for every row, which is twice
 // the row itself in fp32: 55 us for 128 rows of 131072 values with a checkpoint.  Here a thread of the second kernel keeps those of
 // its columns and walks down the rows.
 //
@@ -212,12 +232,12 @@ __device__ __forceinline__ Moments warp_join(Moments m)
     return m;
 }
 
-constexpr int kLnShares = 8;        // blocks of a cluster
+constexpr int kLnShares = 4;        // blocks of a cluster (four of 256 threads: 50 us for the case above, eight of 512: 56)
 template <typename T, int V>
-__global__ void __launch_bounds__(512, 2) ln_statistics_kernel(const __grid_constant__ LnForward<T> p)
+__global__ void __launch_bounds__(256, 4) ln_statistics_kernel(const __grid_constant__ LnForward<T> p)
 {
-    constexpr int U = kLnValues / V;
-    __shared__ Moments warps[16], shares[kLnShares];
+    constexpr int U = 32 / V;
+    __shared__ Moments warps[8], shares[kLnShares];
     grid_dependency_wait();
     cg::cluster_group cluster = cg::this_cluster();
     const unsigned rank = cluster.block_rank();
@@ -225,11 +245,11 @@ __global__ void __launch_bounds__(512, 2) ln_statistics_kernel(const __grid_cons
     const size_t begin = rank * p.share, end = min(begin + p.share, p.n);
     const T *x = p.x + (size_t)row * p.x_pitch;
     Moments m = {0.f, 0.f, 0.f};
-    for (size_t base = begin; base < end; base += 512 * V * U) {
+    for (size_t base = begin; base < end; base += 256 * V * U) {
         float v[U][V], s = 0.f, q = 0.f, count = 0.f;
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const size_t col = base + (size_t)(u * 512 + threadIdx.x) * V;
+            const size_t col = base + (size_t)(u * 256 + threadIdx.x) * V;
             if (col < end) {
                 const Pack<T, V> in = load_pack<T, V>(x + col);
 #pragma unroll
@@ -238,7 +258,7 @@ __global__ void __launch_bounds__(512, 2) ln_statistics_kernel(const __grid_cons
         }
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            if (base + (size_t)(u * 512 + threadIdx.x) * V < end) {
+            if (base + (size_t)(u * 256 + threadIdx.x) * V < end) {
                 count += (float)V;
 #pragma unroll
                 for (int j = 0; j < V; j++) s += v[u][j];
@@ -247,7 +267,7 @@ __global__ void __launch_bounds__(512, 2) ln_statistics_kernel(const __grid_cons
         const float mu = s / fmaxf(count, 1.f);
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            if (base + (size_t)(u * 512 + threadIdx.x) * V < end) {
+            if (base + (size_t)(u * 256 + threadIdx.x) * V < end) {
 #pragma unroll
                 for (int j = 0; j < V; j++) { const float d = v[u][j] - mu; q = fmaf(d, d, q); }
             }
@@ -258,7 +278,7 @@ __global__ void __launch_bounds__(512, 2) ln_statistics_kernel(const __grid_cons
     if (lane == 0) warps[warp] = m;
     __syncthreads();
     if (warp == 0) {
-        m = warp_join(lane < 16 ? warps[lane] : Moments{0.f, 0.f, 0.f});
+        m = warp_join(lane < 8 ? warps[lane] : Moments{0.f, 0.f, 0.f});
         if (lane == 0) *cluster.map_shared_rank(&shares[rank], 0) = m;
     }
     cluster.sync();
@@ -282,7 +302,11 @@ __global__ void __launch_bounds__(kLnSlice) ln_normalise_kernel(const __grid_con
     const bool in = col < p.n;
     float gamma[V], beta[V];
 #pragma unroll
-    for (int j = 0; j < V; j++) { gamma[j] = in ? __ldg(p.gamma + col + j) : 0.f; beta[j] = in ? __ldg(p.beta + col + j) : 0.f; }
+    for (int j = 0; j < V; j++) gamma[j] = beta[j] = 0.f;
+    if (in) {
+        load_params<V>(gamma, p.gamma, col, p.wide);
+        load_params<V>(beta, p.beta, col, p.wide);
+    }
     const size_t blocks = ckpt8_blocks(p.n);
     const int begin = (int)((long long)p.rows * blockIdx.y / p.groups), end = (int)((long long)p.rows * (blockIdx.y + 1) / p.groups);
     for (int row = begin; row < end; row += U) {
@@ -317,20 +341,22 @@ __global__ void __launch_bounds__(kLnSlice) ln_normalise_kernel(const __grid_con
     }
 }
 
+constexpr size_t kLnHeld = 16384;   // values of the longest row that a block holds
 template <typename T, int V>
 static int ln_forward_launch(LnForward<T> p, cudaStream_t s)
 {
-    if (p.n <= 512 * kLnValues) {
-        // teams of one, four or sixteen warps: 1024, 4096 or 16384 values
-        const int teams = p.n <= 32 * kLnValues ? 4 : 1;
-        const Launch launch((unsigned)min((p.rows + teams - 1) / teams, sm_count() * 16), p.n <= 128 * kLnValues ? 128 : 512, 0, s);
-        if (p.n <= 32 * kLnValues) launch(ln_forward_kernel<T, V, 32, 128>, p);
-        else if (p.n <= 128 * kLnValues) launch(ln_forward_kernel<T, V, 128, 128>, p);
-        else launch(ln_forward_kernel<T, V, 512, 512>, p);
+    if (p.n <= kLnHeld) {
+        // teams of one, four or sixteen warps with 16 values a thread (more rows under way on an SM than with 32), or 32
+        const int teams = p.n <= 512 ? 4 : 1;
+        const Launch launch((unsigned)min((p.rows + teams - 1) / teams, sm_count() * 24), p.n <= 2048 ? 128 : 512, 0, s);
+        if (p.n <= 512) launch(ln_forward_kernel<T, V, 16, 32, 128>, p);
+        else if (p.n <= 2048) launch(ln_forward_kernel<T, V, 16, 128, 128>, p);
+        else if (p.n <= 8192) launch(ln_forward_kernel<T, V, 16, 512, 512>, p);
+        else launch(ln_forward_kernel<T, V, 32, 512, 512>, p);
         B200_LAUNCH_CHECK();
         return B200_OK;
     }
-    if (!p.mean || !p.rstd) return fail(B200_E_ARG, "rows of more than %d values need mean and rstd", 512 * kLnValues);
+    if (!p.mean || !p.rstd) return fail(B200_E_ARG, "rows of more than %zu values need mean and rstd", kLnHeld);
     p.share = align_up((p.n + kLnShares - 1) / kLnShares, V);
     const int most = 0x7fffffff / kLnShares;
     for (int row = 0; row < p.rows; row += most) {           // a cluster per row
@@ -339,7 +365,7 @@ static int ln_forward_launch(LnForward<T> p, cudaStream_t s)
         part.mean += row;
         part.rstd += row;
         part.rows = min(most, p.rows - row);
-        Launch(dim3((unsigned)part.rows * kLnShares), 512, 0, s).cluster(kLnShares)(ln_statistics_kernel<T, V>, part);
+        Launch(dim3((unsigned)part.rows * kLnShares), 256, 0, s).cluster(kLnShares)(ln_statistics_kernel<T, V>, part);
         B200_LAUNCH_CHECK();
     }
     // about sixteen blocks of 128 threads per SM, and four rows each at least
@@ -373,6 +399,7 @@ struct LnBackward {
     unsigned *status;
     float *dgamma, *dbeta;       // written directly where there is one group
     int accumulate;
+    int wide;                    // gamma can be read in 16-byte pieces
 };
 
 // V values of dy and of what xh comes from, as loaded
@@ -648,34 +675,49 @@ __global__ void __launch_bounds__(kLnBlock, 1) ln_backward_rows_kernel(const __g
 
 // Longer rows in two passes.  First: a thread owns V columns and walks a group of rows; it sums dgamma and dbeta of its columns, and
 // its warp writes the partial sums of g and g xh of each row.  Second: a block joins a row's partial sums and forms a piece of dx.
+template <int V> constexpr int kLnRuns = V == 1 ? 4 : 1;      // runs of V columns of a thread, a slice apart
 template <typename T, int V>
 __global__ void __launch_bounds__(kLnSlice) ln_backward_columns_kernel(const __grid_constant__ LnBackward<T> p)
 {
-    constexpr int U = 4;
+    constexpr int C = kLnRuns<V>, U = 4 / C > 0 ? 4 / C : 1;   // rows under way
     grid_dependency_wait();
-    const size_t col = ((size_t)blockIdx.x * kLnSlice + threadIdx.x) * V;
+    const size_t first = ((size_t)blockIdx.x * C * kLnSlice + threadIdx.x) * V;
     const int piece = (int)(blockIdx.x * (kLnSlice / 32) + (threadIdx.x >> 5)), lane = threadIdx.x & 31;
-    const bool in = col < p.n;
-    float gamma[V], dgamma[V], dbeta[V];
+    bool in[C];
+    float gamma[C][V], dgamma[C][V], dbeta[C][V];
 #pragma unroll
-    for (int j = 0; j < V; j++) { gamma[j] = in ? __ldg(p.gamma + col + j) : 0.f; dgamma[j] = dbeta[j] = 0.f; }
+    for (int c = 0; c < C; c++) {
+        const size_t col = first + (size_t)c * kLnSlice * V;
+        in[c] = col < p.n;
+#pragma unroll
+        for (int j = 0; j < V; j++) gamma[c][j] = dgamma[c][j] = dbeta[c][j] = 0.f;
+        if (in[c]) load_params<V>(gamma[c], p.gamma, col, p.wide);
+    }
     const int begin = (int)((long long)p.rows * blockIdx.y / p.groups), end = (int)((long long)p.rows * (blockIdx.y + 1) / p.groups);
+#pragma unroll 2
     for (int row = begin; row < end; row += U) {
-        LnRaw<T, V> raw[U];
+        LnRaw<T, V> raw[U][C];
 #pragma unroll
-        for (int u = 0; u < U; u++)
-            if (in && row + u < end) ln_load<T, V>(p, row + u, col, raw[u]);
+        for (int u = 0; u < U; u++) {
+#pragma unroll
+            for (int c = 0; c < C; c++)
+                if (in[c] && row + u < end) ln_load<T, V>(p, row + u, first + (size_t)c * kLnSlice * V, raw[u][c]);
+        }
 #pragma unroll
         for (int u = 0; u < U; u++) {
             if (row + u >= end) break;
-            float dy[V], xh[V], s1 = 0.f, s2 = 0.f;
-            if (in) {
-                ln_values<T, V>(p, raw[u], p.mean ? p.mean[row + u] : 0.f, p.rstd[row + u], dy, xh);
+            const float mu = p.mean ? p.mean[row + u] : 0.f, r = p.rstd[row + u];
+            float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+                if (!in[c]) continue;
+                float dy[V], xh[V];
+                ln_values<T, V>(p, raw[u][c], mu, r, dy, xh);
 #pragma unroll
                 for (int j = 0; j < V; j++) {
-                    dgamma[j] = fmaf(dy[j], xh[j], dgamma[j]);
-                    dbeta[j] += dy[j];
-                    const float g = dy[j] * gamma[j];
+                    dgamma[c][j] = fmaf(dy[j], xh[j], dgamma[c][j]);
+                    dbeta[c][j] += dy[j];
+                    const float g = dy[j] * gamma[c][j];
                     s1 += g;
                     s2 = fmaf(g, xh[j], s2);
                 }
@@ -684,16 +726,20 @@ __global__ void __launch_bounds__(kLnSlice) ln_backward_columns_kernel(const __g
             if (lane == 0) p.row_part[(size_t)(row + u) * p.pieces + piece] = both;
         }
     }
-    if (!p.weights || !in) return;
-    float *out = p.part + (size_t)blockIdx.y * 2 * p.n + col;
+    if (!p.weights) return;
 #pragma unroll
-    for (int j = 0; j < V; j++) { out[j] = dgamma[j]; out[p.n + j] = dbeta[j]; }
+    for (int c = 0; c < C; c++) {
+        if (!in[c]) continue;
+        float *out = p.part + (size_t)blockIdx.y * 2 * p.n + first + (size_t)c * kLnSlice * V;
+#pragma unroll
+        for (int j = 0; j < V; j++) { out[j] = dgamma[c][j]; out[p.n + j] = dbeta[c][j]; }
+    }
 }
 
 template <typename T, int V>
 __global__ void __launch_bounds__(256) ln_backward_apply_kernel(const __grid_constant__ LnBackward<T> p)
 {
-    constexpr int K = 4;
+    constexpr int K = V == 1 ? 8 : 4;
     __shared__ float2 scratch[2][8];
     grid_dependency_wait();
     int turn = 0;
@@ -713,10 +759,11 @@ __global__ void __launch_bounds__(256) ln_backward_apply_kernel(const __grid_con
         for (int k = 0; k < K; k++) {
             const size_t col = base + (size_t)(k * 256 + threadIdx.x) * V;
             if (col >= p.n) continue;
-            float dy[V], xh[V];
+            float dy[V], xh[V], gamma[V];
             ln_values<T, V>(p, raw[k], mu, r, dy, xh);
+            load_params<V>(gamma, p.gamma, col, p.wide);
 #pragma unroll
-            for (int j = 0; j < V; j++) dy[j] = r * (dy[j] * __ldg(p.gamma + col + j) - c1 - xh[j] * c2);
+            for (int j = 0; j < V; j++) dy[j] = r * (dy[j] * gamma[j] - c1 - xh[j] * c2);
             store_pack<T, V>(p.dx + (size_t)row * p.dx_pitch + col, dy);
         }
     }
@@ -762,7 +809,7 @@ static LnPlan ln_plan(int rows, size_t n, int v)
         const int teams = kLnBlock / w.team;
         w.groups = rows <= 8 * teams ? 1 : min((rows + teams - 1) / teams, sm_count());
     } else {
-        const size_t slices = (n + (size_t)kLnSlice * v - 1) / ((size_t)kLnSlice * v);
+        const size_t slice = (size_t)kLnSlice * (v == 1 ? kLnRuns<1> : kLnRuns<4> * v), slices = (n + slice - 1) / slice;
         w.pieces = (int)slices * (kLnSlice / 32);
         // about sixteen blocks of 128 threads per SM, and eight rows each at least
         const long long want = ((long long)sm_count() * 16 + (long long)slices - 1) / (long long)slices;
@@ -782,6 +829,7 @@ static int ln_backward_launch(LnBackward<T> p, float *dgamma, float *dbeta, int 
     p.dgamma = dgamma;
     p.dbeta = dbeta;
     p.accumulate = accumulate;
+    p.wide = wide_params(p.gamma, p.gamma);
     if (w.one_pass) {
         int r = status_word(&p.status);
         if (r) return r;
@@ -808,7 +856,8 @@ static int ln_backward_launch(LnBackward<T> p, float *dgamma, float *dbeta, int 
     } else {
         Launch(dim3((unsigned)(w.pieces / (kLnSlice / 32)), (unsigned)w.groups), kLnSlice, 0, s)(ln_backward_columns_kernel<T, V>, p);
         B200_LAUNCH_CHECK();
-        Launch(dim3((unsigned)((p.n + 1024 * V - 1) / (1024 * V)), (unsigned)min(p.rows, 65535)), 256, 0, s)(ln_backward_apply_kernel<T, V>, p);
+        constexpr size_t kPiece = 256 * (V == 1 ? 8 : 4 * V);
+        Launch(dim3((unsigned)((p.n + kPiece - 1) / kPiece), (unsigned)min(p.rows, 65535)), 256, 0, s)(ln_backward_apply_kernel<T, V>, p);
         B200_LAUNCH_CHECK();
     }
     if (p.weights) {
@@ -840,7 +889,8 @@ int b200_ln_forward(void *y, float *mean, float *rstd, int8_t *codes, uint8_t *e
     const bool wide = wide_rows(x, type, n, x_pitch) && wide_rows(y, type, n, y_pitch);
 #define B200_LN_FWD(T)                                                                                                                               \
     do {                                                                                                                                             \
-        const LnForward<T> p = {(T *)y, mean, rstd, codes, exponents, (const T *)x, gamma, beta, rows, n, x_pitch, y_pitch, eps, 0, 0};              \
+        const LnForward<T> p = {(T *)y, mean, rstd, codes, exponents, (const T *)x, gamma, beta, rows, n, x_pitch, y_pitch, eps,\
+                                 wide_params(gamma, beta), 0, 0};                                                                                    \
         return wide ? ln_forward_launch<T, kWide<T>>(p, ST(stream)) : ln_forward_launch<T, 1>(p, ST(stream));                                        \
     } while (0)
     if (type == B200_F32) B200_LN_FWD(float);
