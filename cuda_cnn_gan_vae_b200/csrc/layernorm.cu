@@ -134,25 +134,32 @@ struct LnForward {
     int groups;                  // and groups of rows
 };
 
-// writes V normalised values and keeps them; col < n may be false for lanes that fill up a block of the checkpoint
-template <typename T, int V>
-__device__ __forceinline__ void ln_put(const LnForward<T> &p, size_t row, size_t col, const float *xh)
+// writes V normalised values of a row and keeps them; col < n may be false for lanes that fill up a block of the checkpoint
+template <typename T> struct LnOut { T *y; int8_t *codes; uint8_t *exponents; uint32_t padded; };
+template <typename T>
+__device__ __forceinline__ LnOut<T> ln_out(const LnForward<T> &p, int row)
 {
-    if (p.codes) {
+    const size_t blocks = ckpt8_blocks(p.n);
+    return {p.y + (size_t)row * p.y_pitch, p.codes ? p.codes + (size_t)row * blocks * kCkptBlock : nullptr, p.exponents + (size_t)row * blocks,
+            (uint32_t)(blocks * kCkptBlock)};
+}
+template <typename T, int V>
+__device__ __forceinline__ void ln_put(const LnForward<T> &p, const LnOut<T> &out, uint32_t col, const float *xh)
+{
+    if (out.codes) {
         const uint32_t b = ckpt8_exponent(ckpt8_top<V>(xh));
-        const size_t blocks = ckpt8_blocks(p.n);
-        if (col < blocks * kCkptBlock) {
-            ckpt8_put<V>(p.codes + row * blocks * kCkptBlock + col, xh, b, false);
-            if (col % kCkptBlock == 0) p.exponents[row * blocks + col / kCkptBlock] = (uint8_t)b;
+        if (col < out.padded) {
+            ckpt8_put<V>(out.codes + col, xh, b, false);
+            if (col % kCkptBlock == 0) out.exponents[col / kCkptBlock] = (uint8_t)b;
         }
     }
-    if (col < p.n) {
+    if (col < (uint32_t)p.n) {
         float y[V], gamma[V], beta[V];
         load_params<V>(gamma, p.gamma, col, p.wide);
         load_params<V>(beta, p.beta, col, p.wide);
 #pragma unroll
         for (int j = 0; j < V; j++) y[j] = fmaf(xh[j], gamma[j], beta[j]);
-        store_pack<T, V>(p.y + row * p.y_pitch + col, y);
+        store_pack<T, V>(out.y + col, y);
     }
 }
 
@@ -197,6 +204,7 @@ __global__ void __launch_bounds__(BLOCK, (VALUES <= 16 ? 1536 : 1024) / BLOCK) l
             if (p.mean) p.mean[row] = mu;
             if (p.rstd) p.rstd[row] = r;
         }
+        const LnOut<T> out = ln_out(p, row);
 #pragma unroll
         for (int k = 0; k < K; k++) {
             if ((k * TEAM + (t & ~31)) * V >= n) break;     // whole warps: their lanes share blocks of the checkpoint
@@ -204,7 +212,7 @@ __global__ void __launch_bounds__(BLOCK, (VALUES <= 16 ? 1536 : 1024) / BLOCK) l
             float xh[V];
 #pragma unroll
             for (int j = 0; j < V; j++) xh[j] = col < n ? (v[k][j] - mu) * r : 0.f;
-            ln_put<T, V>(p, row, col, xh);
+            ln_put<T, V>(p, out, (uint32_t)col, xh);
         }
     }
 }
@@ -297,9 +305,9 @@ __global__ void __launch_bounds__(kLnSlice) ln_normalise_kernel(const __grid_con
 {
     constexpr int U = 4;
     grid_dependency_wait();
-    const size_t first = ((size_t)blockIdx.x * kLnSlice + (threadIdx.x & ~31)) * V, col = first + (threadIdx.x & 31) * V;
-    if (first >= p.n) return;                                // whole warps: their lanes share blocks of the checkpoint
-    const bool in = col < p.n;
+    const uint32_t n = (uint32_t)p.n, first = (blockIdx.x * kLnSlice + (threadIdx.x & ~31u)) * V, col = first + (threadIdx.x & 31) * V;
+    if (first >= n) return;                                  // whole warps: their lanes share blocks of the checkpoint
+    const bool in = col < n;
     float gamma[V], beta[V];
 #pragma unroll
     for (int j = 0; j < V; j++) gamma[j] = beta[j] = 0.f;
@@ -308,6 +316,7 @@ __global__ void __launch_bounds__(kLnSlice) ln_normalise_kernel(const __grid_con
         load_params<V>(beta, p.beta, col, p.wide);
     }
     const size_t blocks = ckpt8_blocks(p.n);
+    const bool in_block = p.codes && col < blocks * kCkptBlock, opens_block = in_block && col % kCkptBlock == 0;
     const int begin = (int)((long long)p.rows * blockIdx.y / p.groups), end = (int)((long long)p.rows * (blockIdx.y + 1) / p.groups);
     for (int row = begin; row < end; row += U) {
         Pack<T, V> raw[U];
@@ -327,10 +336,8 @@ __global__ void __launch_bounds__(kLnSlice) ln_normalise_kernel(const __grid_con
             for (int j = 0; j < V; j++) xh[j] = in ? (to_float(raw[u].v[j]) - mu[u]) * r[u] : 0.f;
             if (p.codes) {
                 const uint32_t b = ckpt8_exponent(ckpt8_top<V>(xh));
-                if (col < blocks * kCkptBlock) {
-                    ckpt8_put<V>(p.codes + (size_t)(row + u) * blocks * kCkptBlock + col, xh, b, false);
-                    if (col % kCkptBlock == 0) p.exponents[(size_t)(row + u) * blocks + col / kCkptBlock] = (uint8_t)b;
-                }
+                if (in_block) ckpt8_put<V>(p.codes + (size_t)(row + u) * blocks * kCkptBlock + col, xh, b, false);
+                if (opens_block) p.exponents[(size_t)(row + u) * blocks + col / kCkptBlock] = (uint8_t)b;
             }
             if (in) {
 #pragma unroll
@@ -405,15 +412,26 @@ struct LnBackward {
 // V values of dy and of what xh comes from, as loaded
 template <typename T, int V> struct LnRaw { Pack<T, V> dy, x; CkptCodes<V> c; uint32_t e; };
 
-template <typename T, int V>
-__device__ __forceinline__ void ln_load(const LnBackward<T> &p, int row, size_t col, LnRaw<T, V> &in)
+// where a row lies (64-bit address arithmetic once a row instead of once a load)
+template <typename T> struct LnRow { const T *dy, *x; const int8_t *codes; const uint8_t *exponents; };
+template <typename T>
+__device__ __forceinline__ LnRow<T> ln_row(const LnBackward<T> &p, int row)
 {
-    in.dy = load_pack<T, V>(p.dy + (size_t)row * p.dy_pitch + col);
+    LnRow<T> r;
+    r.dy = p.dy + (size_t)row * p.dy_pitch;
+    if (p.codes) { r.codes = p.codes + (size_t)row * p.blocks * kCkptBlock; r.exponents = p.exponents + (size_t)row * p.blocks; }
+    else r.x = p.x + (size_t)row * p.x_pitch;
+    return r;
+}
+template <typename T, int V>
+__device__ __forceinline__ void ln_load(const LnBackward<T> &p, const LnRow<T> &row, uint32_t col, LnRaw<T, V> &in)
+{
+    in.dy = load_pack<T, V>(row.dy + col);
     if (p.codes) {
-        in.c = ckpt8_get<V>(p.codes + (size_t)row * p.blocks * kCkptBlock + col);
-        in.e = p.exponents[(size_t)row * p.blocks + col / kCkptBlock];
+        in.c = ckpt8_get<V>(row.codes + col);
+        in.e = row.exponents[col / kCkptBlock];
     } else {
-        in.x = load_pack<T, V>(p.x + (size_t)row * p.x_pitch + col);
+        in.x = load_pack<T, V>(row.x + col);
     }
 }
 template <typename T, int V>
@@ -681,14 +699,14 @@ __global__ void __launch_bounds__(kLnSlice) ln_backward_columns_kernel(const __g
 {
     constexpr int C = kLnRuns<V>, U = 4 / C > 0 ? 4 / C : 1;   // rows under way
     grid_dependency_wait();
-    const size_t first = ((size_t)blockIdx.x * C * kLnSlice + threadIdx.x) * V;
+    const uint32_t first = (blockIdx.x * C * kLnSlice + threadIdx.x) * V, n = (uint32_t)p.n;
     const int piece = (int)(blockIdx.x * (kLnSlice / 32) + (threadIdx.x >> 5)), lane = threadIdx.x & 31;
     bool in[C];
     float gamma[C][V], dgamma[C][V], dbeta[C][V];
 #pragma unroll
     for (int c = 0; c < C; c++) {
-        const size_t col = first + (size_t)c * kLnSlice * V;
-        in[c] = col < p.n;
+        const uint32_t col = first + c * kLnSlice * V;
+        in[c] = col < n;
 #pragma unroll
         for (int j = 0; j < V; j++) gamma[c][j] = dgamma[c][j] = dbeta[c][j] = 0.f;
         if (in[c]) load_params<V>(gamma[c], p.gamma, col, p.wide);
@@ -699,9 +717,11 @@ __global__ void __launch_bounds__(kLnSlice) ln_backward_columns_kernel(const __g
         LnRaw<T, V> raw[U][C];
 #pragma unroll
         for (int u = 0; u < U; u++) {
+            if (row + u >= end) break;
+            const LnRow<T> at = ln_row(p, row + u);
 #pragma unroll
             for (int c = 0; c < C; c++)
-                if (in[c] && row + u < end) ln_load<T, V>(p, row + u, first + (size_t)c * kLnSlice * V, raw[u][c]);
+                if (in[c]) ln_load<T, V>(p, at, first + c * kLnSlice * V, raw[u][c]);
         }
 #pragma unroll
         for (int u = 0; u < U; u++) {
@@ -743,28 +763,29 @@ __global__ void __launch_bounds__(256) ln_backward_apply_kernel(const __grid_con
     __shared__ float2 scratch[2][8];
     grid_dependency_wait();
     int turn = 0;
+    const uint32_t first = (blockIdx.x * 256 * K + threadIdx.x) * V, n = (uint32_t)p.n;
     for (int row = blockIdx.y; row < p.rows; row += gridDim.y, turn ^= 1) {
         LnRaw<T, V> raw[K];
-        const size_t base = (size_t)blockIdx.x * 256 * K * V;
+        const LnRow<T> at = ln_row(p, row);
 #pragma unroll
-        for (int k = 0; k < K; k++) {
-            const size_t col = base + (size_t)(k * 256 + threadIdx.x) * V;
-            if (col < p.n) ln_load<T, V>(p, row, col, raw[k]);
-        }
+        for (int k = 0; k < K; k++)
+            if (first + k * 256 * V < n) ln_load<T, V>(p, at, first + k * 256 * V, raw[k]);
         float2 s = make_float2(0.f, 0.f);
-        for (int i = threadIdx.x; i < p.pieces; i += 256) s = add2(s, p.row_part[(size_t)row * p.pieces + i]);
+        const float2 *parts = p.row_part + (size_t)row * p.pieces;
+        for (int i = threadIdx.x; i < p.pieces; i += 256) s = add2(s, parts[i]);
         s = team_totals<256>(s, scratch[turn], 1);
         const float c1 = s.x / (float)p.n, c2 = s.y / (float)p.n, mu = p.mean ? p.mean[row] : 0.f, r = p.rstd[row];
+        T *dx = p.dx + (size_t)row * p.dx_pitch;
 #pragma unroll
         for (int k = 0; k < K; k++) {
-            const size_t col = base + (size_t)(k * 256 + threadIdx.x) * V;
-            if (col >= p.n) continue;
+            const uint32_t col = first + k * 256 * V;
+            if (col >= n) continue;
             float dy[V], xh[V], gamma[V];
             ln_values<T, V>(p, raw[k], mu, r, dy, xh);
             load_params<V>(gamma, p.gamma, col, p.wide);
 #pragma unroll
             for (int j = 0; j < V; j++) dy[j] = r * (dy[j] * gamma[j] - c1 - xh[j] * c2);
-            store_pack<T, V>(p.dx + (size_t)row * p.dx_pitch + col, dy);
+            store_pack<T, V>(dx + col, dy);
         }
     }
 }
@@ -861,8 +882,8 @@ static int ln_backward_launch(LnBackward<T> p, float *dgamma, float *dbeta, int 
         B200_LAUNCH_CHECK();
     }
     if (p.weights) {
-        // many groups (blocks of the one-pass form) or many columns
-        if (p.groups > 16) Launch((unsigned)((2 * p.n + 31) / 32), 1024, 0, s)(ln_backward_join_kernel<32>, dgamma, dbeta, p.part, p.groups, p.n, accumulate);
+        // few columns need several threads each to fill the machine
+        if (p.n <= 16384 && p.groups > 8) Launch((unsigned)((2 * p.n + 31) / 32), 1024, 0, s)(ln_backward_join_kernel<32>, dgamma, dbeta, p.part, p.groups, p.n, accumulate);
         else Launch((unsigned)((2 * p.n + 1023) / 1024), 1024, 0, s)(ln_backward_join_kernel<1>, dgamma, dbeta, p.part, p.groups, p.n, accumulate);
         B200_LAUNCH_CHECK();
     }
