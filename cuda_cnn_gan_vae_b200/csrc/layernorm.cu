@@ -398,7 +398,8 @@ struct LnBackward {
     int weights;                 // form dgamma and dbeta
     float *part;                 // [groups][2][n] partial sums of dgamma and dbeta
     int groups;
-    float2 *row_part;            // long rows: [rows][pieces] partial sums of g and g xh
+    float2 *row_part;            // long rows: [rows][pieces] partial sums of g and g xh,
+    float2 *row_mean;            // [rows] and their means
     int pieces;
     // one-pass form: shared memory of a team's slot for a row of dy, a row of x or codes, and its number of slots
     uint32_t dy_bytes, x_bytes;
@@ -691,8 +692,10 @@ __global__ void __launch_bounds__(kLnBlock, 1) ln_backward_rows_kernel(const __g
     }
 }
 
-// Longer rows in two passes.  First: a thread owns V columns and walks a group of rows; it sums dgamma and dbeta of its columns, and
-// its warp writes the partial sums of g and g xh of each row.  Second: a block joins a row's partial sums and forms a piece of dx.
+// Longer rows in two passes.  First: a thread owns V columns (four times one, where rows are not read in 16-byte pieces) and walks a
+// group of rows; it sums dgamma and dbeta of its columns, and its warp writes the partial sums of g and g xh of each row.
+// Then a small kernel joins both kinds of sums, and the second pass, again a thread on its columns down a group of rows, forms
+// dx.  (With the rows' sums joined by every block of the second pass, 300 x 40001 fp16 took 71 us.)
 template <int V> constexpr int kLnRuns = V == 1 ? 4 : 1;      // runs of V columns of a thread, a slice apart
 template <typename T, int V>
 __global__ void __launch_bounds__(kLnSlice) ln_backward_columns_kernel(const __grid_constant__ LnBackward<T> p)
@@ -757,47 +760,70 @@ __global__ void __launch_bounds__(kLnSlice) ln_backward_columns_kernel(const __g
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(256) ln_backward_apply_kernel(const __grid_constant__ LnBackward<T> p)
+__global__ void __launch_bounds__(kLnSlice) ln_backward_apply_kernel(const __grid_constant__ LnBackward<T> p)
 {
-    constexpr int K = V == 1 ? 8 : 4;
-    __shared__ float2 scratch[2][8];
+    constexpr int C = kLnRuns<V>, U = 4 / C > 0 ? 4 / C : 1;
     grid_dependency_wait();
-    int turn = 0;
-    const uint32_t first = (blockIdx.x * 256 * K + threadIdx.x) * V, n = (uint32_t)p.n;
-    for (int row = blockIdx.y; row < p.rows; row += gridDim.y, turn ^= 1) {
-        LnRaw<T, V> raw[K];
-        const LnRow<T> at = ln_row(p, row);
+    const uint32_t first = (blockIdx.x * C * kLnSlice + threadIdx.x) * V, n = (uint32_t)p.n;
+    bool in[C];
+    float gamma[C][V];
 #pragma unroll
-        for (int k = 0; k < K; k++)
-            if (first + k * 256 * V < n) ln_load<T, V>(p, at, first + k * 256 * V, raw[k]);
-        float2 s = make_float2(0.f, 0.f);
-        const float2 *parts = p.row_part + (size_t)row * p.pieces;
-        for (int i = threadIdx.x; i < p.pieces; i += 256) s = add2(s, parts[i]);
-        s = team_totals<256>(s, scratch[turn], 1);
-        const float c1 = s.x / (float)p.n, c2 = s.y / (float)p.n, mu = p.mean ? p.mean[row] : 0.f, r = p.rstd[row];
-        T *dx = p.dx + (size_t)row * p.dx_pitch;
+    for (int c = 0; c < C; c++) {
+        in[c] = first + c * kLnSlice * V < n;
+        if (in[c]) load_params<V>(gamma[c], p.gamma, first + c * kLnSlice * V, p.wide);
+    }
+    const int begin = (int)((long long)p.rows * blockIdx.y / p.groups), end = (int)((long long)p.rows * (blockIdx.y + 1) / p.groups);
+#pragma unroll 2
+    for (int row = begin; row < end; row += U) {
+        LnRaw<T, V> raw[U][C];
 #pragma unroll
-        for (int k = 0; k < K; k++) {
-            const uint32_t col = first + k * 256 * V;
-            if (col >= n) continue;
-            float dy[V], xh[V], gamma[V];
-            ln_values<T, V>(p, raw[k], mu, r, dy, xh);
-            load_params<V>(gamma, p.gamma, col, p.wide);
+        for (int u = 0; u < U; u++) {
+            if (row + u >= end) break;
+            const LnRow<T> at = ln_row(p, row + u);
 #pragma unroll
-            for (int j = 0; j < V; j++) dy[j] = r * (dy[j] * gamma[j] - c1 - xh[j] * c2);
-            store_pack<T, V>(dx + col, dy);
+            for (int c = 0; c < C; c++)
+                if (in[c]) ln_load<T, V>(p, at, first + c * kLnSlice * V, raw[u][c]);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (row + u >= end) break;
+            const float2 m = p.row_mean[row + u];
+            const float mu = p.mean ? p.mean[row + u] : 0.f, r = p.rstd[row + u];
+            T *dx = p.dx + (size_t)(row + u) * p.dx_pitch;
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+                if (!in[c]) continue;
+                float dy[V], xh[V];
+                ln_values<T, V>(p, raw[u][c], mu, r, dy, xh);
+#pragma unroll
+                for (int j = 0; j < V; j++) dy[j] = r * (dy[j] * gamma[c][j] - m.x - xh[j] * m.y);
+                store_pack<T, V>(dx + first + c * kLnSlice * V, dy);
+            }
         }
     }
 }
 
 // Sum of the groups' partial rows, in an order that does not depend on how they were scheduled: SPLIT threads take every SPLIT-th
-// group of a column.
+// group of a column.  The blocks from `column_blocks` on join the rows' partial sums instead, a warp to a row.
+struct LnRows { const float2 *part; float2 *mean; int rows, pieces; };
 template <int SPLIT>
-__global__ void __launch_bounds__(1024) ln_backward_join_kernel(float *dgamma, float *dbeta, const float *__restrict__ part, int groups, size_t n, int accumulate)
+__global__ void __launch_bounds__(1024) ln_backward_join_kernel(float *dgamma, float *dbeta, const float *__restrict__ part, int groups, size_t n, int accumulate,
+                                                                unsigned column_blocks, LnRows r)
 {
     constexpr int kWide = 1024 / SPLIT;
     __shared__ float sums[SPLIT][kWide + 1];
     grid_dependency_wait();
+    if (blockIdx.x >= column_blocks) {
+        const long long row = (long long)(blockIdx.x - column_blocks) * 32 + (threadIdx.x >> 5);
+        if (row >= r.rows) return;
+        const float2 *at = r.part + (size_t)row * r.pieces;
+        float2 v = make_float2(0.f, 0.f);
+#pragma unroll 4
+        for (int k = threadIdx.x & 31; k < r.pieces; k += 32) v = add2(v, at[k]);
+        v = warp_totals(v);
+        if ((threadIdx.x & 31) == 0) r.mean[row] = make_float2(v.x / (float)n, v.y / (float)n);
+        return;
+    }
     const int c = threadIdx.x % kWide, w = threadIdx.x / kWide;
     const size_t i = (size_t)blockIdx.x * kWide + c;
     float s = 0.f;
@@ -839,6 +865,8 @@ static LnPlan ln_plan(int rows, size_t n, int v)
     return w;
 }
 
+static size_t row_bytes(const LnPlan &w, int rows) { return w.one_pass ? 0 : align_up((size_t)rows * (w.pieces + 1) * sizeof(float2), 16); }
+
 template <typename T, int V>
 static int ln_backward_launch(LnBackward<T> p, float *dgamma, float *dbeta, int accumulate, char *workspace, cudaStream_t s)
 {
@@ -846,7 +874,8 @@ static int ln_backward_launch(LnBackward<T> p, float *dgamma, float *dbeta, int 
     p.groups = w.groups;
     p.pieces = w.pieces;
     p.row_part = reinterpret_cast<float2 *>(workspace);
-    p.part = reinterpret_cast<float *>(workspace + align_up((size_t)p.rows * w.pieces * sizeof(float2), 16));
+    p.row_mean = p.row_part + (size_t)p.rows * w.pieces;
+    p.part = reinterpret_cast<float *>(workspace + row_bytes(w, p.rows));
     p.dgamma = dgamma;
     p.dbeta = dbeta;
     p.accumulate = accumulate;
@@ -877,14 +906,20 @@ static int ln_backward_launch(LnBackward<T> p, float *dgamma, float *dbeta, int 
     } else {
         Launch(dim3((unsigned)(w.pieces / (kLnSlice / 32)), (unsigned)w.groups), kLnSlice, 0, s)(ln_backward_columns_kernel<T, V>, p);
         B200_LAUNCH_CHECK();
-        constexpr size_t kPiece = 256 * (V == 1 ? 8 : 4 * V);
-        Launch(dim3((unsigned)((p.n + kPiece - 1) / kPiece), (unsigned)min(p.rows, 65535)), 256, 0, s)(ln_backward_apply_kernel<T, V>, p);
+    }
+    const LnRows rows = {p.row_part, p.row_mean, w.one_pass ? 0 : p.rows, w.pieces};
+    const unsigned row_blocks = (unsigned)((rows.rows + 31ll) / 32);
+    // few columns need several threads each to fill the machine
+    const int split = p.n <= 16384 && p.groups > 8 ? 32 : 1;
+    const unsigned column_blocks = p.weights ? (unsigned)((2 * p.n * split + 1023) / 1024) : 0;
+    if (column_blocks + row_blocks) {
+        const Launch launch(column_blocks + row_blocks, 1024, 0, s);
+        if (split > 1) launch(ln_backward_join_kernel<32>, dgamma, dbeta, p.part, p.groups, p.n, accumulate, column_blocks, rows);
+        else launch(ln_backward_join_kernel<1>, dgamma, dbeta, p.part, p.groups, p.n, accumulate, column_blocks, rows);
         B200_LAUNCH_CHECK();
     }
-    if (p.weights) {
-        // few columns need several threads each to fill the machine
-        if (p.n <= 16384 && p.groups > 8) Launch((unsigned)((2 * p.n + 31) / 32), 1024, 0, s)(ln_backward_join_kernel<32>, dgamma, dbeta, p.part, p.groups, p.n, accumulate);
-        else Launch((unsigned)((2 * p.n + 1023) / 1024), 1024, 0, s)(ln_backward_join_kernel<1>, dgamma, dbeta, p.part, p.groups, p.n, accumulate);
+    if (!w.one_pass) {
+        Launch(dim3((unsigned)(w.pieces / (kLnSlice / 32)), (unsigned)w.groups), kLnSlice, 0, s)(ln_backward_apply_kernel<T, V>, p);
         B200_LAUNCH_CHECK();
     }
     return B200_OK;
@@ -927,7 +962,7 @@ size_t b200_ln_backward_workspace(int rows, size_t n)
     size_t most = 0;
     for (int v = 1; v <= 8; v *= v == 1 ? 4 : 2) {
         const LnPlan w = ln_plan(rows, n, v);
-        const size_t bytes = align_up((size_t)rows * w.pieces * sizeof(float2), 16) + sizeof(float) * 2 * n * (size_t)w.groups;
+        const size_t bytes = row_bytes(w, rows) + sizeof(float) * 2 * n * (size_t)w.groups;
         most = bytes > most ? bytes : most;
     }
     return most;
