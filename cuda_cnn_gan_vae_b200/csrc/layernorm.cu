@@ -405,8 +405,8 @@ struct LnBackward {
     uint32_t dy_bytes, x_bytes;
     int depth;
     unsigned *status;
-    float *dgamma, *dbeta;       // written directly where there is one group
-    int accumulate;
+    float *dgamma, *dbeta;       // written directly where the blocks are one cluster
+    int accumulate, one_cluster;
     int wide;                    // gamma can be read in 16-byte pieces
 };
 
@@ -679,17 +679,39 @@ __global__ void __launch_bounds__(kLnBlock, 1) ln_backward_rows_kernel(const __g
         }
         __syncthreads();
     }
-    if (team) return;
-    float *out_g = p.groups == 1 ? p.dgamma : p.part + (size_t)blockIdx.x * 2 * n, *out_b = p.groups == 1 ? p.dbeta : out_g + n;
-    const bool add = p.groups == 1 && p.accumulate;
+    if (!p.one_cluster) {
+        if (team) return;
+        float *out_g = p.part + (size_t)blockIdx.x * 2 * n, *out_b = out_g + n;
 #pragma unroll
-    for (int i = 0; i < kLnBack; i++) {
-        if (!in[i / V]) continue;
-        const int col = (i / V * TEAM + t) * V + i % V;
-        const float vg = i & 1 ? dgamma[i / 2].y : dgamma[i / 2].x, vb = i & 1 ? dbeta[i / 2].y : dbeta[i / 2].x;
-        out_g[col] = add ? out_g[col] + vg : vg;
-        out_b[col] = add ? out_b[col] + vb : vb;
+        for (int i = 0; i < kLnBack; i++) {
+            if (!in[i / V]) continue;
+            const int col = (i / V * TEAM + t) * V + i % V;
+            out_g[col] = i & 1 ? dgamma[i / 2].y : dgamma[i / 2].x;
+            out_b[col] = i & 1 ? dbeta[i / 2].y : dbeta[i / 2].x;
+        }
+        return;
     }
+    // Few rows: the blocks are one cluster and join their sums through distributed shared memory, every block a share of the columns,
+    // in the order of the blocks; no second kernel.
+    float *sums = reinterpret_cast<float *>(ring);
+    if (team == 0) {
+#pragma unroll
+        for (int i = 0; i < kLnBack; i++) {
+            if (!in[i / V]) continue;
+            const int col = (i / V * TEAM + t) * V + i % V;
+            sums[col] = i & 1 ? dgamma[i / 2].y : dgamma[i / 2].x;
+            sums[n + col] = i & 1 ? dbeta[i / 2].y : dbeta[i / 2].x;
+        }
+    }
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    for (int i = (int)cluster.block_rank() * kLnBlock + (int)threadIdx.x; i < 2 * n; i += (int)cluster.num_blocks() * kLnBlock) {
+        float v = 0.f;
+        for (unsigned k = 0; k < cluster.num_blocks(); k++) v += *cluster.map_shared_rank(sums + i, k);
+        float *out = i < n ? p.dgamma + i : p.dbeta + (i - n);
+        *out = p.accumulate ? *out + v : v;
+    }
+    cluster.sync();                                         // no block leaves while another still reads its sums
 }
 
 // Longer rows in two passes.  First: a thread owns V columns (four times one, where rows are not read in 16-byte pieces) and walks a
@@ -845,16 +867,18 @@ __global__ void __launch_bounds__(1024) ln_backward_join_kernel(float *dgamma, f
 }
 
 constexpr size_t kLnOnePass = 8192;
-struct LnPlan { bool one_pass; int team, groups, pieces; };
+struct LnPlan { bool one_pass, one_cluster; int team, groups, pieces; };
 static LnPlan ln_plan(int rows, size_t n, int v)
 {
     LnPlan w = {};
     w.one_pass = n <= kLnOnePass;
     if (w.one_pass) {
         w.team = n <= 512 ? 32 : n <= 1024 ? 64 : n <= 2048 ? 128 : n <= 4096 ? 256 : 512;
-        // One block where each team then has eight rows at most: it writes the gradients itself.
+        // A cluster of up to eight blocks where each team then has four rows at most: it joins the gradients itself.
         const int teams = kLnBlock / w.team;
-        w.groups = rows <= 8 * teams ? 1 : min((rows + teams - 1) / teams, sm_count());
+        w.groups = min((rows + teams - 1) / teams, sm_count());
+        w.one_cluster = rows <= 32 * teams;
+        if (w.one_cluster) w.groups = w.groups > 4 ? 8 : w.groups > 2 ? 4 : w.groups;
     } else {
         const size_t slice = (size_t)kLnSlice * (v == 1 ? kLnRuns<1> : kLnRuns<4> * v), slices = (n + slice - 1) / slice;
         w.pieces = (int)slices * (kLnSlice / 32);
@@ -880,6 +904,7 @@ static int ln_backward_launch(LnBackward<T> p, float *dgamma, float *dbeta, int 
     p.dbeta = dbeta;
     p.accumulate = accumulate;
     p.wide = wide_params(p.gamma, p.gamma);
+    p.one_cluster = w.one_cluster;
     if (w.one_pass) {
         int r = status_word(&p.status);
         if (r) return r;
@@ -887,11 +912,12 @@ static int ln_backward_launch(LnBackward<T> p, float *dgamma, float *dbeta, int 
         p.dy_bytes = (uint32_t)align_up(p.n * sizeof(T) + 16, 16);
         p.x_bytes = p.codes ? (uint32_t)(p.blocks * kCkptBlock) : p.dy_bytes;
         p.depth = min(kLnMostDepth, (int)(kLnRing / (teams * (p.dy_bytes + p.x_bytes))));      // three at least: 8192 values of 4 bytes, twice
-        const uint32_t smem = max((uint32_t)(teams * p.depth) * (p.dy_bytes + p.x_bytes), w.team < kLnBlock ? 32768u : 0u);
+        // the ring, and after it the sums of the teams (32 KB) and of the block (two for every column)
+        const uint32_t smem = max(max((uint32_t)(teams * p.depth) * (p.dy_bytes + p.x_bytes), 32768u), (uint32_t)(2 * sizeof(float) * p.n));
 #define B200_LN_ROWS(TEAM)                                                                                                                           \
     do {                                                                                                                                             \
         if ((r = allow_shared<ln_backward_rows_kernel<T, V, TEAM>>((int)kLnRing))) return r;                                                         \
-        Launch((unsigned)w.groups, kLnBlock, smem, s)(ln_backward_rows_kernel<T, V, TEAM>, p);                                                       \
+        Launch((unsigned)w.groups, kLnBlock, smem, s).cluster(w.one_cluster ? (unsigned)w.groups : 1u)(ln_backward_rows_kernel<T, V, TEAM>, p);      \
     } while (0)
         switch (w.team) {
         case 32: B200_LN_ROWS(32); break;
@@ -902,7 +928,7 @@ static int ln_backward_launch(LnBackward<T> p, float *dgamma, float *dbeta, int 
         }
 #undef B200_LN_ROWS
         B200_LAUNCH_CHECK();
-        if (w.groups == 1) return B200_OK;
+        if (w.one_cluster) return B200_OK;
     } else {
         Launch(dim3((unsigned)(w.pieces / (kLnSlice / 32)), (unsigned)w.groups), kLnSlice, 0, s)(ln_backward_columns_kernel<T, V>, p);
         B200_LAUNCH_CHECK();
