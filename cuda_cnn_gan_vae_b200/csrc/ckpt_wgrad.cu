@@ -66,19 +66,23 @@ __global__ void __launch_bounds__(256) ckpt8_wgrad_simt_kernel(float *dweight, f
 // A CTA pair computes 256 x 256 outputs: 256 of delta's columns (128 per CTA) by 256 of the input's (128 decoded by each CTA and
 // read by both), one 256-row MMA per 16 rows of the batch, accumulated in tensor memory.  Both operands are MN-major, so a
 // row of delta or of the checkpoint becomes a row of the shared-memory tile as it lies in memory: no transposition anywhere.
-//   * The kept values have 8 significant bits and are exact in bf16 with their scale.  delta is cut into PARTS pieces of 8 bits (bf16 1,
-//     fp16 2, fp32 3, in either tensor-core mode), each exact, so every product is exact and the only
-//     roundings are those of the fp32 accumulator.  The tensor core truncates its sums, a bias that grows with their number:
-//     after kChunk stages the accumulator is added to the output (rounded to nearest) and starts again from zero.  8192 rows at
-//     a stretch were off by 2.5e-6 of the result, chunks of 2048 are by 4e-7.
-//   * One warp brings the codes and delta in by TMA (bf16 straight into the operand tile); four groups of four warps decode and
-//     split from shared memory into a ring of operand stages (five instructions for two values, once per pair and tile).  A
-//     group takes every fourth stage, so four stages are in work at a time: with all sixteen warps on each stage its chain of
-//     waits, loads and stores was in series with the next one's (514 us at 8192 rows, 4096 x 4096, bf16; and 1030 us where
-//     they loaded from global memory into registers three stages ahead).
+//   * The kept values have 8 significant bits and are exact in bf16 with their scale.  delta is cut into PARTS pieces of 8 bits
+//     (bf16 1, fp16 2, fp32 3, in either tensor-core mode), each exact, so every product is exact and the only roundings are
+//     those of the fp32 accumulator.  The tensor core truncates its sums, a bias that grows with their number: after kChunk
+//     stages the accumulator is added to the output (rounded to nearest) and starts again from zero.  8192 rows at a stretch
+//     were off by 2.5e-6 of the result, chunks of 2048 are by 4e-7, for 22 of 261 us.
+//   * One warp each brings the codes and delta in by TMA (bf16 straight into the operand tile); four groups of four warps decode
+//     and split from shared memory into a ring of operand stages (five instructions for two values, once per pair and tile).
+//     A group takes every fourth stage, so four stages are in work at a time: with all sixteen warps on each stage its chain of
+//     waits, loads and stores was in series with the next one's.  Stages are as long as the rings allow (bf16 with 32 rows
+//     in place of 64: 350 us for 261; fp16 with 16 for 32: 652 for 495), because a stage's waits, exponents and fences cost a
+//     group some hundred instructions whatever its length.
 //   * The grid is one pair per two SMs.  Whole tiles go round the pairs; what is left over (or everything, where there are
 //     fewer tiles than pairs) is split along the batch into units that write partial tiles, joined by a second
 //     kernel in the order of the units.  No atomics: the result does not depend on scheduling.
+// Measured at 8192 rows, 4096 x 4096: bf16 261 us = 1.05 PFLOP/s (303 us with inputs that are not in L2), fp16 495, fp32 782; the
+// tensor pipe is active half the time in bf16, the converter warps issue in 60 % of the cycles, and without their stores
+// (199 us) or without the products (199 us) it is no faster than shared memory and the two together allow.
 constexpr int kPairTile = 256;                     // outputs of a pair in both directions
 constexpr int kEpilogueWarps = 4, kConverterWarps = 16, kGroupWarps = 4, kGroups = kConverterWarps / kGroupWarps;
 constexpr int kConverters = kConverterWarps * 32;
@@ -468,8 +472,8 @@ ckpt8_wgrad_tc_kernel(const __grid_constant__ CUtensorMap codes_map, const __gri
     } else if (warp == kIssuer) {
         // ------------------------------------------------------------------ MMA issuer (one thread of the leader)
         // The peer's thread passes its full stages on.  (An arrival with .release.cluster here took some 1500 cycles, more than all
-        // the work on a stage, 900 us in place of MEASURE at 8192 rows, 4096 x 4096.  The tile itself stays in the peer's shared
-        // memory, where its writers have made it visible to the tensor core before they arrived.)
+        // the work on a stage: 900 us in place of 440 at the time.  The tile itself stays in the peer's shared memory, where its
+        // writers have made it visible to the tensor core before they arrived.)
         if (rank == 1 && lane == 0) {
             ItemCursor at;
             int stage = 0;

@@ -948,7 +948,12 @@ int status_word(unsigned **dev)
     if (d < 0 || d >= 64) d = 0;
     if (!g_status_host[d]) {
         void *h = nullptr, *dp = nullptr;
-        B200_CUDA(cudaHostAlloc(&h, sizeof(unsigned), cudaHostAllocMapped));
+        // the first call may be part of a stream capture, which forbids allocations to threads in the stricter modes
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        B200_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+        const cudaError_t e = cudaHostAlloc(&h, sizeof(unsigned), cudaHostAllocMapped);
+        B200_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+        B200_CUDA(e);
         *(unsigned *)h = 0;
         B200_CUDA(cudaHostGetDevicePointer(&dp, h, 0));
         g_status_host[d] = (unsigned *)h;

@@ -142,8 +142,15 @@ class Checkpoint8:
         return cls(torch.empty(rows, 32 * blocks, dtype=torch.int8, device=device),
                    torch.empty(rows, blocks, dtype=torch.uint8, device=device), n)
 
+    def _here(self):
+        """This checkpoint, which must be on the current device."""
+        if self.codes.get_device() != _device():
+            raise B200Error(2, f"the checkpoint is on {self.codes.device}, the current device is cuda:{_device()}")
+        return self
+
     def _match(self, x, name):
         got = _rows(x, name)
+        self._here()
         if got[1] != self.rows or got[2] != self.n:
             raise B200Error(1, f"{name} must have {self.rows} rows of {self.n} values")
         return got
@@ -538,7 +545,7 @@ def ln_forward(x, gamma, beta, eps=1e-6, y=None, mean=None, rstd=None, checkpoin
     y_pitch = _like(y, "y", (kind, rows, n), "x")[3]
     codes = exponents = None
     if checkpoint is not None:
-        if checkpoint.rows != rows or checkpoint.n != n:
+        if checkpoint._here().rows != rows or checkpoint.n != n:
             raise B200Error(1, f"the checkpoint must have {rows} rows of {n} values")
         codes, exponents = checkpoint.codes.data_ptr(), checkpoint.exponents.data_ptr()
     _check(load().b200_ln_forward(y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), codes, exponents, x.data_ptr(), gamma.data_ptr(),
@@ -557,7 +564,7 @@ def ln_backward(dy, x, mean, rstd, gamma, dgamma, dbeta, create_delta_weight=Tru
     codes = exponents = x_ptr = mean_ptr = None
     x_pitch = n
     if isinstance(x, Checkpoint8):
-        if x.rows != rows or x.n != n:
+        if x._here().rows != rows or x.n != n:
             raise B200Error(1, f"the checkpoint must have {rows} rows of {n} values")
         codes, exponents = x.codes.data_ptr(), x.exponents.data_ptr()
     else:
@@ -577,7 +584,7 @@ def checkpoint_wgrad(dweight, dbias, delta, checkpoint, accumulate=True, workspa
     """Gradients of a Linear layer whose input was kept in 8 bits: dweight [out x n] (+)= delta^T * values and, unless dbias is
     None, dbias [out] (+)= sum of delta over the rows.  delta [rows x out] in fp32, bf16 or fp16; the gradients are fp32."""
     kind, rows, out, pitch = _rows(delta, "delta")
-    if checkpoint.rows != rows:
+    if checkpoint._here().rows != rows:
         raise B200Error(1, "delta and the checkpoint must have the same number of rows")
     _param(dweight, out * checkpoint.n, "dweight")
     if dbias is not None:

@@ -330,7 +330,7 @@ int b200_adam_prepared(float *weight, const float *dweight, float *m, float *v, 
 enum { B200_F32 = 0, B200_BF16 = 1, B200_F16 = 2 };
 
 /* In this section a tensor is a matrix of `rows` rows of n values; row r starts at element r * pitch (pitch >= n; a dense
- * tensor [W,Z,Y,X] taken per sample has rows = W, n = pitch = Z*Y*X).  1 <= n <= 2^31 - 4096, as many rows at most; rows may be 0 (nothing is read, and
+ * tensor [W,Z,Y,X] taken per sample has rows = W, n = pitch = Z*Y*X).  1 <= n <= 2^31 - 65536, as many rows at most; rows may be 0 (nothing is read, and
  * gradients that are not accumulated become zero).  Pointers are aligned to the element size, codes to 16 bytes.  Nothing here
  * uses the library's scratch arena: a call that needs scratch takes it from the caller (16-byte aligned, at least as many bytes
  * as its ..._workspace() says for the same sizes; the contents need not be kept between calls), so calls on several streams and

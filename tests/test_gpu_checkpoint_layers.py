@@ -240,3 +240,43 @@ def test_refusals(ops):
         NetLayerLayerNormalization((3, 4, 5), 2, dims=4)
     with pytest.raises(ops.B200Error):
         dcgan_discriminator(2, image=(3, 32, 32), widths=(8,), norm="group")
+
+
+FIRST_CALL = """
+import sys
+sys.path.insert(0, {root!r})
+import torch
+from cuda_cnn_gan_vae_b200 import ops
+n = {n}
+x, g, b = torch.randn(64, n, device="cuda"), torch.ones(n, device="cuda"), torch.zeros(n, device="cuda")
+y, dx, mean, rstd = torch.empty_like(x), torch.empty_like(x), torch.empty(64, device="cuda"), torch.empty(64, device="cuda")
+dg, db, delta = torch.empty(n, device="cuda"), torch.empty(n, device="cuda"), torch.randn(64, 48, device="cuda")
+dw, dbias, c = torch.empty(48, n, device="cuda"), torch.empty(48, device="cuda"), ops.Checkpoint8.empty(64, n)
+def step():
+    ops.ln_forward(x, g, b, y=y, mean=mean, rstd=rstd, checkpoint=c)
+    ops.ln_backward(y, c, None, rstd, g, dg, db, accumulate=False, dx=dx)
+    ops.CTensorApplyFunc.Backward(dx, c, dx, "tanh")
+    ops.checkpoint_wgrad(dw, dbias, delta, c, accumulate=False)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    step()
+graph.replay()
+torch.cuda.synchronize()
+got = [t.clone() for t in (y, dx, dg, db, dw, dbias)]
+step()
+ops.stream_status()
+assert all(torch.equal(a, b) for a, b in zip(got, (y, dx, dg, db, dw, dbias)))
+print("captured")
+"""
+
+
+@pytest.mark.parametrize("n", [300, 20000])
+def test_first_calls_of_a_process_inside_a_capture(n):
+    """Nothing that a first call sets up is forbidden while a stream is captured."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL.format(root=root, n=n)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stdout[-500:] + r.stderr[-2000:]

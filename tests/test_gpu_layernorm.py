@@ -282,3 +282,13 @@ def test_refusals(ops):
         with pytest.raises(B):
             bad()
     ops.stream_status()
+
+
+@pytest.mark.parametrize("n", [1000, 20000])
+def test_an_infinity_in_a_row_is_its_mean(ops, n):
+    x, _, gamma, beta = make(5, n, "float32", 12)
+    x[1, n // 3], x[2, n - 2], x[3, 7], x[3, 9] = float("inf"), float("-inf"), float("inf"), float("-inf")
+    got = ops.ln_forward(x, gamma, beta)
+    mean = got["mean"].cpu()
+    assert mean[1] == float("inf") and mean[2] == float("-inf") and torch.isnan(mean[3]) and torch.isfinite(mean[[0, 4]]).all()
+    assert torch.isnan(got["y"][1:4]).all() and torch.isfinite(got["y"][[0, 4]]).all()
