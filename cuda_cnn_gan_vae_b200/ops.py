@@ -74,19 +74,20 @@ _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
 
 
-def _stream_id():
-    """The current stream of the current device as a number (a call of a few microseconds is made of little else)."""
-    return torch._C._cuda_getCurrentRawStream(_device())
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_F32 = torch.float32
 
 
-def _rows(x, name="tensor"):
+# The calls below take a few microseconds, most of them spent here: each looks the device up once and hands it on.
+
+def _rows(x, name, dev):
     """(type code, rows, values in a row, pitch) of an activation tensor: its first dimension is the rows, the others (dense)
     are a row.  A 2-D tensor may have any pitch between its rows."""
     kind = _TYPES.get(x.dtype) if isinstance(x, torch.Tensor) else None
     if kind is None or not x.is_cuda:
         raise B200Error(2, f"{name} must be an fp32, bf16 or fp16 CUDA tensor")
-    if x.get_device() != _device():
-        raise B200Error(2, f"{name} is on {x.device}, the current device is cuda:{_device()}")
+    if x.get_device() != dev:
+        raise B200Error(2, f"{name} is on {x.device}, the current device is cuda:{dev}")
     shape = x.shape
     if len(shape) == 2 and shape[1]:
         rows, n = shape
@@ -99,24 +100,27 @@ def _rows(x, name="tensor"):
     return kind, shape[0], n, n
 
 
-def _param(x, n, name):
-    """A contiguous fp32 tensor of n elements on the current device."""
-    if isinstance(x, torch.Tensor) and x.dtype == torch.float32 and x.numel() == n and x.get_device() == _device() and x.is_contiguous():
-        return x
+def _param(x, n, name, dev):
+    """The address of x, a contiguous fp32 tensor of n elements on the current device."""
+    try:
+        if x.dtype is _F32 and x.numel() == n and x.get_device() == dev and x.is_contiguous():
+            return x.data_ptr()
+    except AttributeError:
+        pass
     _t(x, name)
     if x.numel() != n:
         raise B200Error(1, f"{name} must have {n} elements")
-    raise B200Error(2, f"{name} is on {x.device}, the current device is cuda:{_device()}")
+    raise B200Error(2, f"{name} is on {x.device}, the current device is cuda:{dev}")
 
 
-def _like(x, name, want, other):
-    """_rows(x), which must have the type, rows and row length of `other`."""
-    got = _rows(x, name)
+def _like(x, name, want, other, dev):
+    """The pitch of x, which must have the type, rows and row length of `other`."""
+    got = _rows(x, name, dev)
     if got[0] != want[0]:
         raise B200Error(2, f"{name} must have the type of {other}")
     if got[1:3] != want[1:3]:
         raise B200Error(1, f"{name} must have the size of {other}")
-    return got
+    return got[3]
 
 
 class Checkpoint8:
@@ -142,31 +146,33 @@ class Checkpoint8:
         return cls(torch.empty(rows, 32 * blocks, dtype=torch.int8, device=device),
                    torch.empty(rows, blocks, dtype=torch.uint8, device=device), n)
 
-    def _here(self):
+    def _here(self, dev):
         """This checkpoint, which must be on the current device."""
-        if self.codes.get_device() != _device():
-            raise B200Error(2, f"the checkpoint is on {self.codes.device}, the current device is cuda:{_device()}")
+        if self.codes.get_device() != dev:
+            raise B200Error(2, f"the checkpoint is on {self.codes.device}, the current device is cuda:{dev}")
         return self
 
-    def _match(self, x, name):
-        got = _rows(x, name)
-        self._here()
+    def _match(self, x, name, dev):
+        got = _rows(x, name, dev)
+        self._here(dev)
         if got[1] != self.rows or got[2] != self.n:
             raise B200Error(1, f"{name} must have {self.rows} rows of {self.n} values")
         return got
 
     def store(self, x, keep_sign=False):
         """Keeps x.  keep_sign: a negative value never becomes 0 (the derivative of ReLU and LeakyReLU is then exact)."""
-        kind, rows, n, pitch = self._match(x, "x")
+        dev = _device()
+        kind, rows, n, pitch = self._match(x, "x", dev)
         _check(load().b200_ckpt8_store(self.codes.data_ptr(), self.exponents.data_ptr(), x.data_ptr(), kind, rows, n, pitch,
-                                       int(keep_sign), _stream_id()))
+                                       int(keep_sign), _raw_stream(dev)))
         return self
 
     def load(self, output):
         """The kept values into `output` (fp32, bf16 or fp16), which is returned."""
-        kind, rows, n, pitch = self._match(output, "output")
+        dev = _device()
+        kind, rows, n, pitch = self._match(output, "output", dev)
         _check(load().b200_ckpt8_load(output.data_ptr(), self.codes.data_ptr(), self.exponents.data_ptr(), kind, rows, n, pitch,
-                                      _stream_id()))
+                                      _raw_stream(dev)))
         return output
 
 
@@ -486,10 +492,11 @@ class CTensorApplyFunc:
     def Backward(output, z, error, func, leaky_slope=0.1):
         """output = f'(z) * error.  z may be a Checkpoint8 (of the function's input); output and error then may be fp32, bf16 or fp16."""
         if isinstance(z, Checkpoint8):
-            kind, rows, n, pitch = z._match(output, "output")
-            e = _like(error, "error", (kind, rows, n), "output")
+            dev = _device()
+            kind, rows, n, pitch = z._match(output, "output", dev)
+            error_pitch = _like(error, "error", (kind, rows, n), "output", dev)
             _check(load().b200_ckpt8_activation_backward(output.data_ptr(), z.codes.data_ptr(), z.exponents.data_ptr(), error.data_ptr(),
-                                                         kind, rows, n, pitch, e[3], ACT[func], leaky_slope, _stream_id()))
+                                                         kind, rows, n, pitch, error_pitch, ACT[func], leaky_slope, _raw_stream(dev)))
             return
         _t(output), _t(z), _t(error)
         _check(load().b200_activation_backward(_ptr(output), _ptr(z), _ptr(error), z.numel(), ACT[func], leaky_slope, _stream()))
@@ -522,77 +529,84 @@ def bn_backward(dy, xhat, ivar, gamma, dgamma, dbeta, create_delta_weight=True):
     return dx
 
 
-def _workspace(size, given, name, like):
-    """The caller's workspace tensor, or a fresh one from torch's allocator (which orders its reuse by stream and keeps the
-    workspaces of captured graphs apart); `like`: an fp32 tensor on the current device."""
+def _workspace(size, given, name, like, dev):
+    """(tensor, address, bytes) of the caller's workspace, or of a fresh one from torch's allocator (which orders its reuse by stream
+    and keeps the workspaces of captured graphs apart); `like`: an fp32 tensor on the current device."""
     if given is None:
-        return (like.new_empty((size + 3) // 4), size) if size else (None, 0)
-    if not (isinstance(given, torch.Tensor) and given.is_cuda and given.is_contiguous() and given.get_device() == _device()):
+        if not size:
+            return None, None, 0
+        given = like.new_empty((size + 3) // 4)
+        return given, given.data_ptr(), size
+    if not (isinstance(given, torch.Tensor) and given.is_cuda and given.is_contiguous() and given.get_device() == dev):
         raise B200Error(2, f"{name}: the workspace must be a contiguous tensor on the current device")
-    return given, given.numel() * given.element_size()
+    return given, given.data_ptr(), given.numel() * given.element_size()
 
 
 def ln_forward(x, gamma, beta, eps=1e-6, y=None, mean=None, rstd=None, checkpoint=None):
     """Layer normalisation of every row of x (its first dimension is the rows, the others are normalised together) in fp32,
     bf16 or fp16 with fp32 parameters.  checkpoint: a Checkpoint8 that receives the normalised values for ln_backward.
     Returns dict(y, mean, rstd)."""
-    kind, rows, n, pitch = _rows(x, "x")
-    _param(gamma, n, "gamma"), _param(beta, n, "beta")
+    dev = _device()
+    kind, rows, n, pitch = _rows(x, "x", dev)
     if y is None:
         y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    mean = torch.empty(rows, device=x.device) if mean is None else _param(mean, rows, "mean")
-    rstd = torch.empty(rows, device=x.device) if rstd is None else _param(rstd, rows, "rstd")
-    y_pitch = _like(y, "y", (kind, rows, n), "x")[3]
+    if mean is None:
+        mean = torch.empty(rows, device=x.device)
+    if rstd is None:
+        rstd = torch.empty(rows, device=x.device)
+    y_pitch = _like(y, "y", (kind, rows, n), "x", dev)
     codes = exponents = None
     if checkpoint is not None:
-        if checkpoint._here().rows != rows or checkpoint.n != n:
+        if checkpoint._here(dev).rows != rows or checkpoint.n != n:
             raise B200Error(1, f"the checkpoint must have {rows} rows of {n} values")
         codes, exponents = checkpoint.codes.data_ptr(), checkpoint.exponents.data_ptr()
-    _check(load().b200_ln_forward(y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), codes, exponents, x.data_ptr(), gamma.data_ptr(),
-                                  beta.data_ptr(), kind, rows, n, pitch, y_pitch, eps, _stream_id()))
+    _check(load().b200_ln_forward(y.data_ptr(), _param(mean, rows, "mean", dev), _param(rstd, rows, "rstd", dev), codes, exponents,
+                                  x.data_ptr(), _param(gamma, n, "gamma", dev), _param(beta, n, "beta", dev), kind, rows, n, pitch,
+                                  y_pitch, eps, _raw_stream(dev)))
     return dict(y=y, mean=mean, rstd=rstd)
 
 
 def ln_backward(dy, x, mean, rstd, gamma, dgamma, dbeta, create_delta_weight=True, accumulate=True, dx=None, workspace=None):
     """Backward pass of ln_forward; returns dx.  x: the input of the forward pass, or the Checkpoint8 it filled (mean is then
     not read and may be None).  dgamma, dbeta (fp32, n elements) are added to, or written with accumulate=False."""
-    kind, rows, n, dy_pitch = _rows(dy, "dy")
-    _param(gamma, n, "gamma"), _param(rstd, rows, "rstd")
+    dev = _device()
+    kind, rows, n, dy_pitch = _rows(dy, "dy", dev)
     if dx is None:
         dx = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device)
-    dx_pitch = _like(dx, "dx", (kind, rows, n), "dy")[3]
-    codes = exponents = x_ptr = mean_ptr = None
+    dx_pitch = _like(dx, "dx", (kind, rows, n), "dy", dev)
+    codes = exponents = x_ptr = mean_ptr = dg = db = None
     x_pitch = n
     if isinstance(x, Checkpoint8):
-        if x._here().rows != rows or x.n != n:
+        if x._here(dev).rows != rows or x.n != n:
             raise B200Error(1, f"the checkpoint must have {rows} rows of {n} values")
         codes, exponents = x.codes.data_ptr(), x.exponents.data_ptr()
     else:
-        x_pitch = _like(x, "x", (kind, rows, n), "dy")[3]
-        x_ptr, mean_ptr = x.data_ptr(), _param(mean, rows, "mean").data_ptr()
-    dg = db = None
+        x_pitch = _like(x, "x", (kind, rows, n), "dy", dev)
+        x_ptr, mean_ptr = x.data_ptr(), _param(mean, rows, "mean", dev)
+    gamma_ptr, rstd_ptr = _param(gamma, n, "gamma", dev), _param(rstd, rows, "rstd", dev)
     if create_delta_weight:
-        dg, db = _param(dgamma, n, "dgamma").data_ptr(), _param(dbeta, n, "dbeta").data_ptr()
-    workspace, size = _workspace(load().b200_ln_backward_workspace(rows, n), workspace, "ln_backward", gamma)
-    _check(load().b200_ln_backward(dx.data_ptr(), dg, db, dy.data_ptr(), x_ptr, mean_ptr, rstd.data_ptr(), codes, exponents, gamma.data_ptr(),
-                                   kind, rows, n, dx_pitch, dy_pitch, x_pitch, int(create_delta_weight), int(accumulate),
-                                   workspace.data_ptr() if workspace is not None else None, size, _stream_id()))
+        dg, db = _param(dgamma, n, "dgamma", dev), _param(dbeta, n, "dbeta", dev)
+    lib = load()
+    workspace, ws, size = _workspace(lib.b200_ln_backward_workspace(rows, n), workspace, "ln_backward", gamma, dev)
+    _check(lib.b200_ln_backward(dx.data_ptr(), dg, db, dy.data_ptr(), x_ptr, mean_ptr, rstd_ptr, codes, exponents, gamma_ptr,
+                                kind, rows, n, dx_pitch, dy_pitch, x_pitch, int(create_delta_weight), int(accumulate), ws, size,
+                                _raw_stream(dev)))
     return dx
 
 
 def checkpoint_wgrad(dweight, dbias, delta, checkpoint, accumulate=True, workspace=None):
     """Gradients of a Linear layer whose input was kept in 8 bits: dweight [out x n] (+)= delta^T * values and, unless dbias is
     None, dbias [out] (+)= sum of delta over the rows.  delta [rows x out] in fp32, bf16 or fp16; the gradients are fp32."""
-    kind, rows, out, pitch = _rows(delta, "delta")
-    if checkpoint._here().rows != rows:
+    dev = _device()
+    kind, rows, out, pitch = _rows(delta, "delta", dev)
+    n = checkpoint.n
+    if checkpoint._here(dev).rows != rows:
         raise B200Error(1, "delta and the checkpoint must have the same number of rows")
-    _param(dweight, out * checkpoint.n, "dweight")
-    if dbias is not None:
-        _param(dbias, out, "dbias")
-    workspace, size = _workspace(load().b200_ckpt8_wgrad_workspace(kind, rows, out, checkpoint.n, delta.data_ptr(), pitch), workspace, "checkpoint_wgrad", dweight)
-    _check(load().b200_ckpt8_wgrad(dweight.data_ptr(), dbias.data_ptr() if dbias is not None else None, int(accumulate), delta.data_ptr(),
-                                   checkpoint.codes.data_ptr(), checkpoint.exponents.data_ptr(), kind, rows, out, checkpoint.n, pitch,
-                                   workspace.data_ptr() if workspace is not None else None, size, _stream_id()))
+    dw, db, d = _param(dweight, out * n, "dweight", dev), None if dbias is None else _param(dbias, out, "dbias", dev), delta.data_ptr()
+    lib = load()
+    workspace, ws, size = _workspace(lib.b200_ckpt8_wgrad_workspace(kind, rows, out, n, d, pitch), workspace, "checkpoint_wgrad", dweight, dev)
+    _check(lib.b200_ckpt8_wgrad(dw, db, int(accumulate), d, checkpoint.codes.data_ptr(), checkpoint.exponents.data_ptr(), kind, rows, out,
+                                n, pitch, ws, size, _raw_stream(dev)))
 
 
 def vae_forward(mu, logvar, eps, want_kl=True):
