@@ -452,23 +452,39 @@ __device__ __forceinline__ void ln_values(const LnBackward<T> &p, const LnRaw<T,
 // Rows of up to 8192 values in one pass: a team holds a row, a thread the same sixteen columns of every row, so gamma stays in
 // registers and dgamma, dbeta are summed there; the teams of a block join theirs in shared memory, the blocks (one per SM) in a
 // second kernel, or, where the rows are few, in distributed shared memory.  Rows come into a ring of slots in shared memory by
-// bulk copies, several rows ahead.  A bulk copy moves whole 16-byte pieces; the values before the first and after the last of a
-// row that starts anywhere (at most seven each) are loaded by their threads a row ahead.
-// Measured at 16384 x 2048 bf16 with the rows kept in 8 bits: 48 us, 3.5 TB/s, half the cycles issue (sixteen warps an SM wait for
+// bulk copies, several rows ahead.  A bulk copy moves whole 16-byte pieces: of a row that starts anywhere also the neighbours'
+// values in its first and its last piece, which nobody looks at.  Only pieces that lie whole in the tensor are copied; the values
+// of the others (at most seven at either end of the tensor) are loaded by their threads.  (With each row's own whole pieces copied
+// and its first and last values loaded a row ahead, 5003 x 1021 fp16 took 22.5 us.)
+// Measured at 16384 x 2048 bf16 with the rows kept in 8 bits: 47 us, 3.6 TB/s, half the cycles issue (sixteen warps an SM wait for
 // one another at a row's barrier); loads into registers, two blocks an SM, took 91 us, eight columns a thread with 1024 threads 80.
 constexpr int kLnBack = 16;
 constexpr int kLnBlock = 512;
 constexpr uint32_t kLnRing = 198656;
 constexpr int kLnMostDepth = 8;
 
-// the whole 16-byte pieces of a row of n values: values [first, last)
+// The 16-byte pieces that a row of n values touches, as far as they lie whole in its tensor: address, bytes (may be 0), and how far
+// behind the row's first piece they start
 template <typename T>
-__device__ __forceinline__ void whole_pieces(const T *row, int n, int &first, int &last)
+__device__ __forceinline__ const T *row_pieces(const T *tensor, int rows, size_t pitch, int n, int row, uint32_t &bytes, uint32_t &skip)
 {
-    const uintptr_t s = reinterpret_cast<uintptr_t>(row), e = s + (size_t)n * sizeof(T);
-    const uintptr_t lo = (s + 15) & ~(uintptr_t)15, hi = e & ~(uintptr_t)15;
-    if (hi > lo) { first = (int)((lo - s) / sizeof(T)); last = (int)((hi - s) / sizeof(T)); }
-    else { first = n; last = n; }
+    const uintptr_t first = reinterpret_cast<uintptr_t>(tensor), end = reinterpret_cast<uintptr_t>(tensor + (size_t)(rows - 1) * pitch + n);
+    const uintptr_t at = reinterpret_cast<uintptr_t>(tensor + (size_t)row * pitch), piece = at & ~(uintptr_t)15;
+    const uintptr_t lo = max(piece, (first + 15) & ~(uintptr_t)15), hi = min((at + (size_t)n * sizeof(T) + 15) & ~(uintptr_t)15, end & ~(uintptr_t)15);
+    bytes = hi > lo ? (uint32_t)(hi - lo) : 0u;
+    skip = (uint32_t)(lo - piece);
+    return reinterpret_cast<const T *>(lo);
+}
+// the values of a row before `head` and from `tail` on lie in pieces that reach out of the tensor
+template <typename T>
+__device__ __forceinline__ void row_edges(const T *tensor, int rows, size_t pitch, int n, int row, int &head, int &tail)
+{
+    asm volatile("" : "+l"(tensor));                        // (not worked out ahead for every row, in registers that spill)
+    const T *at = tensor + (size_t)row * pitch, *end = tensor + (size_t)(rows - 1) * pitch + n;
+    const uintptr_t lo = (reinterpret_cast<uintptr_t>(tensor) + 15) & ~(uintptr_t)15, hi = reinterpret_cast<uintptr_t>(end) & ~(uintptr_t)15;
+    const long long h = (long long)(lo - reinterpret_cast<uintptr_t>(at)) / (int)sizeof(T), l = (long long)(hi - reinterpret_cast<uintptr_t>(at)) / (int)sizeof(T);
+    head = (int)max(0ll, h);
+    tail = (int)min((long long)n, l);
 }
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar)
 {
@@ -503,56 +519,34 @@ __global__ void __launch_bounds__(kLnBlock, 1) ln_backward_rows_kernel(const __g
 
     const int step = (int)gridDim.x * kTeams;
     int row = (int)blockIdx.x * kTeams + team;
-    // one thread of the team: the whole pieces of a row into slot d
+    // one thread: the pieces of a row into slot d
     auto issue = [&](int at, int d) {
         const uint32_t bar = bar0 + 8u * d, dst = ptx::smem_u32(mine + (size_t)d * slot_bytes);
-        const T *dy = p.dy + (size_t)at * p.dy_pitch;
-        int f0, l0, f1 = 0, l1 = 0;
-        whole_pieces(dy, n, f0, l0);
-        const T *x = p.x + (size_t)at * p.x_pitch;
-        const uint32_t dy_size = (uint32_t)(l0 - f0) * (uint32_t)sizeof(T);
-        uint32_t x_size;
-        if (p.codes) {
-            x_size = (uint32_t)(p.blocks * kCkptBlock);
-        } else {
-            whole_pieces(x, n, f1, l1);
-            x_size = (uint32_t)(l1 - f1) * (uint32_t)sizeof(T);
+        const T *dy = p.dy + (size_t)at * p.dy_pitch, *x = p.x + (size_t)at * p.x_pitch;
+        uint32_t dy_size = (uint32_t)n * (uint32_t)sizeof(T), x_size = dy_size, dy_skip = 0, x_skip = 0;
+        if constexpr (V == 1) {
+            dy = row_pieces(p.dy, p.rows, p.dy_pitch, n, at, dy_size, dy_skip);
+            if (!p.codes) x = row_pieces(p.x, p.rows, p.x_pitch, n, at, x_size, x_skip);
         }
+        if (p.codes) x_size = (uint32_t)(p.blocks * kCkptBlock);
         ptx::mbar_arrive_expect_tx(bar, dy_size + x_size);
-        // a value lies in its slot at the row's own offset from a 16-byte boundary
-        if (dy_size) bulk_load(dst + (uint32_t)(reinterpret_cast<uintptr_t>(dy) & 15) + (uint32_t)f0 * (uint32_t)sizeof(T), dy + f0, dy_size, bar);
+        if (V > 1 || dy_size) bulk_load(dst + dy_skip, dy, dy_size, bar);
         if (p.codes) bulk_load(dst + p.dy_bytes, p.codes + (size_t)at * p.blocks * kCkptBlock, x_size, bar);
-        else if (x_size) bulk_load(dst + p.dy_bytes + (uint32_t)(reinterpret_cast<uintptr_t>(x) & 15) + (uint32_t)f1 * (uint32_t)sizeof(T), x + f1, x_size, bar);
+        else if (V > 1 || x_size) bulk_load(dst + p.dy_bytes + x_skip, x, x_size, bar);
     };
-    if (t == 0) {
-        for (int d = 0, at = row; d < depth && at < p.rows; d++, at += step) issue(at, d);
-    }
-    // What does not come by bulk copies, a row ahead: statistics, and of rows of single values the first seven and the last
-    // seven (this thread's column among the first, and the one among the last).
-    const T *dy_next = p.dy + (size_t)row * p.dy_pitch, *x_next = p.x + (size_t)row * p.x_pitch;
+    if (t < depth && row + (long long)t * step < p.rows) issue(row + t * step, t);
+    // what does not come by bulk copies, a row ahead: statistics, and the row's place in its slot
     T *dx_row = p.dx + (size_t)row * p.dx_pitch;
-    const size_t dy_step = (size_t)step * p.dy_pitch, x_step = (size_t)step * p.x_pitch, dx_step = (size_t)step * p.dx_pitch;
-    float next_mu = 0.f, next_r = 0.f, head_dy = 0.f, head_x = 0.f, tail_dy = 0.f, tail_x = 0.f;
-    uint32_t next_dy_at = 0, next_x_at = 0;                  // the next row's place in its slot
-    const int tail_k = V == 1 && t < n ? (n - 1 - t) / TEAM : -1, tail_column = tail_k * TEAM + t;
-    const bool has_head = V == 1 && t < 7 && t < n, has_tail = V == 1 && tail_k >= 0 && tail_column >= n - 7;
+    const size_t dx_step = (size_t)step * p.dx_pitch;
+    uint32_t next_dy_at = (uint32_t)(reinterpret_cast<uintptr_t>(p.dy + (size_t)row * p.dy_pitch) & 15);
+    uint32_t next_x_at = p.codes ? 0u : (uint32_t)(reinterpret_cast<uintptr_t>(p.x + (size_t)row * p.x_pitch) & 15);
+    const uint32_t dy_turn = (uint32_t)step * (uint32_t)p.dy_pitch * (uint32_t)sizeof(T), x_turn = p.codes ? 0u : (uint32_t)step * (uint32_t)p.x_pitch * (uint32_t)sizeof(T);
+    // the rows that may touch a piece that reaches out of the tensor, from its first row and from its last (16 bytes: eight values at most)
+    const int edge = V > 1 ? 0 : n >= 8 ? 1 : 8;
+    float next_mu = 0.f, next_r = 0.f;
     auto ahead = [&](int at) {
         next_r = p.rstd[at];
         if (p.mean) next_mu = p.mean[at];
-        if (V == 1) {
-            next_dy_at = (uint32_t)(reinterpret_cast<uintptr_t>(dy_next) & 15);
-            next_x_at = p.dy_bytes + (p.codes ? 0u : (uint32_t)(reinterpret_cast<uintptr_t>(x_next) & 15));
-            if (has_head) {
-                head_dy = to_float(dy_next[t]);
-                if (!p.codes) head_x = to_float(x_next[t]);
-            }
-            if (has_tail) {
-                tail_dy = to_float(dy_next[tail_column]);
-                if (!p.codes) tail_x = to_float(x_next[tail_column]);
-            }
-        }
-        dy_next += dy_step;
-        x_next += x_step;
     };
     // exponents: into a register two rows ahead, into shared memory one row ahead
     const bool has_exp = p.codes && t < (int)p.blocks;
@@ -596,8 +590,8 @@ __global__ void __launch_bounds__(kLnBlock, 1) ln_backward_rows_kernel(const __g
             }
         }
         const uint8_t *src = mine + (uint32_t)slot * slot_bytes;
-        const T *dy_in = reinterpret_cast<const T *>(src + next_dy_at);
-        const T *x_in = reinterpret_cast<const T *>(src + (V == 1 ? next_x_at : p.dy_bytes));
+        const T *dy_in = reinterpret_cast<const T *>(src + (V == 1 ? next_dy_at : 0u));
+        const T *x_in = reinterpret_cast<const T *>(src + p.dy_bytes + (V == 1 ? next_x_at : 0u));
         const int8_t *code_in = reinterpret_cast<const int8_t *>(src + p.dy_bytes);
         const float r = next_r, mu = next_mu;
         float dy[kLnBack], xh[kLnBack];
@@ -610,21 +604,31 @@ __global__ void __launch_bounds__(kLnBlock, 1) ln_backward_rows_kernel(const __g
                 const Pack<T, V> a = load_pack<T, V>(dy_in + col);
 #pragma unroll
                 for (int j = 0; j < V; j++) dy[k * V + j] = to_float(a.v[j]);
-                if (V == 1 && k == 0 && has_head) dy[0] = head_dy;
-                if (V == 1 && has_tail && k == tail_k) dy[k] = tail_dy;
                 if (p.codes) {
                     ckpt8_values<V>(xh + k * V, ckpt8_get<V>(code_in + col), exps[team][turn][col / kCkptBlock]);
                 } else {
                     const Pack<T, V> b = load_pack<T, V>(x_in + col);
 #pragma unroll
                     for (int j = 0; j < V; j++) xh[k * V + j] = to_float(b.v[j]);
-                    if (V == 1 && k == 0 && has_head) xh[0] = head_x;
-                    if (V == 1 && has_tail && k == tail_k) xh[k] = tail_x;
 #pragma unroll
                     for (int j = 0; j < V; j++) xh[k * V + j] = (xh[k * V + j] - mu) * r;
                 }
             }
         }
+        if (V == 1 && (row < edge || row >= p.rows - edge)) {
+            int head, tail, x_head = 0, x_tail = n;
+            row_edges(p.dy, p.rows, p.dy_pitch, n, row, head, tail);
+            if (!p.codes) row_edges(p.x, p.rows, p.x_pitch, n, row, x_head, x_tail);
+            const T *dy_at = p.dy + (size_t)row * p.dy_pitch + t, *x_at = p.x + (size_t)row * p.x_pitch + t;
+#pragma unroll
+            for (int k = 0; k < K; k++) {
+                const int col = k * TEAM + t;
+                if (in[k] && (col < head || col >= tail)) dy[k] = to_float(dy_at[k * TEAM]);
+                if (in[k] && (col < x_head || col >= x_tail)) xh[k] = (to_float(x_at[k * TEAM]) - mu) * r;
+            }
+        }
+        next_dy_at = (next_dy_at + dy_turn) & 15;
+        next_x_at = (next_x_at + x_turn) & 15;
         float2 g[kPairs], s1 = make_float2(0.f, 0.f), s2 = s1;
 #pragma unroll
         for (int i = 0; i < kPairs; i++) {

@@ -108,6 +108,46 @@ def test_backward_from_checkpoint(ops, rows, n, kind):
     cu.within(host(dbeta), want[2], edb + cu.U * np.abs(want[2]), "dbeta")
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("checkpoint", [False, True])
+@pytest.mark.parametrize("n", [1, 2, 3, 7, 9, 33, 517, 1021, 4099])
+def test_backward_at_the_ends_of_a_tensor(ops, n, kind, checkpoint):
+    """Rows whose first and last 16 bytes they share with other rows, or with what lies around the tensor: it is NaN and must
+    neither count nor change."""
+    t = getattr(torch, kind)
+
+    def around(x, start):
+        wide = torch.full((x.numel() + 32,), float("nan"), dtype=t, device="cuda")
+        inner = wide[start:start + x.numel()].view(x.shape)
+        inner.copy_(x)
+        return wide, inner
+
+    for rows in (1, 2, 9, 40):
+        x, dy, gamma, _ = make(rows, n, kind, 7)
+        mean, var = x.double().mean(1), x.double().var(1, correction=0)
+        rstd = (1 / (var + 1e-5).sqrt()).float()
+        mean = mean.float()
+        xh = (x.double() - mean.double()[:, None]) * rstd.double()[:, None]
+        c = None
+        if checkpoint:
+            c = ops.Checkpoint8.empty(rows, n).store(xh.float())
+            xh = c.load(torch.empty(rows, n, device="cuda")).double()
+        for start in (0, 1, 5, 8, 15):
+            wide_dy, in_dy = around(dy, start)
+            _, in_x = around(x, (3 * start + 1) % 16)
+            wide_dx, dx = around(torch.zeros_like(dy), start)
+            dg, db = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+            ops.ln_backward(in_dy, c if checkpoint else in_x, None if checkpoint else mean, rstd, gamma, dg, db, dx=dx)
+            ops.stream_status()
+            want, g, b = cu.ln_backward(host(dy), host(xh), host(rstd), host(gamma))
+            e, eg, eb = cu.ln_backward_bounds(host(dy), host(xh), host(rstd), host(gamma), kind)
+            cu.within(host(dx), want, e, "dx")
+            cu.within(host(dg), g, eg + cu.U * np.abs(g), "dgamma")
+            cu.within(host(db), b, eb + cu.U * np.abs(b), "dbeta")
+            outside = torch.isnan(wide_dx)
+            assert outside[:start].all() and outside[start + dx.numel():].all() and int(outside.sum()) == 32
+
+
 @pytest.mark.parametrize("n", [24, 1000, 8192, 40000])
 def test_pitched_rows_and_untouched_surroundings(ops, n):
     """Rows inside wider matrices, starting at odd elements: nothing outside the rows is read into the result or written."""
