@@ -8,6 +8,7 @@
 #pragma once
 #include <cuda_runtime.h>
 #include <cstdint>
+#include "types.cuh"
 
 namespace b200 {
 
@@ -90,10 +91,16 @@ template <int V> __device__ __forceinline__ void ckpt8_values(float *f, CkptCode
 {
     // the byte u = q + 128 under the exponent of 2^23 is the float 2^23 + u: no conversion instruction; the step may be subnormal
     const float step = ckpt8_unit(b) * 0.015625f;
+    auto byte = [&](int i) { return __uint_as_float(__byte_perm(c.w[i / 4] ^ 0x80808080u, 0x4b000000u, 0x7540 | (i & 3))); };
+    if constexpr (V == 1) {
+        f[0] = (byte(0) - 8388736.f) * step;
+    } else {
 #pragma unroll
-    for (int i = 0; i < V; i++) {
-        const uint32_t u = __byte_perm(c.w[i / 4] ^ 0x80808080u, 0x4b000000u, 0x7540 | (i & 3));
-        f[i] = (__uint_as_float(u) - 8388736.f) * step;
+        for (int i = 0; i < V; i += 2) {
+            const float2 v = mul2(add2(make_float2(byte(i), byte(i + 1)), make_float2(-8388736.f, -8388736.f)), make_float2(step, step));
+            f[i] = v.x;
+            f[i + 1] = v.y;
+        }
     }
 }
 
