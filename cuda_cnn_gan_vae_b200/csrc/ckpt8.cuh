@@ -32,8 +32,16 @@ template <int V> __device__ __forceinline__ void ckpt8_codes(uint32_t *q, const 
 {
     const float scale = __uint_as_float((260u - max(b, 6u)) << 23);            // 2^(133-b) for b = 6 .. 255
     if (b >= 6u && b < 254u) {
+        if constexpr (V == 1) {
+            q[0] = __float_as_uint(fmaf(x[0], scale, 12582912.f));
+        } else {
 #pragma unroll
-        for (int i = 0; i < V; i++) q[i] = __float_as_uint(fmaf(x[i], scale, 12582912.f));
+            for (int i = 0; i < V; i += 2) {
+                const float2 v = fma2(make_float2(x[i], x[i + 1]), make_float2(scale, scale), make_float2(12582912.f, 12582912.f));
+                q[i] = __float_as_uint(v.x);
+                q[i + 1] = __float_as_uint(v.y);
+            }
+        }
     } else {
         const float more = __uint_as_float((127u + max(b, 6u) - b) << 23);     // 2^(6-b) below 6, else 1
 #pragma unroll
@@ -50,16 +58,28 @@ template <int V> __device__ __forceinline__ void ckpt8_codes(uint32_t *q, const 
 __device__ __forceinline__ float ckpt8_unit(uint32_t b) { return __uint_as_float(b << 23); }
 __device__ __forceinline__ float ckpt8_value(int q, float unit) { return ((float)q * 0.015625f) * unit; }
 
+// The largest of three magnitudes; a NaN if one of them is
+__device__ __forceinline__ float largest(float a, float b, float c)
+{
+    float d;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
 // A group of lanes that hold V neighbouring values each shares a block: its largest magnitude.
 template <int V> __device__ __forceinline__ uint32_t ckpt8_top(const float *f)
 {
-    uint32_t top = 0;
+    if constexpr (V == 1) {
+        return __reduce_max_sync(0xffffffffu, __float_as_uint(f[0]) & 0x7fffffffu);
+    } else {
+        float most = largest(f[0], f[1], f[2]);
 #pragma unroll
-    for (int i = 0; i < V; i++) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
-    if constexpr (V == 1) return __reduce_max_sync(0xffffffffu, top);
+        for (int i = 3; i < V; i += 2) most = largest(most, f[i], i + 1 < V ? f[i + 1] : 0.f);
+        uint32_t top = __float_as_uint(most);
 #pragma unroll
-    for (int o = 1; o < kCkptBlock / V; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    return top;
+        for (int o = 1; o < kCkptBlock / V; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        return top;
+    }
 }
 
 // codes of V values at dst (a multiple of V bytes), and the values of V codes

@@ -70,19 +70,20 @@ __global__ void __launch_bounds__(256) ckpt8_wgrad_simt_kernel(float *dweight, f
 //     (bf16 1, fp16 2, fp32 3, in either tensor-core mode), each exact, so every product is exact and the only roundings are
 //     those of the fp32 accumulator.  The tensor core truncates its sums, a bias that grows with their number: after kChunk
 //     stages the accumulator is added to the output (rounded to nearest) and starts again from zero.  8192 rows at a stretch
-//     were off by 2.5e-6 of the result, chunks of 2048 are by 4e-7, for 22 of 261 us.
+//     were off by 2.5e-6 of the result, chunks of 2048 are by 4e-7, for 22 of 264 us.
 //   * One warp each brings the codes and delta in by TMA (bf16 straight into the operand tile); four groups of four warps decode
 //     and split from shared memory into a ring of operand stages (five instructions for two values, once per pair and tile).
 //     A group takes every fourth stage, so four stages are in work at a time: with all sixteen warps on each stage its chain of
 //     waits, loads and stores was in series with the next one's.  Stages are as long as the rings allow (bf16 with 32 rows
-//     in place of 64: 350 us for 261; fp16 with 16 for 32: 652 for 495), because a stage's waits, exponents and fences cost a
+//     in place of 64: 350 us for 264; fp16 with 16 for 32: 652 for 495), because a stage's waits, exponents and fences cost a
 //     group some hundred instructions whatever its length.
 //   * The grid is one pair per two SMs.  Whole tiles go round the pairs; what is left over (or everything, where there are
 //     fewer tiles than pairs) is split along the batch into units that write partial tiles, joined by a second
 //     kernel in the order of the units.  No atomics: the result does not depend on scheduling.
-// Measured at 8192 rows, 4096 x 4096: bf16 261 us = 1.05 PFLOP/s (303 us with inputs that are not in L2), fp16 495, fp32 782; the
-// tensor pipe is active half the time in bf16, the converter warps issue in 60 % of the cycles, and without their stores
-// (199 us) or without the products (199 us) it is no faster than shared memory and the two together allow.
+// Measured at 8192 rows, 4096 x 4096, inputs from memory: bf16 264 us = 1.04 PFLOP/s (302 us after a second of nothing else, when the
+// power limit holds the clock at 1.55 GHz; L2 prefetches ahead of the loads changed nothing), fp16 497, fp32 782; the tensor pipe
+// is active half the time in bf16, the converter warps issue in 60 % of the cycles, and without their stores (199 us) or without the
+// products (199 us) it is no faster than shared memory and the two together allow.
 constexpr int kPairTile = 256;                     // outputs of a pair in both directions
 constexpr int kEpilogueWarps = 4, kConverterWarps = 16, kGroupWarps = 4, kGroups = kConverterWarps / kGroupWarps;
 constexpr int kConverters = kConverterWarps * 32;

@@ -91,6 +91,34 @@ __device__ __forceinline__ void load_params(float *f, const float *p, size_t col
 #pragma unroll
     for (int i = 0; i < V; i++) f[i] = __ldg(p + col + i);
 }
+
+// (x - mu) r and xh gamma + beta of V values, in pairs
+template <int V> __device__ __forceinline__ void normalise(float *xh, const float *x, float mu, float r)
+{
+    if constexpr (V == 1) {
+        xh[0] = (x[0] - mu) * r;
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; j += 2) {
+            const float2 h = mul2(add2(make_float2(x[j], x[j + 1]), make_float2(-mu, -mu)), make_float2(r, r));
+            xh[j] = h.x;
+            xh[j + 1] = h.y;
+        }
+    }
+}
+template <int V> __device__ __forceinline__ void affine(float *y, const float *xh, const float *gamma, const float *beta)
+{
+    if constexpr (V == 1) {
+        y[0] = fmaf(xh[0], gamma[0], beta[0]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; j += 2) {
+            const float2 v = fma2(make_float2(xh[j], xh[j + 1]), make_float2(gamma[j], gamma[j + 1]), make_float2(beta[j], beta[j + 1]));
+            y[j] = v.x;
+            y[j + 1] = v.y;
+        }
+    }
+}
 inline bool wide_params(const void *a, const void *b) { return !((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15); }
 
 // ---- forward -----------------------------------------------------------------------------------------------------------------
@@ -134,8 +162,7 @@ __device__ __forceinline__ void ln_put(const LnForward<T> &p, const LnOut<T> &ou
         float y[V], gamma[V], beta[V];
         load_params<V>(gamma, p.gamma, col, p.wide);
         load_params<V>(beta, p.beta, col, p.wide);
-#pragma unroll
-        for (int j = 0; j < V; j++) y[j] = fmaf(xh[j], gamma[j], beta[j]);
+        affine<V>(y, xh, gamma, beta);
         store_pack<T, V>(out.y + col, y);
     }
 }
@@ -309,17 +336,19 @@ __global__ void __launch_bounds__(kLnSlice) ln_normalise_kernel(const __grid_con
 #pragma unroll
         for (int u = 0; u < U; u++) {
             if (row + u >= end) break;
-            float xh[V], y[V];
+            float xh[V] = {}, y[V];
+            if (in) {
 #pragma unroll
-            for (int j = 0; j < V; j++) xh[j] = in ? (to_float(raw[u].v[j]) - mu[u]) * r[u] : 0.f;
+                for (int j = 0; j < V; j++) y[j] = to_float(raw[u].v[j]);
+                normalise<V>(xh, y, mu[u], r[u]);
+            }
             if (p.codes) {
                 const uint32_t b = ckpt8_exponent(ckpt8_top<V>(xh));
                 if (in_block) ckpt8_put<V>(p.codes + (size_t)(row + u) * blocks * kCkptBlock + col, xh, b, false);
                 if (opens_block) p.exponents[(size_t)(row + u) * blocks + col / kCkptBlock] = (uint8_t)b;
             }
             if (in) {
-#pragma unroll
-                for (int j = 0; j < V; j++) y[j] = fmaf(xh[j], gamma[j], beta[j]);
+                affine<V>(y, xh, gamma, beta);
                 store_pack<T, V>(p.y + (size_t)(row + u) * p.y_pitch + col, y);
             }
         }
@@ -434,7 +463,8 @@ __device__ __forceinline__ void ln_values(const LnBackward<T> &p, const LnRaw<T,
 // of the others (at most seven at either end of the tensor) are loaded by their threads.  (With each row's own whole pieces copied
 // and its first and last values loaded a row ahead, 5003 x 1021 fp16 took 22.5 us.)
 // Measured at 16384 x 2048 bf16 with the rows kept in 8 bits: 47 us, 3.6 TB/s, half the cycles issue (sixteen warps an SM wait for
-// one another at a row's barrier); loads into registers, two blocks an SM, took 91 us, eight columns a thread with 1024 threads 80.
+// one another at a row's barrier); loads into registers, two blocks an SM, took 91 us, eight columns a thread with 1024 threads 80.  With the
+// next row's sums formed before this row's are waited for, and the values formed again after it, 56.
 constexpr int kLnBack = 16;
 constexpr int kLnBlock = 512;
 constexpr uint32_t kLnRing = 198656;
