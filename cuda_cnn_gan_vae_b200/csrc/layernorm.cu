@@ -728,15 +728,17 @@ __global__ void __launch_bounds__(kLnBlock, 1) ln_backward_rows_kernel(const __g
     cluster.sync();                                         // no block leaves while another still reads its sums
 }
 
-// Longer rows in two passes.  First: a thread owns V columns (four times one, where rows are not read in 16-byte pieces) and walks a
+// Longer rows in two passes.  First: a thread owns four columns (four single ones, where rows are not read in pieces) and walks a
 // group of rows; it sums dgamma and dbeta of its columns, and its warp writes the partial sums of g and g xh of each row.
 // Then a small kernel joins both kinds of sums, and the second pass, again a thread on its columns down a group of rows, forms
-// dx.  (With the rows' sums joined by every block of the second pass, 300 x 40001 fp16 took 71 us.)
+// dx.  512 x 16384 bf16: 33 us; with eight columns a thread and eight rows under way (140 registers) it took 49, with twice the groups
+// 36.  (With the rows' sums joined by every block of the second pass, 300 x 40001 fp16 took 71 us, now 43.)
 template <int V> constexpr int kLnRuns = V == 1 ? 4 : 1;      // runs of V columns of a thread, a slice apart
+template <int V> constexpr int kLnLong = V == 1 ? 1 : 4;
 template <typename T, int V>
 __global__ void __launch_bounds__(kLnSlice) ln_backward_columns_kernel(const __grid_constant__ LnBackward<T> p)
 {
-    constexpr int C = kLnRuns<V>, U = 4 / C > 0 ? 4 / C : 1;   // rows under way
+    constexpr int C = kLnRuns<V>, U = V == 1 ? 1 : 2;          // rows under way
     grid_dependency_wait();
     const uint32_t first = (blockIdx.x * C * kLnSlice + threadIdx.x) * V, n = (uint32_t)p.n;
     const int piece = (int)(blockIdx.x * (kLnSlice / 32) + (threadIdx.x >> 5)), lane = threadIdx.x & 31;
@@ -751,7 +753,7 @@ __global__ void __launch_bounds__(kLnSlice) ln_backward_columns_kernel(const __g
         if (in[c]) load_params<V>(gamma[c], p.gamma, col, p.wide);
     }
     const int begin = (int)((long long)p.rows * blockIdx.y / p.groups), end = (int)((long long)p.rows * (blockIdx.y + 1) / p.groups);
-#pragma unroll 2
+#pragma unroll(V == 1 ? 2 : 1)
     for (int row = begin; row < end; row += U) {
         LnRaw<T, V> raw[U][C];
 #pragma unroll
@@ -798,7 +800,7 @@ __global__ void __launch_bounds__(kLnSlice) ln_backward_columns_kernel(const __g
 template <typename T, int V>
 __global__ void __launch_bounds__(kLnSlice) ln_backward_apply_kernel(const __grid_constant__ LnBackward<T> p)
 {
-    constexpr int C = kLnRuns<V>, U = 4 / C > 0 ? 4 / C : 1;
+    constexpr int C = kLnRuns<V>, U = V == 1 ? 1 : 2;
     grid_dependency_wait();
     const uint32_t first = (blockIdx.x * C * kLnSlice + threadIdx.x) * V, n = (uint32_t)p.n;
     bool in[C];
@@ -809,7 +811,7 @@ __global__ void __launch_bounds__(kLnSlice) ln_backward_apply_kernel(const __gri
         if (in[c]) load_params<V>(gamma[c], p.gamma, first + c * kLnSlice * V, p.wide);
     }
     const int begin = (int)((long long)p.rows * blockIdx.y / p.groups), end = (int)((long long)p.rows * (blockIdx.y + 1) / p.groups);
-#pragma unroll 2
+#pragma unroll(V == 1 ? 2 : 1)
     for (int row = begin; row < end; row += U) {
         LnRaw<T, V> raw[U][C];
 #pragma unroll
@@ -896,8 +898,9 @@ static LnPlan ln_plan(int rows, size_t n, int v)
     } else {
         const size_t slice = (size_t)kLnSlice * (v == 1 ? kLnRuns<1> : kLnRuns<4> * v), slices = (n + slice - 1) / slice;
         w.pieces = (int)slices * (kLnSlice / 32);
-        // about sixteen blocks of 128 threads per SM, and eight rows each at least
-        const long long want = ((long long)sm_count() * 16 + (long long)slices - 1) / (long long)slices;
+        // about eight blocks of 128 threads per SM (sixteen where single values need more loads under way), and eight rows each at
+        // least: a group's partial sums are written and read once more
+        const long long want = ((long long)sm_count() * (v == 1 ? 16 : 8) + (long long)slices - 1) / (long long)slices;
         w.groups = (int)max(1ll, min(want, (long long)(rows + 7) / 8));
     }
     return w;
@@ -908,7 +911,8 @@ static size_t row_bytes(const LnPlan &w, int rows) { return w.one_pass ? 0 : ali
 template <typename T, int V>
 static int ln_backward_launch(LnBackward<T> p, float *dgamma, float *dbeta, int accumulate, char *workspace, cudaStream_t s)
 {
-    const LnPlan w = ln_plan(p.rows, p.n, V);
+    constexpr int kLong = kLnLong<V>;
+    const LnPlan w = ln_plan(p.rows, p.n, kLong);
     p.groups = w.groups;
     p.pieces = w.pieces;
     p.row_part = reinterpret_cast<float2 *>(workspace);
@@ -944,7 +948,7 @@ static int ln_backward_launch(LnBackward<T> p, float *dgamma, float *dbeta, int 
         B200_LAUNCH_CHECK();
         if (w.one_cluster) return B200_OK;
     } else {
-        Launch(dim3((unsigned)(w.pieces / (kLnSlice / 32)), (unsigned)w.groups), kLnSlice, 0, s)(ln_backward_columns_kernel<T, V>, p);
+        Launch(dim3((unsigned)(w.pieces / (kLnSlice / 32)), (unsigned)w.groups), kLnSlice, 0, s)(ln_backward_columns_kernel<T, kLong>, p);
         B200_LAUNCH_CHECK();
     }
     const LnRows rows = {p.row_part, p.row_mean, w.one_pass ? 0 : p.rows, w.pieces};
@@ -959,7 +963,7 @@ static int ln_backward_launch(LnBackward<T> p, float *dgamma, float *dbeta, int 
         B200_LAUNCH_CHECK();
     }
     if (!w.one_pass) {
-        Launch(dim3((unsigned)(w.pieces / (kLnSlice / 32)), (unsigned)w.groups), kLnSlice, 0, s)(ln_backward_apply_kernel<T, V>, p);
+        Launch(dim3((unsigned)(w.pieces / (kLnSlice / 32)), (unsigned)w.groups), kLnSlice, 0, s)(ln_backward_apply_kernel<T, kLong>, p);
         B200_LAUNCH_CHECK();
     }
     return B200_OK;
@@ -1000,7 +1004,7 @@ size_t b200_ln_backward_workspace(int rows, size_t n)
     if (check_rows(rows, n) || rows == 0) return 0;
     // enough for either width of the loads
     size_t most = 0;
-    for (int v = 1; v <= 8; v *= v == 1 ? 4 : 2) {
+    for (int v : {kLnLong<1>, kLnLong<4>}) {
         const LnPlan w = ln_plan(rows, n, v);
         const size_t bytes = row_bytes(w, rows) + sizeof(float) * 2 * n * (size_t)w.groups;
         most = bytes > most ? bytes : most;

@@ -52,12 +52,13 @@ __device__ __forceinline__ uint32_t from_float2(float2 v, __half)
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-// V neighbouring values (V = 1, or the number in 16 bytes: the address is then a multiple of 16)
-template <typename T, int V> struct alignas(V == 1 ? sizeof(T) : 16) Pack { T v[V]; };
+// V neighbouring values: one, or 8 or 16 bytes of them at a multiple of that
+template <typename T, int V> struct alignas(V * sizeof(T)) Pack { T v[V]; };
 template <typename T, int V> __device__ __forceinline__ Pack<T, V> load_pack(const T *p)
 {
     Pack<T, V> r;
     if constexpr (V == 1) r.v[0] = *p;
+    else if constexpr (V * sizeof(T) == 8) *reinterpret_cast<uint2 *>(r.v) = *reinterpret_cast<const uint2 *>(p);
     else *reinterpret_cast<uint4 *>(r.v) = *reinterpret_cast<const uint4 *>(p);
     return r;
 }
@@ -68,10 +69,11 @@ template <typename T, int V> __device__ __forceinline__ void store_pack(T *p, co
     } else if constexpr (sizeof(T) == 4) {
         *reinterpret_cast<float4 *>(p) = make_float4(f[0], f[1], f[2], f[3]);
     } else {
-        uint32_t w[4];
+        uint32_t w[V / 2];
 #pragma unroll
-        for (int i = 0; i < 4; i++) w[i] = from_float2(make_float2(f[2 * i], f[2 * i + 1]), T());
-        *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+        for (int i = 0; i < V / 2; i++) w[i] = from_float2(make_float2(f[2 * i], f[2 * i + 1]), T());
+        if constexpr (V == 4) *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
+        else *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
     }
 }
 template <typename T> constexpr int kWide = 16 / (int)sizeof(T);
