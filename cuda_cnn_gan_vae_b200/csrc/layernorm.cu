@@ -232,8 +232,9 @@ struct Moments { float count, mean, q; };
 __device__ __forceinline__ Moments join(Moments a, Moments b)
 {
     const float count = a.count + b.count, part = count > 0.f ? b.count / count : 0.f, d = b.mean - a.mean;
-    // (the mean of a row with an infinity is that infinity, on whichever side of the pair it is)
-    return {count, isfinite(d) ? fmaf(d, part, a.mean) : a.mean + b.mean, a.q + b.q + d * d * a.count * part};
+    // (the mean of a row with an infinity is that infinity, on whichever side of the pair it is).  The counts come before the second
+    // d: beside an empty side, where d is the other side's whole mean, the term is 0 times d and not infinity times 0.
+    return {count, isfinite(d) ? fmaf(d, part, a.mean) : a.mean + b.mean, a.q + b.q + d * (a.count * part) * d};
 }
 __device__ __forceinline__ Moments warp_join(Moments m)
 {

@@ -332,3 +332,31 @@ def test_an_infinity_in_a_row_is_its_mean(ops, n):
     mean = got["mean"].cpu()
     assert mean[1] == float("inf") and mean[2] == float("-inf") and torch.isnan(mean[3]) and torch.isfinite(mean[[0, 4]]).all()
     assert torch.isnan(got["y"][1:4]).all() and torch.isfinite(got["y"][[0, 4]]).all()
+
+
+@pytest.mark.parametrize("kind", ["float32", "bfloat16"])
+@pytest.mark.parametrize("n", [9000, 20000, 131072])
+def test_large_magnitudes(ops, n, kind):
+    """Means whose square leaves fp32 and deviations whose square does not.  Constant rows of 2^66: every sum of up to 32 of them is exact,
+    so is every mean, and the deviation is 0.  Alternating rows m (1 +- 2^-7), both exact in bf16: m^2 times a count of values is beyond
+    fp32 (2^120 at least, times thousands), the sum of squared deviations is not (2^108 times 2^17 at most); compared with the
+    formula, to the bounds of the other sizes."""
+    t = getattr(torch, kind)
+    gamma, beta = make(1, n, kind, 13)[2:]
+    x = torch.full((2, n), 2.0 ** 66, dtype=t, device="cuda")
+    x[1] = -x[1]
+    got = ops.ln_forward(x, gamma, beta, 1e-5)
+    ops.stream_status()
+    assert torch.equal(got["mean"], x[:, 0].float())
+    assert torch.equal(got["y"], beta.to(t).expand(2, n))
+    np.testing.assert_allclose(host(got["rstd"]), float(np.float32(1e-5)) ** -0.5, rtol=3 * cu.U)
+    sign = torch.where(torch.arange(n, device="cuda") % 2 == 0, 1.0, -1.0)
+    x = torch.stack([2.0 ** 61 * (1 + sign * 2.0 ** -7), -(2.0 ** 60) * (1 + sign * 2.0 ** -7)]).to(t)
+    args = (host(x), host(gamma), host(beta), float(np.float32(1e-5)))
+    got = ops.ln_forward(x, gamma, beta, 1e-5)
+    ops.stream_status()
+    y, mu, r, _ = cu.ln_forward(*args)
+    ey, em, er, _ = cu.ln_forward_bounds(*args, kind)
+    cu.within(host(got["mean"]), mu, em, "mean")
+    cu.within(host(got["rstd"]), r, er, "rstd")
+    cu.within(host(got["y"]), y, ey, "y")
