@@ -104,6 +104,8 @@ __global__ void __launch_bounds__(256) ckpt8_load_kernel(T *out, const int8_t *_
             for (int j = 0; j < V; j++) {
                 if (FUNC < 0) f[j] = ckpt8_clip<T>(f[j]);
                 else f[j] = act_derivative(f[j], FUNC, slope) * to_float(e[k].v[j]);
+                // a NaN is not above zero: without this the finite neighbours of an infinity would pass for negative values
+                if ((FUNC == B200_ACT_RELU || FUNC == B200_ACT_LEAKY_RELU) && b[k] == 255u) f[j] = __int_as_float(0x7fffffff);
             }
             store_pack<T, V>(out + row[k] * g.pitch + col[k], f);
         }

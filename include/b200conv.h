@@ -356,13 +356,15 @@ int b200_ln_backward(void *dx, float *dgamma, float *dbeta, const void *dy, cons
  * (at least 1), one more where that value would round to 128 (not past 254, where it saturates at 127); q is rounded to
  * nearest, ties to even.  A value is off by at most half a step, 1/127 of the largest magnitude of its block (a whole step where
  * it saturates).  A block that holds an infinity or a NaN reads as NaN.  keep_sign != 0: a negative value never gets q = 0
- * but -1 (off by less than a step), so that the derivatives of ReLU and LeakyReLU at the kept values are those at the tensor's. */
+ * but -1 (off by less than a step), so that the derivatives of ReLU and LeakyReLU at the kept values are those at the tensor's
+ * in every block of finite values. */
 int b200_ckpt8_store(int8_t *codes, uint8_t *exponents, const void *x, int type, int rows, size_t n, size_t x_pitch, int keep_sign,
                      void *stream);
 /* Reads the values back (exact in fp32 and bf16; in fp16 rounded once, beyond its range the largest finite number). */
 int b200_ckpt8_load(void *out, const int8_t *codes, const uint8_t *exponents, int type, int rows, size_t n, size_t out_pitch,
                     void *stream);
-/* b200_activation_backward for a function layer whose input was kept in 8 bits: out = f'(value) * error.  out may be error. */
+/* b200_activation_backward for a function layer whose input was kept in 8 bits: out = f'(value) * error.  out may be error.  In a
+ * block that reads as NaN out is NaN, whatever the function, except for B200_ACT_LINEAR (whose derivative is 1 everywhere). */
 int b200_ckpt8_activation_backward(void *out, const int8_t *codes, const uint8_t *exponents, const void *error, int type, int rows,
                                    size_t n, size_t out_pitch, size_t error_pitch, int func, double leaky_slope, void *stream);
 /* Gradients of a Linear layer (netlayer/cnetlayerlinear.cu.h:415) whose input [rows][in] was kept in 8 bits:

@@ -149,6 +149,28 @@ def test_kept_signs_make_relu_exact(ops):
         assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("func", FUNCTIONS)
+@pytest.mark.parametrize("n", [200, 203])
+def test_function_backward_of_blocks_without_values(ops, n, func, kind):
+    """A block that held an infinity or a NaN is NaN in the error below: its finite values are lost, and none of them may pass for a
+    negative one.  Only the linear function needs no value.  Other blocks are as ever."""
+    x = torch.from_numpy(np.random.default_rng(n).normal(0, 1, (3, n)).astype(np.float32)).cuda()
+    good = ops.Checkpoint8.empty(3, n).store(x, keep_sign=True)
+    x[0, 40], x[1, n - 1], x[2, 64] = float("inf"), float("nan"), float("-inf")
+    bad = ops.Checkpoint8.empty(3, n).store(x, keep_sign=True)
+    e = torch.ones(3, n, device="cuda").to(getattr(torch, kind))
+    got, want = torch.empty_like(e), torch.empty_like(e)
+    ops.CTensorApplyFunc.Backward(got, bad, e, func, 0.2)
+    ops.CTensorApplyFunc.Backward(want, good, e, func, 0.2)
+    ops.stream_status()
+    lost = torch.zeros(3, n, dtype=torch.bool, device="cuda")
+    if func != "linear":
+        lost[0, 32:64] = lost[1, 192:] = lost[2, 64:96] = True
+    assert torch.equal(torch.isnan(got), lost)
+    assert torch.equal(got[~lost], want[~lost])
+
+
 WGRAD = [(1, 1, 1), (1, 40, 3), (2, 33, 64), (31, 100, 129), (64, 100, 8192), (128, 16384, 256), (200, 1000, 130), (333, 257, 65), (1000, 64, 64),
          (5000, 300, 70), (8192, 512, 384), (257, 31, 1)]
 
