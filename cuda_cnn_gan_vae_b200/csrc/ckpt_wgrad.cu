@@ -11,7 +11,8 @@ namespace b200 {
 
 constexpr int kTile = 64, kDepth = 16;
 
-// 64 x 64 outputs per block of 256 threads, 4 x 4 per thread, the checkpoint decoded while a slice of 16 rows is staged
+// 64 x 64 outputs per block of 256 threads, 4 x 4 per thread, the checkpoint decoded while a slice of 16 rows is staged.  The blocks
+// are numbered along the inputs first, in one dimension: the grid's second one ends at 65535, 4 194 240 outputs.
 template <typename T>
 __global__ void __launch_bounds__(256) ckpt8_wgrad_simt_kernel(float *dweight, float *dbias, const T *__restrict__ delta, const int8_t *__restrict__ codes,
                                                                const uint8_t *__restrict__ exponents, int rows, int out, size_t in, size_t pitch, size_t blocks,
@@ -19,8 +20,9 @@ __global__ void __launch_bounds__(256) ckpt8_wgrad_simt_kernel(float *dweight, f
 {
     __shared__ float a[kDepth][kTile], b[kDepth][kTile];
     grid_dependency_wait();
-    const size_t i0 = (size_t)blockIdx.x * kTile;
-    const int o0 = (int)blockIdx.y * kTile;
+    const uint32_t tiles_in = (uint32_t)((in + kTile - 1) / kTile), tile_out = blockIdx.x / tiles_in;
+    const size_t i0 = (size_t)(blockIdx.x - tile_out * tiles_in) * kTile;
+    const int o0 = (int)tile_out * kTile;
     const int ti = threadIdx.x & 15, to = threadIdx.x >> 4;
     float acc[4][4] = {}, bias[4] = {};
     for (int r0 = 0; r0 < rows; r0 += kDepth) {
@@ -50,7 +52,7 @@ __global__ void __launch_bounds__(256) ckpt8_wgrad_simt_kernel(float *dweight, f
     for (int x = 0; x < 4; x++) {
         const int o = o0 + to * 4 + x;
         if (o >= out) break;
-        if (dbias && blockIdx.x == 0 && ti == 0) dbias[o] = accumulate ? dbias[o] + bias[x] : bias[x];
+        if (dbias && i0 == 0 && ti == 0) dbias[o] = accumulate ? dbias[o] + bias[x] : bias[x];
 #pragma unroll
         for (int y = 0; y < 4; y++) {
             const size_t i = i0 + ti * 4 + y;
@@ -760,7 +762,9 @@ int b200_ckpt8_wgrad(float *dweight, float *dbias, int accumulate, const void *d
         return wgrad_tc_launch<float, 3>(p, w, delta, delta_pitch, codes, type, fits, ST(stream));
     }
     // B200_FP32: fp32 products on the CUDA cores, summed row by row
-    const Launch launch(dim3((unsigned)((in + kTile - 1) / kTile), (unsigned)ceil_div(out, kTile)), 256, 0, ST(stream));
+    const size_t tiles = ((in + kTile - 1) / kTile) * (((size_t)out + kTile - 1) / kTile);
+    if (tiles > 0x7fffffffu) return fail(B200_E_SHAPE, "%zu tiles of the weight gradient are more than a grid has blocks", tiles);
+    const Launch launch((unsigned)tiles, 256, 0, ST(stream));
     if (type == B200_F32) launch(ckpt8_wgrad_simt_kernel<float>, dweight, dbias, (const float *)delta, codes, exponents, rows, out, in, delta_pitch, blocks, accumulate);
     else if (type == B200_BF16) launch(ckpt8_wgrad_simt_kernel<__nv_bfloat16>, dweight, dbias, (const __nv_bfloat16 *)delta, codes, exponents, rows, out, in, delta_pitch, blocks, accumulate);
     else launch(ckpt8_wgrad_simt_kernel<__half>, dweight, dbias, (const __half *)delta, codes, exponents, rows, out, in, delta_pitch, blocks, accumulate);

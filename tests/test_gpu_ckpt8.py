@@ -309,3 +309,22 @@ def test_wgrad_repeats_bit_for_bit(ops, kind, rows, n, out):
         first = first or (dw, db)
         assert i % 20 or (torch.equal(dw, first[0]) and torch.equal(db, first[1]))
     ops.stream_status()
+
+
+@pytest.mark.parametrize("mode", ["TF32X3", "FP32"])
+@pytest.mark.parametrize("n,out", [(2, 4194304 + 131), (4194304 + 70, 2)])
+def test_wgrad_of_very_many_outputs(ops, n, out, mode):
+    """More than 65535 tiles of 64 in either direction, in both forms of the product.  Whole numbers: every sum is exact."""
+    ops.set_precision(getattr(ops, mode))
+    try:
+        rows = 3
+        x = torch.randint(-7, 8, (rows, n), device="cuda").float()
+        delta = torch.randint(-7, 8, (rows, out), device="cuda").float()
+        c = ops.Checkpoint8.empty(rows, n).store(x)
+        dw, db = torch.full((out, n), 5.0, device="cuda"), torch.full((out,), 5.0, device="cuda")
+        ops.checkpoint_wgrad(dw, db, delta, c)
+        ops.stream_status()
+        assert torch.equal(dw.double(), 5 + delta.double().t() @ x.double())
+        assert torch.equal(db.double(), 5 + delta.double().sum(0))
+    finally:
+        ops.set_precision(ops.TF32X3)
