@@ -41,7 +41,13 @@ bool dependent_launch_enabled()
     return on;
 }
 static thread_local cudaError_t g_launch_error = cudaSuccess;
-void note_launch_error(cudaError_t e) { if (g_launch_error == cudaSuccess) g_launch_error = e; }
+// A refused launch is reported by the call it was part of: the runtime's own note of it is cleared here, or the next call would
+// find it and fail too.
+void note_launch_error(cudaError_t e)
+{
+    (void)cudaGetLastError();
+    if (g_launch_error == cudaSuccess) g_launch_error = e;
+}
 cudaError_t take_launch_error()
 {
     const cudaError_t e = g_launch_error;
