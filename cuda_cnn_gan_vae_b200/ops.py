@@ -76,6 +76,7 @@ _device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _F32 = torch.float32
+_MOST_ROWS = (1 << 31) - 65536       # rows, and values in a row (b200conv.h)
 
 
 # The calls below take a few microseconds, most of them spent here: each looks the device up once and hands it on.
@@ -89,14 +90,20 @@ def _rows(x, name, dev):
     if x.get_device() != dev:
         raise B200Error(2, f"{name} is on {x.device}, the current device is cuda:{dev}")
     shape = x.shape
+    if shape and shape[0] > _MOST_ROWS:
+        raise B200Error(1, f"{name} has {shape[0]} rows, {_MOST_ROWS} at most")      # (a C int would keep the lower 32 bits)
     if len(shape) == 2 and shape[1]:
         rows, n = shape
+        if n > _MOST_ROWS:
+            raise B200Error(1, f"{name} has rows of {n} values, {_MOST_ROWS} at most")
         pitch, inner = x.stride()
         if (inner == 1 or n == 1) and (pitch >= n or rows <= 1):
             return kind, rows, n, pitch if pitch > n else n
     if not shape or not x.is_contiguous():
         raise B200Error(2, f"{name} must be contiguous, or a matrix of contiguous rows")
     n = torch.Size(shape[1:]).numel()
+    if n > _MOST_ROWS:
+        raise B200Error(1, f"{name} has rows of {n} values, {_MOST_ROWS} at most")
     return kind, shape[0], n, n
 
 

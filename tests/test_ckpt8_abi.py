@@ -78,3 +78,27 @@ def test_the_restated_format_keeps_its_promises():
     assert ((kept < 0) == (x < 0)).all()
     torch = pytest.importorskip("torch")
     assert np.array_equal(torch.from_numpy(v).bfloat16().double().numpy(), v)
+
+
+@pytest.mark.parametrize("shape", [(2 ** 32 + 5, 1), (2 ** 32 + 4, 1, 1), (2 ** 31 - 65535, 2), (3, 2 ** 32 + 64), (3, 2 ** 16, 2 ** 16 + 1)])
+def test_sizes_beyond_the_interface_are_refused_and_not_cut_to_32_bits(monkeypatch, shape):
+    """Tensors without memory (nothing may look at their data): more rows, or longer ones, than the library takes."""
+    torch = pytest.importorskip("torch")
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from cuda_cnn_gan_vae_b200 import ops
+    monkeypatch.setattr(ops, "_device", lambda: 0)
+    with FakeTensorMode():
+        x = torch.empty(shape, device="cuda", dtype=torch.bfloat16)
+        n = x[0].numel()
+        blocks = -(-n // 32)
+        gamma = torch.empty(n, device="cuda")
+        kept = ops.Checkpoint8(torch.empty(shape[0], 32 * blocks, dtype=torch.int8, device="cuda"),
+                               torch.empty(shape[0], blocks, dtype=torch.uint8, device="cuda"), n)
+        stat = torch.empty(shape[0], device="cuda")
+        dw, db = torch.empty(n, 8, device="cuda"), torch.empty(n, device="cuda")
+        short = ops.Checkpoint8(torch.empty(shape[0], 32, dtype=torch.int8, device="cuda"), torch.empty(shape[0], 1, dtype=torch.uint8, device="cuda"), 8)
+        for call in (lambda: kept.store(x), lambda: kept.load(x), lambda: ops.ln_forward(x, gamma, gamma, y=x, mean=stat, rstd=stat),
+                     lambda: ops.ln_backward(x, kept, None, stat, gamma, gamma, gamma, dx=x),
+                     lambda: ops.CTensorApplyFunc.Backward(x, kept, x, "relu"), lambda: ops.checkpoint_wgrad(dw, db, x, short)):
+            with pytest.raises(ops.B200Error, match="at most"):
+                call()
