@@ -476,16 +476,21 @@ class Net:
 
     def share_tensors(self):
         """Two output tensors and two error tensors for all layers (each of which keeps what it needs in a checkpoint): layer i
-        reads the one that layer i - 1 wrote and writes the other."""
+        reads the one that layer i - 1 wrote and writes the other.  The net's output may be its next input, and the error at its
+        input the next one at its output: in a net of an odd number of layers, where the first layer would write the tensor
+        that the last one wrote, the last output and the first error are tensors of their own."""
         def shared(count):
             return [torch.empty(max([count(layer) for layer in self.layers[k::2]], default=0), device="cuda") for k in range(2)]
         outs = shared(lambda layer: self.batch * int(np.prod(layer.out_shape)))
         errors = shared(lambda layer: self.batch * int(np.prod(layer.in_shape)))
+        odd = len(self.layers) % 2 == 1
         for i, layer in enumerate(self.layers):
-            layer.H = outs[i % 2][:layer.H.numel()].view(layer.H.shape)
-            name = "delta" if isinstance(layer, NetLayerFunction) else "prev_error"
-            old = getattr(layer, name)
-            setattr(layer, name, errors[i % 2][:old.numel()].view(old.shape))
+            if not (odd and i + 1 == len(self.layers)):
+                layer.H = outs[i % 2][:layer.H.numel()].view(layer.H.shape)
+            if not (odd and i == 0):
+                name = "delta" if isinstance(layer, NetLayerFunction) else "prev_error"
+                old = getattr(layer, name)
+                setattr(layer, name, errors[i % 2][:old.numel()].view(old.shape))
 
     @property
     def parameter_count(self):

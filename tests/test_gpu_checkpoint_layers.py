@@ -280,3 +280,43 @@ def test_first_calls_of_a_process_inside_a_capture(n):
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     r = subprocess.run([sys.executable, "-c", FIRST_CALL.format(root=root, n=n)], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "captured" in r.stdout, r.stdout[-500:] + r.stderr[-2000:]
+
+
+def chain(spec, shape, batch, share=True, checkpoint8=True, **kw):
+    """A net, with or without tensors shared by its layers."""
+    from cuda_cnn_gan_vae_b200.layers import Net
+    keep = Net.share_tensors
+    if not share:
+        Net.share_tensors = lambda self: None
+    try:
+        return Net(shape, batch, spec, seed=3, checkpoint8=checkpoint8, **kw)
+    finally:
+        Net.share_tensors = keep
+
+
+@pytest.mark.parametrize("layers", [2, 3, 4, 5])
+def test_a_net_may_be_fed_its_own_output(ops, layers):
+    """The output handed back as the next input, the error at the input as the next one at the output, for nets of two to five layers
+    that share their tensors: the same bits as with tensors for every layer."""
+    from cuda_cnn_gan_vae_b200.layers import NetLayerFunction, NetLayerLayerNormalization, NetLayerLinear
+    n = 160
+    kinds = [(NetLayerLinear, dict(neurons=n)), (NetLayerLayerNormalization, {}), (NetLayerLinear, dict(neurons=n)),
+             (NetLayerFunction, dict(func="tanh")), (NetLayerLinear, dict(neurons=n))]
+    x, error = torch.randn(9, 1, n, 1, device="cuda"), torch.randn(9, 1, n, 1, device="cuda")
+    results = []
+    for share in (False, True):
+        net = chain(kinds[:layers], (1, n, 1), 9, share)
+        y = x.clone()
+        outs = []
+        for _ in range(3):
+            y = net.Forward(y if share else y.clone())
+            outs.append(y.clone())
+        e = error.clone()
+        for _ in range(3):
+            net.TrainingResetDeltaWeight()
+            e = net.TrainingBackward(e if share else e.clone(), True, need_input_error=True)
+            outs += [e.clone(), net.grads.buffer.clone()]
+        ops.stream_status()
+        results.append(outs)
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
