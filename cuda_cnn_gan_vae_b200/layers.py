@@ -372,6 +372,24 @@ class NetLayerConcatenator(_Layer):
         return self.prev_error_a, self.prev_error_b
 
 
+# The layers of a chain that write an output tensor H and, all but the time embedding, an error tensor of their own
+_CHAINED = (NetLayerConvolution, NetLayerBackConvolution, NetLayerLinear, NetLayerFunction, NetLayerBatchNormalization,
+            NetLayerBatchNormalizationFunction, NetLayerLayerNormalization, NetLayerMaxPooling, NetLayerUpSampling, NetLayerTimeEmbedding)
+
+
+def _error_name(layer):
+    """The attribute that is the error a layer hands down; None: it hands down the tensor it was given."""
+    if isinstance(layer, NetLayerTimeEmbedding):
+        return None
+    return "delta" if isinstance(layer, NetLayerFunction) else "prev_error"
+
+
+def _forgets(layer):
+    """Whether a layer is done with its input when Forward returns: what its backward pass needs it has kept elsewhere."""
+    return getattr(layer, "kept", None) is not None or type(layer) in (NetLayerBatchNormalization, NetLayerBatchNormalizationFunction,
+                                                                      NetLayerMaxPooling, NetLayerUpSampling, NetLayerTimeEmbedding)
+
+
 class AdamCorrections:
     """The two bias corrections of Adam for the current step in device memory, refreshed from the host before a step by a
     16-byte stream-ordered copy.  The copy reads pinned host memory when it executes, and the host may run many steps ahead
@@ -405,9 +423,9 @@ class Net:
         the PeerBuffer (memory every rank maps), and
         TrainingUpdateWeight(fused=True) runs the library's reduce-scatter + Adam + all-gather kernel on `channel`.
         fold: function layers next to a convolution layer are folded into that layer's Forward (see fold_functions).
-        checkpoint8: the Linear, function and layer-normalisation layers keep what their backward passes need in 8 bits.  A net of
-        only such layers then holds two output tensors and two error tensors in all, used in turn by its layers, in place
-        of two for each."""
+        checkpoint8: the Linear, function and layer-normalisation layers keep what their backward passes need in 8 bits, and the
+        tensors that then nobody needs for long are shared (see share_tensors).  Every Forward fills the checkpoints, an
+        answer without a backward pass after it too."""
         self.batch, self.in_shape = batch, tuple(in_shape)
         self.layers, shape = [], tuple(in_shape)
         for cls, kw in spec:
@@ -417,11 +435,21 @@ class Net:
             if checkpoint8 and cls in (NetLayerLinear, NetLayerFunction, NetLayerLayerNormalization):
                 kw = dict(kw, checkpoint8=True)
             layer = cls(shape, batch, **kw)
+            if checkpoint8 and type(layer) in _CHAINED:
+                layer.H = None                              # given back before the next layer is made
+                if _error_name(layer):
+                    setattr(layer, _error_name(layer), None)
             self.layers.append(layer)
             shape = layer.out_shape
         self.out_shape = shape
-        if self.layers and all(getattr(layer, "kept", None) is not None for layer in self.layers):
+        if checkpoint8 or (self.layers and all(getattr(layer, "kept", None) is not None for layer in self.layers)):
             self.share_tensors()
+        for layer in self.layers if checkpoint8 else ():    # what is not shared
+            if type(layer) in _CHAINED:
+                if layer.H is None:
+                    layer.H = torch.empty((batch,) + tuple(layer.out_shape), device="cuda")
+                if _error_name(layer) and getattr(layer, _error_name(layer)) is None:
+                    setattr(layer, _error_name(layer), torch.empty((batch,) + tuple(layer.in_shape), device="cuda"))
         self.fold_functions(fold)
         shapes = {}
         for i, layer in enumerate(self.layers):
@@ -475,22 +503,26 @@ class Net:
                 layer.folded, layer.materialise, next_l.before = "into_next", materialise, layer
 
     def share_tensors(self):
-        """Two output tensors and two error tensors for all layers (each of which keeps what it needs in a checkpoint): layer i
-        reads the one that layer i - 1 wrote and writes the other.  The net's output may be its next input, and the error at its
-        input the next one at its output: in a net of an odd number of layers, where the first layer would write the tensor
-        that the last one wrote, the last output and the first error are tensors of their own."""
-        def shared(count):
-            return [torch.empty(max([count(layer) for layer in self.layers[k::2]], default=0), device="cuda") for k in range(2)]
-        outs = shared(lambda layer: self.batch * int(np.prod(layer.out_shape)))
-        errors = shared(lambda layer: self.batch * int(np.prod(layer.in_shape)))
-        odd = len(self.layers) % 2 == 1
-        for i, layer in enumerate(self.layers):
-            if not (odd and i + 1 == len(self.layers)):
-                layer.H = outs[i % 2][:layer.H.numel()].view(layer.H.shape)
-            if not (odd and i == 0):
-                name = "delta" if isinstance(layer, NetLayerFunction) else "prev_error"
-                old = getattr(layer, name)
-                setattr(layer, name, errors[i % 2][:old.numel()].view(old.shape))
+        """Two output tensors for all layers whose outputs nobody needs once the layer behind has read them -- it keeps a checkpoint, or
+        its backward pass does not look at its input -- and two error tensors for all layers: each layer reads one and writes
+        the other.  What a convolution layer reads stays, as does the net's output, and the error at its input.  (A net
+        that keeps all its layers' inputs in checkpoints shares these two as well where that leaves the output free to be the
+        next input, and the error at the input the next one at the output: an even number of layers, the first of which
+        writes the tensor that the last one did not.)"""
+        layers, last = self.layers, len(self.layers) - 1
+        closed = last % 2 == 1 and all(getattr(layer, "kept", None) is not None for layer in layers)
+        chained = [i for i, layer in enumerate(layers) if type(layer) in _CHAINED]
+        users = [[] for _ in range(4)]                       # of the two output and the two error tensors: layer, attribute, size
+        for i in chained:
+            if closed if i == last else _forgets(layers[i + 1]):
+                users[i % 2].append((layers[i], "H", layers[i].out_shape))
+        backward = [i for i in reversed(chained) if _error_name(layers[i])]
+        for turn, i in enumerate(backward if closed else backward[:-1]):
+            users[2 + turn % 2].append((layers[i], _error_name(layers[i]), layers[i].in_shape))
+        for members in users:
+            room = torch.empty(self.batch * max([int(np.prod(size)) for _, _, size in members], default=0), device="cuda")
+            for layer, name, size in members:
+                setattr(layer, name, room[:self.batch * int(np.prod(size))].view((self.batch,) + tuple(size)))
 
     @property
     def parameter_count(self):

@@ -320,3 +320,66 @@ def test_a_net_may_be_fed_its_own_output(ops, layers):
         results.append(outs)
     for a, b in zip(*results):
         assert torch.equal(a, b)
+
+
+def mixed():
+    """A chain of every kind of layer: convolutions keep their inputs, the others let theirs go (the time embedding hands the error on)."""
+    from cuda_cnn_gan_vae_b200 import layers as l
+    return [(l.NetLayerTimeEmbedding, {}), (l.NetLayerConvolution, dict(kernel_amount=8, kernel_size=3, stride=1, padding=1)),
+            (l.NetLayerLayerNormalization, {}), (l.NetLayerFunction, dict(func="leaky_relu")), (l.NetLayerMaxPooling, dict(pooling=2)),
+            (l.NetLayerTimeEmbedding, {}), (l.NetLayerBatchNormalization, {}), (l.NetLayerFunction, dict(func="tanh")), (l.NetLayerUpSampling, dict(factor=2)),
+            (l.NetLayerBackConvolution, dict(kernel_amount=6, kernel_size=4, stride=2, padding=1)),
+            (l.NetLayerBatchNormalizationFunction, dict(func="leaky_relu")), (l.NetLayerConvolution, dict(kernel_amount=4, kernel_size=3, stride=2, padding=1)),
+            (l.NetLayerFunction, dict(func="sigmoid")), (l.NetLayerLinear, dict(neurons=50)), (l.NetLayerFunction, dict(func="gelu")),
+            (l.NetLayerLayerNormalization, dict(dims=2)), (l.NetLayerLinear, dict(neurons=3))]
+
+
+@pytest.mark.parametrize("start", range(5))
+def test_shared_tensors_of_mixed_nets_change_nothing(ops, start):
+    """Nets that begin with any of the first layers of the chain, two steps each: the same bits as with tensors for every layer."""
+    spec = mixed()
+    shape = (2, 12, 16) if start < 2 else (8, 12, 16)
+    x, error = torch.randn(6, *shape, device="cuda"), torch.randn(6, 1, 3, 1, device="cuda")
+    results = []
+    for share in (False, True):
+        net = chain(spec[start:], shape, 6, share)
+        outs = []
+        for turn in range(2):
+            net.TrainingResetDeltaWeight()
+            y = net.Forward(x * (1 + turn))
+            dx = net.TrainingBackward(error, True, need_input_error=True)
+            outs += [y.clone(), dx.clone(), net.grads.buffer.clone()]
+        ops.stream_status()
+        results.append(outs)
+        if share:
+            names = [n for layer in net.layers for n in ("H", "prev_error", "delta") if getattr(layer, n, None) is not None]
+            assert len({getattr(layer, n).data_ptr() for layer in net.layers for n in ("H", "prev_error", "delta") if getattr(layer, n, None) is not None}) < len(names)
+    for a, b in zip(*results):
+        assert torch.equal(a, b) and torch.isfinite(a).all()
+
+
+def held(make):
+    """What a net's construction leaves allocated and the most it had meanwhile, in bytes."""
+    import gc
+    gc.collect()
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    net = make()
+    return net, torch.cuda.memory_allocated() - before, torch.cuda.max_memory_allocated() - before
+
+
+@pytest.mark.parametrize("norm", ["batch", "layer"])
+def test_checkpoints_save_memory_in_a_discriminator(ops, norm):
+    """Per stage of N values without checkpoints: three outputs and three errors, and xhat of the batch normalisation.  With: the
+    convolution's input and two checkpoints of 33 bytes for 32 values; outputs and errors are the largest stage's, twice each."""
+    from cuda_cnn_gan_vae_b200.nets import dcgan_discriminator
+    net, plain, _ = held(lambda: dcgan_discriminator(64, norm=norm))
+    values = [64 * int(np.prod(layer.out_shape)) * 4 for layer in net.layers[:-2:3]]
+    net, with_checkpoints, most = held(lambda: dcgan_discriminator(64, norm=norm, checkpoint8=True))
+    # saved: outputs of convolution and normalisation and three errors of every stage; held: the shared ones, the checkpoints
+    saved, cost = 5 * sum(values), 4 * max(values) + (33 / 128) * (2 if norm == "layer" else 1) * sum(values)
+    assert with_checkpoints < plain - 0.9 * (saved - cost)
+    # nor is more than that needed while it is made, but for one layer's own tensors
+    assert most < with_checkpoints + 4 * max(values)
