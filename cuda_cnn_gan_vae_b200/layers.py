@@ -117,6 +117,8 @@ class NetLayerLinear(_Layer):
     checkpoint8: the layer keeps its input in 8 bits (ops.Checkpoint8) and forms its weight and bias gradients from that; the
     tensor it was given is not needed after Forward."""
 
+    stores = True       # False: another layer that is given the same input before this one fills the checkpoint of both
+
     def __init__(self, in_shape, batch, neurons, checkpoint8=False):
         self.in_shape, self.batch, self.neurons = tuple(in_shape), batch, neurons
         self.n_in = int(np.prod(in_shape))
@@ -134,10 +136,10 @@ class NetLayerLinear(_Layer):
         self.w["b"].zero_()
 
     def Forward(self, x):
-        if self.kept is not None:
-            self.kept.store(x.view(self.batch, self.n_in))
-        else:
+        if self.kept is None:
             self.x = x
+        elif self.stores:
+            self.kept.store(x.view(self.batch, self.n_in))
         ops.CTensorMath.Mul(self.H, self.w["w"], x.view(self.batch, 1, self.n_in, 1))
         ops.CTensorMath.Add(self.H, self.H, self.w["b"])
         return self.H

@@ -197,12 +197,18 @@ class VAEStep:
 
     def __init__(self, batch, world=1, image=(3, 128, 128), widths=(32, 64, 128, 256), latent=256, kl_speed=1.0, leaky_slope=0.1,
                  checkpoint8=False):
-        """checkpoint8: the two heads keep the features they read in 8 bits for their weight gradients."""
+        """checkpoint8: the two heads keep the features they read in 8 bits, once for both, for their weight gradients; the features
+        themselves then make room for the error that the first head hands down."""
         self.batch, self.world, self.kl_speed = batch, world, kl_speed
         self.encoder = vae_encoder(batch, image, widths, leaky_slope)
         feat = self.encoder.out_shape
         self.mu = Net(feat, batch, [(NetLayerLinear, dict(neurons=latent))], seed=6, checkpoint8=checkpoint8)
         self.logvar = Net(feat, batch, [(NetLayerLinear, dict(neurons=latent))], seed=7, checkpoint8=checkpoint8)
+        if checkpoint8:
+            mu, logvar = self.mu.layers[0], self.logvar.layers[0]
+            logvar.kept, logvar.stores = mu.kept, False         # (mu's Forward comes first)
+            # the encoder ends with a pooling layer, whose backward pass does not look at its output
+            mu.prev_error = self.encoder.layers[-1].H
         self.decoder = vae_decoder(batch, latent, feat, tuple(widths[-2::-1]) + (image[0],), leaky_slope)
         assert self.decoder.out_shape == tuple(image), (self.decoder.out_shape, image)
         self.nets = (self.encoder, self.mu, self.logvar, self.decoder)

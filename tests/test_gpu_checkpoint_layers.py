@@ -383,3 +383,27 @@ def test_checkpoints_save_memory_in_a_discriminator(ops, norm):
     assert with_checkpoints < plain - 0.9 * (saved - cost)
     # nor is more than that needed while it is made, but for one layer's own tensors
     assert most < with_checkpoints + 4 * max(values)
+
+
+def test_vae_step_keeps_its_features_once(ops):
+    """One checkpoint for both heads, and the features' own tensor used again on the way back: less memory than without, and the
+    gradients of every step are those of heads with checkpoints and tensors of their own."""
+    from cuda_cnn_gan_vae_b200.nets import VAEStep
+    args = dict(image=(3, 64, 64), widths=(8, 16, 64), latent=24)
+    _, plain, _ = held(lambda: VAEStep(16, **args))
+    step, with_checkpoints, _ = held(lambda: VAEStep(16, checkpoint8=True, **args))
+    feat, weights = 16 * 64 * 8 * 8 * 4, 2 * 24 * 64 * 8 * 8 * 4         # (the heads' scratch for weight gradients goes too)
+    assert with_checkpoints < plain - weights - 0.7 * feat
+    x, eps = torch.rand(16, 3, 64, 64, device="cuda"), torch.randn(16, 1, 24, 1, device="cuda")
+    apart = VAEStep(16, checkpoint8=True, **args)
+    feat_shape = apart.encoder.out_shape
+    for net in (apart.mu, apart.logvar):
+        head = net.layers[0]
+        head.kept, head.stores = ops.Checkpoint8.empty(16, head.n_in), True
+        head.prev_error = torch.empty((16,) + feat_shape, device="cuda")
+    for turn in range(3):
+        outs = [s(x, eps).clone() for s in (step, apart)]
+        ops.stream_status()
+        assert torch.equal(*outs) and torch.equal(step.feat_error, apart.feat_error)
+        for a, b in zip(step.nets, apart.nets):
+            assert torch.equal(a.grads.buffer, b.grads.buffer) and torch.equal(a.weights.buffer, b.weights.buffer)
