@@ -253,8 +253,8 @@ class NetLayerBatchNormalizationFunction(NetLayerBatchNormalization):
 
 
 class NetLayerLayerNormalization(_Layer):
-    """Layer normalisation: statistics of each sample itself (batch normalisation mixes the samples of a batch, which a gradient
-    penalty per sample or a batch of one does not allow).  dims: how many of the dimensions (Z, Y, X) are normalised together, from
+    """Layer normalisation: statistics of each sample itself (batch normalisation mixes the samples of a batch, and has nothing to
+    normalise by in a batch of one).  dims: how many of the dimensions (Z, Y, X) are normalised together, from
     the last: 3 the whole sample, 2 every plane, 1 every row of X.  No reference counterpart.
 
     checkpoint8: the normalised values are kept in 8 bits for the way back instead of the layer's input, which is not

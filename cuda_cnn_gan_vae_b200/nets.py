@@ -37,8 +37,8 @@ def dcgan_generator(batch, noise=100, base=512, widths=(256, 128, 64, 3), leaky_
 def dcgan_discriminator(batch, image=(3, 64, 64), widths=(64, 128, 256, 512), leaky_slope=0.2, seed=3, fused=False, peer=False, channel=0,
                         norm="batch", checkpoint8=False):
     """image -> 4x4 stride-2 convolutions with batch normalisation and LeakyReLU -> Linear to one logit -> sigmoid.
-    norm="layer": every sample normalised by itself (a discriminator's answer to one image must not depend on the others
-    under a gradient penalty per sample).  checkpoint8: as in Net."""
+    norm="layer": every sample normalised by itself, so that the discriminator's answer to one image does not depend on the others
+    of its batch.  checkpoint8: as in Net."""
     if norm not in ("batch", "layer"):
         raise ops.B200Error(2, "norm must be 'batch' or 'layer'")
     spec = []
@@ -62,8 +62,9 @@ class DCGANStep:
     respect to the logit, formed as in cuda/netmodel/cmodel_basicgan.cu.h:352-376 but on the device)."""
 
     def __init__(self, batch, world=1, widths_g=(256, 128, 64, 3), widths_d=(64, 128, 256, 512), base=512, noise=100, leaky_slope=0.2,
-                 use_graph=True, fused=False, update="fused", overlap=False, lean=True):
-        """update (several ranks): "fused" -- the library's reduce-scatter + Adam + all-gather kernel over NVLink peer memory,
+                 use_graph=True, fused=False, update="fused", overlap=False, lean=True, norm="batch", checkpoint8=False):
+        """norm, checkpoint8: of the discriminator (see dcgan_discriminator).
+        update (several ranks): "fused" -- the library's reduce-scatter + Adam + all-gather kernel over NVLink peer memory,
         one launch per net on the main stream; "nccl" -- an NCCL all-reduce of each gradient arena on a side stream followed
         by the Adam launch.  overlap: the discriminator's exchange on a side stream beside the generator's backward pass
         (measured on 2 GPUs: no gain -- the exchange kernel's CTAs take whole SMs from the backward pass for as long as they
@@ -75,7 +76,8 @@ class DCGANStep:
             from .dp import PeerBuffer
             peer = PeerBuffer(32 << 20)         # one buffer for both nets (weights + gradients of ~6.4 M parameters, with room to spare)
         self.G = dcgan_generator(batch, noise, base, widths_g, leaky_slope, fused=fused, peer=peer, channel=1)
-        self.D = dcgan_discriminator(batch, self.G.out_shape, widths_d, leaky_slope, fused=fused, peer=peer, channel=0)
+        self.D = dcgan_discriminator(batch, self.G.out_shape, widths_d, leaky_slope, fused=fused, peer=peer, channel=0,
+                                     norm=norm, checkpoint8=checkpoint8)
         if lean:    # function layers folded into the convolution behind them do not write an output tensor nobody reads
             self.G.fold_functions(True, materialise=False)
             self.D.fold_functions(True, materialise=False)

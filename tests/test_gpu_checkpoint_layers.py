@@ -407,3 +407,21 @@ def test_vae_step_keeps_its_features_once(ops):
         assert torch.equal(*outs) and torch.equal(step.feat_error, apart.feat_error)
         for a, b in zip(step.nets, apart.nets):
             assert torch.equal(a.grads.buffer, b.grads.buffer) and torch.equal(a.weights.buffer, b.weights.buffer)
+
+
+@pytest.mark.parametrize("norm,checkpoint8", [("layer", False), ("layer", True), ("batch", True)])
+def test_dcgan_step_with_such_a_discriminator(ops, norm, checkpoint8):
+    """Captured and replayed steps leave the weights that eager ones do."""
+    from cuda_cnn_gan_vae_b200.nets import DCGANStep
+    args = dict(widths_g=(32, 16, 8, 3), widths_d=(8, 16, 32, 48), base=64, norm=norm, checkpoint8=checkpoint8)
+    z, labels = torch.randn(8, 1, 100, 1, device="cuda"), torch.ones(8, 1, 1, 1, device="cuda")
+    steps = [DCGANStep(8, use_graph=g, **args) for g in (False, True)]
+    assert (steps[0].D.layers[-1].kept is not None) == checkpoint8
+    assert type(steps[0].D.layers[1]).__name__ == ("NetLayerLayerNormalization" if norm == "layer" else "NetLayerBatchNormalization")
+    for _ in range(5):
+        outs = [s(z, labels).clone() for s in steps]
+        ops.stream_status()
+        assert torch.equal(*outs)
+    assert steps[1].graph is not None
+    for a, b in zip((steps[0].G, steps[0].D), (steps[1].G, steps[1].D)):
+        assert torch.equal(a.weights.buffer, b.weights.buffer) and torch.isfinite(a.weights.buffer).all()
