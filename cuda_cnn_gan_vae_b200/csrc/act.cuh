@@ -1,5 +1,6 @@
 // The neuron functions of the reference (cpu/ctensorapplyfunc.h:128-257: sigmoid and tanh with the argument clamped to +-30,
-// LeakyReLU multiplied in double precision, derivative 1 at zero for ReLU and LeakyReLU) as device functions shared by the
+// LeakyReLU multiplied in double precision, derivative 1 at zero for ReLU and LeakyReLU, for GELU an expression that is not the
+// derivative of its function but 0.5 (1 + tanh u + 0.5 v / cosh^2 u) u', kept as it is) as device functions shared by the
 // element-wise kernels, the operand packs and the epilogue of the tensor-core kernel, so that an activation gives the same
 // bits wherever it is applied.
 #pragma once

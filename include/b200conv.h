@@ -71,7 +71,10 @@ typedef struct b200_conv_geom {
 
 /* Activation codes (netlayer/neuron.cu.h NEURON_FUNCTION_*; scalar definitions
  * cpu/ctensorapplyfunc.h:128-257).  LEAKY_RELU uses the slope given to the call, a double multiplied
- * in double precision as the reference does with its constant 0.1. */
+ * in double precision as the reference does with its constant 0.1.  f' in this file is the reference's ApplyDifferential*.  For
+ * GELU, f(v) = v/2 (1 + tanh u) with u = c (v + 0.044715 v^3), c = 0.7978845608, that is
+ * (1 + tanh u + v/2 / cosh^2 u) u' / 2, which is not the derivative of f (0.399 where that is 0.5, at v = 0); every entry point
+ * that takes a neuron function uses it. */
 enum { B200_ACT_SIGMOID = 0, B200_ACT_RELU = 1, B200_ACT_LEAKY_RELU = 2, B200_ACT_LINEAR = 3,
        B200_ACT_TANH = 4, B200_ACT_GELU = 5 };
 

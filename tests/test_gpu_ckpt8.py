@@ -149,6 +149,25 @@ def test_kept_signs_make_relu_exact(ops):
         assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("n", [200, 203])
+def test_function_backward_of_gelu_is_the_stated_expression(ops, n):
+    """Against (1 + tanh u + v/2 / cosh^2 u) u' / 2 in 64 bits.  In fp32 u is off by at most 4 units of 2^-24 of itself, tanhf and
+    coshf by 2 ulp: tanh u by 4 |u| / cosh^2 u + 4 <= 6 units, 1 / cosh^2 u by 2 (4 |u| + 6) units of itself, which v/2 / cosh^2 u
+    (at most 0.3; 0.3 |u| too) makes 6, the sums and products 4 more: less than 32 units of 1 + |u'| (u' / 2 and its own error
+    of 4 units on at most 2)."""
+    z = torch.from_numpy(np.random.default_rng(n).normal(0, 2, (9, n)).astype(np.float32)).cuda()
+    e = torch.from_numpy(np.random.default_rng(n + 1).normal(0, 1, (9, n)).astype(np.float32)).cuda()
+    c = ops.Checkpoint8.empty(9, n).store(z)
+    v = cu.decode(c.codes.cpu().numpy(), c.exponents.cpu().numpy(), n)
+    k, b = float(np.float32(0.7978845608)), float(np.float32(0.044715))
+    u, du = k * (v + b * v ** 3), k * (1 + 3 * b * v ** 2)
+    want = 0.5 * (1 + np.tanh(u) + 0.5 * v / np.cosh(u) ** 2) * du * wide(e)
+    got = torch.empty_like(z)
+    ops.CTensorApplyFunc.Backward(got, c, e, "gelu")
+    ops.stream_status()
+    cu.within(wide(got), want, 32 * cu.U * (1 + du) * np.abs(wide(e)), "gelu")
+
+
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("func", FUNCTIONS)
 @pytest.mark.parametrize("n", [200, 203])
