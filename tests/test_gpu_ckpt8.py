@@ -347,3 +347,106 @@ def test_wgrad_of_very_many_outputs(ops, n, out, mode):
         assert torch.equal(db.double(), 5 + delta.double().sum(0))
     finally:
         ops.set_precision(ops.TF32X3)
+
+
+# ---- large tensors: every loop of the kernels turns several times -----------------------------------------------------------------
+
+def encode_there(x, keep_sign=False):
+    """ckpt8_util.encode in 64 bits on the GPU (finite values)."""
+    rows, n = x.shape
+    v = torch.nn.functional.pad(x.double(), (0, -n % 32)).view(rows, -1, 32)
+    top = v.abs().amax(2)
+    e = torch.where(top > 0, (torch.frexp(top).exponent - 1).clamp(min=-126), -126)
+    b = e + 127
+    b = b + ((torch.round(torch.ldexp(top, 133 - b)) > 127) & (b < 254)).int()
+    q = torch.round(torch.ldexp(v, (133 - b)[:, :, None])).clamp(-127, 127)
+    if keep_sign:
+        q = torch.where((v < 0) & (q == 0), -1.0, q)
+    return q.to(torch.int8).view(rows, -1), b.to(torch.uint8)
+
+
+# more spans (32 lanes of 16 bytes, or of one value) than four for each warp of 8 x 148 blocks; one long row, rows of whole blocks,
+# rows that end inside a block, rows that start anywhere
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows,n", [(1, 6000001), (2600, 4096), (2601, 4104), (5003, 1021), (160000, 40)])
+def test_large_tensors_bit_for_bit(ops, rows, n, kind):
+    t = getattr(torch, kind)
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    low, high = {"float32": (-140, 120), "bfloat16": (-125, 120), "float16": (-20, 12)}[kind]
+    power = torch.randint(low, high, (rows, -(-n // 32)), device="cuda", generator=g).repeat_interleave(32, dim=1)[:, :n]
+    x = torch.ldexp(torch.randn(rows, n, device="cuda", generator=g, dtype=torch.float64), power).to(t)
+    for keep_sign in (False, True):
+        c = ops.Checkpoint8.empty(rows, n).store(x, keep_sign=keep_sign)
+        codes, exponents = encode_there(x, keep_sign)
+        assert torch.equal(c.codes, codes) and torch.equal(c.exponents, exponents)
+    values = torch.ldexp(codes.double(), (exponents.int() - 133).repeat_interleave(32, dim=1))[:, :n]
+    at = c.load(torch.empty(rows, n, device="cuda"))
+    assert torch.equal(at.double(), values)
+    assert torch.equal(c.load(torch.empty(rows, n, device="cuda", dtype=torch.bfloat16)).double(), values)
+    e = torch.randn(rows, n, device="cuda", generator=g).to(t)
+    for func in ("leaky_relu", "tanh"):
+        want, got = torch.empty(rows, n, device="cuda"), torch.empty_like(e)
+        ops.CTensorApplyFunc.Backward(want, at, e.float(), func, 0.2)
+        ops.CTensorApplyFunc.Backward(got, c, e, func, 0.2)
+        assert torch.equal(got, want.to(t))
+    ops.stream_status()
+
+
+# tiles of 256 x 256 outputs over 74 pairs of SMs, chunks of 2048 rows (bf16) or 1024, a tail of tiles split along the batch:
+# 90 tiles = one round and a split tail; the same with several chunks a tile, ragged and not; 32 tiles in two units of several chunks;
+# one tile in 70 units; 272 tiles = three rounds and a tail that is not split
+LARGE_WGRAD = [(300, 2500, 2100), (2500, 2501, 2090), (2500, 2560, 2304), (8192, 2048, 1024), (9000, 256, 256), (5000, 4103, 4096)]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows,n,out", LARGE_WGRAD)
+def test_wgrad_of_many_tiles_and_chunks(ops, rows, n, out, kind):
+    """First with whole numbers, whose sums (at most 49 rows < 2^24) are exact in any order: a tile, a chunk or a row that is left
+    out or counted twice shows.  Then with any numbers: products are exact, a chunk's additions may truncate (2^-23 of the
+    magnitudes each, rows of the chunk + 64 of them), and the chunks and the units of a split tile (74 at most) are added
+    in fp32."""
+    t = getattr(torch, kind)
+    g = torch.Generator(device="cuda").manual_seed(rows + n)
+    chunk = 2048 if kind == "bfloat16" else 1024
+    for whole in (True, False):
+        if whole:
+            x = torch.randint(-7, 8, (rows, n), device="cuda", generator=g).float()
+            delta = torch.randint(-7, 8, (rows, out), device="cuda", generator=g).to(t)
+        else:
+            x = torch.randn(rows, n, device="cuda", generator=g)
+            delta = torch.randn(rows, out, device="cuda", generator=g).to(t)
+        c = ops.Checkpoint8.empty(rows, n).store(x)
+        v, d = c.load(torch.empty_like(x)).double(), delta.double()
+        assert not whole or torch.equal(v, x.double())
+        want, want_b = d.t() @ v, d.sum(0)
+        steps = (min(rows, chunk) + 64) * 2.0 ** -23 + (rows // chunk + 1 + 74) * cu.U
+        bound, bound_b = (0, 0) if whole else (steps * (d.abs().t() @ v.abs()), (rows + 64) * cu.U * d.abs().sum(0))
+        dw, db = torch.full((out, n), 5.0, device="cuda"), torch.full((out,), -5.0, device="cuda")
+        ops.checkpoint_wgrad(dw, db, delta, c, accumulate=False)
+        ops.stream_status()
+        assert ((dw.double() - want).abs() <= bound).all() and ((db.double() - want_b).abs() <= bound_b).all()
+        first = dw.clone(), db.clone()
+        ops.checkpoint_wgrad(dw, db, delta, c)
+        ops.stream_status()
+        if whole:
+            assert torch.equal(dw, 2 * first[0]) and torch.equal(db, 2 * first[1])
+        else:
+            assert ((dw.double() - 2 * want).abs() <= 2 * bound + 2 * cu.U * want.abs()).all()
+            assert ((db.double() - 2 * want_b).abs() <= 2 * bound_b + 2 * cu.U * want_b.abs()).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_wgrad_empties_its_accumulator(ops, kind):
+    """The tensor core truncates what does not fit 24 bits, so its sums are taken over 2048 rows (1024 in fp16 and fp32) and added to
+    the output.  Sixteen rows add 63441, an odd number: 2048 rows stay below 2^23, where every sum is exact, and so are the
+    multiples of 128 x 63441 that are added then.  One sum over 8192 rows would leave 2^24 behind after half of them, where
+    the odd ones lose their last bit."""
+    rows, n, out = 8192, 2560, 2304
+    delta = torch.full((rows, out), 63.0, device="cuda")
+    delta[::16] = 62.0
+    c = ops.Checkpoint8.empty(rows, n).store(torch.full((rows, n), 63.0, device="cuda"))
+    dw, db = torch.empty(out, n, device="cuda"), torch.empty(out, device="cuda")
+    ops.checkpoint_wgrad(dw, db, delta.to(getattr(torch, kind)), c, accumulate=False)
+    ops.stream_status()
+    assert 63441 == 15 * 63 * 63 + 62 * 63 and 128 * 63441 < 2 ** 23
+    assert (dw == 512 * 63441).all() and (db == 63 * rows - rows // 16).all()

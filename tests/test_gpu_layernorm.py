@@ -360,3 +360,87 @@ def test_large_magnitudes(ops, n, kind):
     cu.within(host(got["mean"]), mu, em, "mean")
     cu.within(host(got["rstd"]), r, er, "rstd")
     cu.within(host(got["y"]), y, ey, "y")
+
+
+# ---- many rows: every loop down the rows turns several times -------------------------------------------------------------------
+
+def close(got, want, bound, name):
+    off = (got.double() - want).abs() - bound
+    assert not torch.isnan(off).any(), name
+    worst = int(off.argmax())
+    assert off.max() <= 0, f"{name}[{worst}]: {got.flatten()[worst]} against {want.flatten()[worst]}, over the bound by {off.max()}"
+
+
+# Rows for a team of the one-pass backward (148 SMs; a team of 32 threads up to 512 values, 64 up to 1024, ... 512 up to 8192, 512
+# threads a block): 13, 11, 16, 17, 17, 28, where its ring has 3 to 8 slots; then rows of two passes in several groups, with both joins
+MANY = [(30000, 100), (12000, 1021), (9000, 2048), (5000, 4099), (2500, 8192), (66000, 33), (150, 9001), (150, 16384), (61, 20001), (40, 65536)]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("checkpoint", [False, True])
+@pytest.mark.parametrize("rows,n", MANY)
+def test_backward_of_many_rows(ops, rows, n, kind, checkpoint):
+    """Errors and normalised values are whole numbers, means and inverse deviations such that both are exact in every type: each
+    product and each sum over the rows (at most 9 rows < 2^24) is exact, so a row that is left out or counted twice shows in
+    dgamma or dbeta.  dx by the bounds of the other sizes."""
+    t = getattr(torch, kind)
+    g = torch.Generator(device="cuda").manual_seed(rows + n)
+    xh = torch.randint(-3, 4, (rows, n), device="cuda", generator=g).float()
+    dy = torch.randint(-3, 4, (rows, n), device="cuda", generator=g).to(t)
+    mean = torch.randint(-2, 3, (rows,), device="cuda", generator=g).float()
+    rstd = torch.exp2(torch.randint(-1, 2, (rows,), device="cuda", generator=g).float())
+    gamma = 1 + 0.3 * torch.randn(n, device="cuda", generator=g)
+    x = (xh / rstd[:, None] + mean[:, None]).to(t)
+    source = ops.Checkpoint8.empty(rows, n).store(xh) if checkpoint else x
+    dgamma, dbeta = torch.full((n,), 7.0, device="cuda"), torch.full((n,), -7.0, device="cuda")
+    dx = ops.ln_backward(dy, source, mean, rstd, gamma, dgamma, dbeta)
+    ops.stream_status()
+    xh, r = xh.double(), rstd.double()[:, None]
+    assert torch.equal(dgamma.double(), 7 + (dy.double() * xh).sum(0))
+    assert torch.equal(dbeta.double(), dy.double().sum(0) - 7)
+    gg = dy.double() * gamma.double()
+    c1, c2 = gg.mean(1, keepdim=True), (gg * xh).mean(1, keepdim=True)
+    want = r * (gg - c1 - xh * c2)
+    # as in ckpt8_util.ln_backward_bounds
+    k, a1, a2 = cu.sum_steps(n), gg.abs().mean(1, keepdim=True), (gg * xh).abs().mean(1, keepdim=True)
+    e = r * ((k + 5) * cu.U * (a1 + xh.abs() * a2) + 5 * cu.U * (gg.abs() + a1 + xh.abs() * a2)) + 2 * cu.U * want.abs()
+    close(dx, want, e + cu.HALF_STEP[kind] * (want.abs() + e) + cu.TINY[kind], "dx")
+    # written in place of what was there, and again, with the same bits
+    other = ops.ln_backward(dy, source, mean, rstd, gamma, dgamma, dbeta, accumulate=False)
+    assert torch.equal(other, dx)
+    assert torch.equal(dgamma.double(), (dy.double() * xh).sum(0)) and torch.equal(dbeta.double(), dy.double().sum(0))
+
+
+# more rows than the grid has teams (24 blocks for each of 148 SMs, of four rows up to 512 values, else of one), then long rows in
+# several groups
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows,n", [(33000, 100), (9000, 1000), (9000, 1021), (3700, 4099), (3600, 9001), (3600, 16384), (150, 20001), (70, 65536), (90, 20000)])
+def test_forward_of_many_rows(ops, rows, n, kind):
+    t = getattr(torch, kind)
+    g = torch.Generator(device="cuda").manual_seed(rows + n)
+    x = ((torch.randn(rows, n, device="cuda", generator=g) + 0.5) * (0.5 + torch.rand(rows, 1, device="cuda", generator=g))).to(t)
+    gamma, beta = 1 + 0.3 * torch.randn(n, device="cuda", generator=g), 0.3 * torch.randn(n, device="cuda", generator=g)
+    c = ops.Checkpoint8.empty(rows, n)
+    got = ops.ln_forward(x, gamma, beta, 1e-5, checkpoint=c)
+    ops.stream_status()
+    plain = ops.ln_forward(x, gamma, beta, 1e-5)
+    assert all(torch.equal(got[name], plain[name]) for name in got)
+    xd = x.double()
+    var, mu = torch.var_mean(xd, 1, correction=0)
+    r = 1 / (var + float(np.float32(1e-5))).sqrt()
+    # as in ckpt8_util.ln_forward_bounds
+    k = cu.sum_steps(n)
+    m = (k + 2) * cu.U * xd.abs().mean(1)
+    rel = 0.5 * ((k + 4) * cu.U + (m * r) ** 2) + 3 * cu.U
+    close(got["mean"], mu, m + cu.U * mu.abs(), "mean")
+    close(got["rstd"], r, r * rel, "rstd")
+    xh = (xd - mu[:, None]) * r[:, None]
+    del xd
+    e = xh.abs() * (rel + 3 * cu.U)[:, None] + (m * r)[:, None] * 1.01
+    kept = c.load(torch.empty(rows, n, device="cuda"))
+    step = torch.exp2(c.exponents.double() - 133).repeat_interleave(32, dim=1)[:, :n]
+    close(kept, xh, 0.5 * step + e, "kept")
+    del step, kept
+    y = xh * gamma.double() + beta.double()
+    e = gamma.double().abs() * e + 2 * cu.U * ((gamma.double() * xh).abs() + y.abs())
+    close(got["y"], y, e + cu.HALF_STEP[kind] * (y.abs() + e) + cu.TINY[kind], "y")
