@@ -450,3 +450,23 @@ def test_wgrad_empties_its_accumulator(ops, kind):
     ops.stream_status()
     assert 63441 == 15 * 63 * 63 + 62 * 63 and 128 * 63441 < 2 ** 23
     assert (dw == 512 * 63441).all() and (db == 63 * rows - rows // 16).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows,n,out,launches", [(8192, 2048, 1024, 3000), (2500, 2501, 2090, 600), (200, 1000, 700, 1000)])
+def test_wgrad_reads_every_stage_in_its_turn(ops, rows, n, out, launches, kind):
+    """Three sets of whole numbers in turn, thousands of launches: a slot of a ring that is read before it is filled, or filled again
+    before it is read, holds other rows' values or another set's, and shows."""
+    sets = []
+    for k in range(3):
+        x = torch.randint(-7, 8, (rows, n), device="cuda").float()
+        delta = torch.randint(-7, 8, (rows, out), device="cuda").to(getattr(torch, kind))
+        want = (delta.double().t() @ x.double()).float()
+        sets.append((delta, ops.Checkpoint8.empty(rows, n).store(x), want, delta.double().sum(0).float()))
+    dw, db, wrong = torch.empty(out, n, device="cuda"), torch.empty(out, device="cuda"), torch.zeros((), dtype=torch.int64, device="cuda")
+    for turn in range(launches):
+        delta, c, want, want_b = sets[turn % 3]
+        ops.checkpoint_wgrad(dw, db, delta, c, accumulate=False)
+        wrong += (dw != want).sum() + (db != want_b).sum()
+    ops.stream_status()
+    assert int(wrong) == 0
