@@ -654,7 +654,9 @@ __global__ void __launch_bounds__(kLnBlock, 1) ln_backward_rows_kernel(const __g
             if (row + 2ll * step < p.rows) next_exp = *exp_next;
         }
         if (row + step < p.rows) ahead(row + step);
-        // after the barrier in here every thread has read the slot and written its exponents
+        // after the barrier in here every thread has read the slot and written its exponents; the fence orders its reads and the copy
+        // that then refills the slot (no time on any of the sizes measured)
+        ptx::fence_proxy_async();
         const float2 s = team_totals<TEAM>(make_float2(s1.x + s1.y, s2.x + s2.y), scratch[team][turn], 1 + team);
         if (TEAM == 32) __syncwarp();
         if (t == 0 && row + (long long)depth * step < p.rows) issue(row + depth * step, slot);

@@ -444,3 +444,29 @@ def test_forward_of_many_rows(ops, rows, n, kind):
     y = xh * gamma.double() + beta.double()
     e = gamma.double().abs() * e + 2 * cu.U * ((gamma.double() * xh).abs() + y.abs())
     close(got["y"], y, e + cu.HALF_STEP[kind] * (y.abs() + e) + cu.TINY[kind], "y")
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("checkpoint", [False, True])
+@pytest.mark.parametrize("rows,n", [(9000, 100), (9000, 1021), (6000, 2048), (2500, 8192)])
+def test_backward_reads_every_row_in_its_turn(ops, rows, n, kind, checkpoint):
+    """Three sets of whole numbers in turn, hundreds of launches: a slot of a team's ring that is read before it is filled, or filled again
+    before it is read, holds another row's values, and shows."""
+    t, sets = getattr(torch, kind), []
+    for k in range(3):
+        g = torch.Generator(device="cuda").manual_seed(k)
+        xh = torch.randint(-3, 4, (rows, n), device="cuda", generator=g).float()
+        dy = torch.randint(-3, 4, (rows, n), device="cuda", generator=g).to(t)
+        gamma = torch.randint(1, 4, (n,), device="cuda", generator=g).float()
+        sets.append((dy, ops.Checkpoint8.empty(rows, n).store(xh) if checkpoint else xh.to(t), gamma, (dy.double() * xh.double()).sum(0).float(),
+                     dy.double().sum(0).float()))
+    mean, rstd = torch.zeros(rows, device="cuda"), torch.ones(rows, device="cuda")
+    dg, db, dx = torch.empty(n, device="cuda"), torch.empty(n, device="cuda"), torch.empty(rows, n, device="cuda", dtype=t)
+    first = [ops.ln_backward(s[0], s[1], mean, rstd, s[2], dg, db, accumulate=False) for s in sets]
+    wrong = torch.zeros((), dtype=torch.int64, device="cuda")
+    for turn in range(300):
+        dy, source, gamma, want_g, want_b = sets[turn % 3]
+        ops.ln_backward(dy, source, mean, rstd, gamma, dg, db, accumulate=False, dx=dx)
+        wrong += (dg != want_g).sum() + (db != want_b).sum() + (dx != first[turn % 3]).sum()
+    ops.stream_status()
+    assert int(wrong) == 0
