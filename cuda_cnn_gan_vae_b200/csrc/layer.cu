@@ -411,6 +411,13 @@ int b200_conv_layer_forward_fused(b200_conv_layer *l, float *out, const float *i
     return layer_forward(l, out, input, kernel, bias, fusion, stream);
 }
 
+int b200_conv_layer_forget_error(b200_conv_layer *l)
+{
+    if (!l) return fail(B200_E_ARG, "null argument");
+    l->er_valid = 0;
+    return B200_OK;
+}
+
 int b200_conv_layer_backward(b200_conv_layer *l, float *input_delta, float *dkernel, float *dbias, int accumulate,
                              const float *output_delta, const float *input, const float *kernel, void *stream)
 {

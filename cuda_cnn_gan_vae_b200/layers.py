@@ -100,6 +100,8 @@ class NetLayerConvolution(_Layer):
                           self.g["kernel"] if create_delta_weight else None,
                           self.g["bias"] if create_delta_weight else None,
                           delta, self.x, self.w["kernel"], accumulate=True)
+        if create_delta_weight and not need_prev:
+            self.ctx.forget_error()         # the next error comes in the same tensor, and is another one
         return self.prev_error if need_prev else None
 
 

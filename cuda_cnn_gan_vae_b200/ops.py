@@ -679,6 +679,10 @@ class ConvLayer:
                                                _ptr(dbias) if dbias is not None else None, int(accumulate),
                                                _ptr(output_delta), _ptr(inp), _ptr(kernel), _stream()))
 
+    def forget_error(self):
+        """The next backward call packs its output error anew, even if it is the tensor of the weights-only call before it."""
+        _check(load().b200_conv_layer_forget_error(self._h))
+
     def close(self):
         if self._h:
             load().b200_conv_layer_destroy(self._h)

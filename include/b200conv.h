@@ -201,6 +201,10 @@ int b200_conv_layers_prepack(b200_conv_layer *const *layers, const float *const 
 int b200_conv_layer_backward(b200_conv_layer *layer, float *input_delta, float *dkernel, float *dbias, int accumulate,
                              const float *output_delta, const float *input, const float *kernel, void *stream);
 
+/* Host-side note only: the backward call that follows packs its output error itself, whatever the one before it was given.  For
+ * callers that reuse one tensor for the output errors of several backward calls without a forward call between them. */
+int b200_conv_layer_forget_error(b200_conv_layer *layer);
+
 /* Allocation-free form of b200_conv_wgrad_batch (no counterpart in the reference, which allocates
  * its per-sample gradient tensors up front in the layer objects).  For callers that must not allocate
  * device memory where they call the library: hosts that hand out all device memory from their own pool

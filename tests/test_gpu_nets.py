@@ -355,3 +355,25 @@ def test_separable_gan_iteration_matches_twin(ops, port):
                 tol = 2.1 * speed * 2 if noise_gradient else 0.01 * speed
                 assert np.max(np.abs(got - want)) <= tol, (type(layer).__name__, name, np.max(np.abs(got - want)))
     assert keep is not None
+
+
+@pytest.mark.parametrize("first", ["convolution", "transposed"])
+def test_a_second_error_without_a_forward_pass_between(ops, first):
+    """Gradients from one error, then the error at the input from another (a discriminator that judges, then teaches), one forward
+    pass for both: the second backward pass must not find anything of the first in the layers."""
+    from cuda_cnn_gan_vae_b200 import layers as l
+    cls = l.NetLayerConvolution if first == "convolution" else l.NetLayerBackConvolution
+    spec = [(cls, dict(kernel_amount=40, kernel_size=4, stride=2, padding=1)), (l.NetLayerFunction, dict(func="leaky_relu")),
+            (l.NetLayerLinear, dict(neurons=1))]
+    x = torch.randn(8, 32, 16, 16, device="cuda")
+    one, two = torch.randn(8, 1, 1, 1, device="cuda"), torch.randn(8, 1, 1, 1, device="cuda")
+    answers = []
+    for both in (False, True):
+        net = l.Net((32, 16, 16), 8, spec, seed=1)
+        net.TrainingResetDeltaWeight()
+        net.Forward(x)
+        if both:
+            net.TrainingBackward(one, True)
+        answers.append(net.TrainingBackward(two, False, need_input_error=True).clone())
+    ops.stream_status()
+    assert torch.equal(*answers)
