@@ -362,7 +362,8 @@ int b200_ln_backward(void *dx, float *dgamma, float *dbeta, const void *dy, cons
  * [rows][blocks] bytes, blocks = ceil(n / 32): 33 bytes for 32 values.  b is the exponent field of the block's largest magnitude
  * (at least 1), one more where that value would round to 128 (not past 254, where it saturates at 127); q is rounded to
  * nearest, ties to even.  A value is off by at most half a step, 1/127 of the largest magnitude of its block (a whole step where
- * it saturates).  A block that holds an infinity or a NaN reads as NaN.  keep_sign != 0: a negative value never gets q = 0
+ * it saturates; in a block whose largest magnitude is below 2^-126 the step is 2^-132 all the same, and half of it may be all
+ * there is: values up to 2^-133 read as 0).  A block that holds an infinity or a NaN reads as NaN.  keep_sign != 0: a negative value never gets q = 0
  * but -1 (off by less than a step), so that the derivatives of ReLU and LeakyReLU at the kept values are those at the tensor's
  * in every block of finite values. */
 int b200_ckpt8_store(int8_t *codes, uint8_t *exponents, const void *x, int type, int rows, size_t n, size_t x_pitch, int keep_sign,

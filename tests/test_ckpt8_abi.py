@@ -102,3 +102,13 @@ def test_sizes_beyond_the_interface_are_refused_and_not_cut_to_32_bits(monkeypat
                      lambda: ops.CTensorApplyFunc.Backward(x, kept, x, "relu"), lambda: ops.checkpoint_wgrad(dw, db, x, short)):
             with pytest.raises(ops.B200Error, match="at most"):
                 call()
+
+
+def test_blocks_of_subnormal_numbers_keep_half_a_step_and_no_more():
+    """Below 2^-126 the step stays 2^-132: off by 2^-133 at most, which for the smallest numbers is all of them."""
+    x = np.zeros((3, 32), np.float32)
+    x[0, 0], x[1, 3], x[2, :] = 2.0 ** -149, 2.0 ** -133, np.float32(2.0 ** -126) * (np.arange(32, dtype=np.float32) / 32)
+    codes, exponents = cu.encode(x)
+    v = cu.decode(codes, exponents, 32)
+    assert (exponents == 1).all() and not v[:2].any()
+    assert (np.abs(v - x.astype(np.float64)) <= 2.0 ** -133).all()
