@@ -12,8 +12,8 @@ namespace b200 {
 // bytes, or one value where the rows cannot be read in 16-byte pieces); a block's lanes find its largest magnitude by shuffles.  All
 // loads of the kSpans spans are under way before the first is used.  A dense tensor whose rows are whole blocks is one long
 // row, so the division that finds a span's row is left to ragged ones.
-// Measured on 128 x 524288 fp32 values: store 66 us (5.1 TB/s; 90 us with conversion instructions, clamps and two factors
-// for every code), load 55 us (6.1 TB/s), backward of LeakyReLU 92 us (6.6 TB/s).
+// Measured on 128 x 524288 fp32 values: store 63 us (5.4 TB/s; 90 us with conversion instructions, clamps and two factors
+// for every code), load 53 us (6.4 TB/s), backward of LeakyReLU 91 us (6.7 TB/s).
 constexpr int kSpans = 4;
 
 struct CkptShape {

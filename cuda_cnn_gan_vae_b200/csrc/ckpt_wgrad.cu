@@ -82,10 +82,11 @@ __global__ void __launch_bounds__(256) ckpt8_wgrad_simt_kernel(float *dweight, f
 //   * The grid is one pair per two SMs.  Whole tiles go round the pairs; what is left over (or everything, where there are
 //     fewer tiles than pairs) is split along the batch into units that write partial tiles, joined by a second
 //     kernel in the order of the units.  No atomics: the result does not depend on scheduling.
-// Measured at 8192 rows, 4096 x 4096, inputs from memory: bf16 264 us = 1.04 PFLOP/s (302 us after a second of nothing else, when the
-// power limit holds the clock at 1.55 GHz; L2 prefetches ahead of the loads changed nothing), fp16 497, fp32 782; the tensor pipe
-// is active half the time in bf16, the converter warps issue in 60 % of the cycles, and without their stores (199 us) or without the
-// products (199 us) it is no faster than shared memory and the two together allow.
+// Measured at 8192 rows, 4096 x 4096, a single pass with inputs from memory: bf16 272 us = 1.01 PFLOP/s (303 us after a second of
+// nothing else, when the power limit holds the clock at 1.55 GHz; L2 prefetches ahead of the loads changed nothing), fp16 537, fp32
+// 859; six passes in a row 269, 520 and 829 each.  The tensor pipe is active half the time in bf16, the converter warps issue in
+// 58 % of the cycles, and without their stores (199 us of 264 at the time) or without the products (199 too) it is no faster than shared memory and
+// the two together allow.
 constexpr int kPairTile = 256;                     // outputs of a pair in both directions
 constexpr int kEpilogueWarps = 4, kConverterWarps = 16, kGroupWarps = 4, kGroups = kConverterWarps / kGroupWarps;
 constexpr int kConverters = kConverterWarps * 32;
