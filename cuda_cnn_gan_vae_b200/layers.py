@@ -165,7 +165,8 @@ class NetLayerFunction(_Layer):
     delta = f'(layer input) * error, which TrainingBackward hands to the previous layer.
 
     checkpoint8: the layer keeps its input in 8 bits, signs kept, so that the errors below ReLU and LeakyReLU are those of the
-    tensor itself (in a block of 32 with an infinity or a NaN they are NaN) and the other functions' are taken at the kept values.  Such a layer is not folded into a convolution layer."""
+    tensor itself (in a block of 32 with an infinity or a NaN they are NaN) and the other functions' are taken at the kept values.
+    Such a layer is not folded into a convolution layer."""
 
     # folded = "into_next": the convolution layer behind applies the function while it packs its input (Forward here only
     # remembers its input; H is written by that layer when `materialise` is set); folded = "into_prev": the convolution layer
